@@ -23,7 +23,10 @@ EXTRA = {"ncf_score.hip": ["-mllvm", "-amdgpu-mfma-vgpr-form"]}
 HIPCC = os.environ.get("HIPCC", "/opt/rocm/bin/hipcc")
 ARCH = "gfx950"
 CFLAGS = ["--offload-arch=" + ARCH, "-O3", "-fPIC", "-std=c++17", "-I" + INCLUDE, "-I" + HERE,
-          "-Wno-unused-result"]
+          "-Wno-unused-result",
+          # no packed fp32 (v_pk_add/mul/fma_f32): some of their forms have given wrong results on
+          # MI355X; the scalar forms round alike
+          "-Xclang", "-target-feature", "-Xclang", "-packed-fp32-ops"]
 
 
 HASH_MARK = b"NCF_SRC_SHA256="
