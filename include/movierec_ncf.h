@@ -509,6 +509,28 @@ int ncf_score_topk(const ncf_shape_t* shape, const ncf_model_t* model, const int
                    int32_t k, int32_t precision, int32_t* top_items, float* top_scores, void* ws, size_t ws_bytes,
                    void* stream);
 
+/* Catalogue operators: a user's logits over all items, drawing items from them, and learning them
+ * from a teacher (movierec/catalogue.py).  Matrices are row-major with their last dimension dense;
+ * ld* is the distance between rows in elements.  Element types: */
+#define NCF_F32 0
+#define NCF_BF16 1
+#define NCF_F16 2
+
+/* Block-scaled 8-bit operands (e4m3, largest value 448).  scale = max(max|x| / 448, 2^-126) of the
+ * 128 consecutive values of a row that share it (tile == 0: scale[rows][ceil(cols/128)]) or of a
+ * 128 x 128 tile (tile != 0: scale[ceil(rows/128)][ceil(cols/128)]); q = e4m3(x / scale), rounded to
+ * nearest even.  A block that holds a NaN or an infinity has that scale (its values: NaN, and 0 for
+ * the finite ones beside an infinity).  Bytes past cols in a row of q are not written. */
+int ncf_quantize_blocks(const void* x, int32_t dtype, int64_t rows, int64_t cols, int64_t ld, int32_t tile, void* q,
+                        int64_t q_ld, float* scale, void* stream);
+/* y[m][n] = bias[n] + sum over blocks j of a_scale[m][j] b_scale[n][j] (sum over the block of
+ * a[m][k] b[n][k]), in fp32, rounded once to out_dtype.  a: m x k, b: n x k (e4m3, any alignment);
+ * a_scale[m][ceil(k/128)]; b_scale the same of n rows, or [ceil(n/128)][ceil(k/128)] with
+ * b_tile != 0; bias[n] or NULL. */
+int ncf_matmul_blocks(const void* a, int64_t a_ld, const float* a_scale, const void* b, int64_t b_ld,
+                      const float* b_scale, int32_t b_tile, const float* bias, int64_t m, int64_t n, int64_t k,
+                      int32_t out_dtype, void* y, int64_t y_ld, void* stream);
+
 /* On-device negative sampling + batch assembly.  Replaces
  * MovieLensDataGenerator.__getitem__ (data_pipeline.py:115-150): for the n_pos positives
  * order[first .. first+n_pos) (indexes into pos_users/pos_items, the epoch's shuffled order,

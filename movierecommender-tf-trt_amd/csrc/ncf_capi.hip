@@ -1474,6 +1474,63 @@ int ncf_lazy_flush(const ncf_shape_t* s, ncf_model_t* model, ncf_optim_t* optim,
 
 // ------------------------------------------------------------ negative sampling
 
+// ------------------------------------------------------------------ catalogue operators
+
+// a matrix of rows x cols with rows ld apart, of at most 2^31 - 129 columns (a column index and its
+// block's end fit 32 bits)
+static int check_matrix(const char* name, const void* p, int64_t rows, int64_t cols, int64_t ld) {
+    if (!p) return fail(NCF_EINVAL, "%s is NULL", name);
+    if (cols < 1 || cols > INT32_MAX - 128) return fail(NCF_EINVAL, "%s: %lld columns", name, (long long)cols);
+    if (rows > 1 && ld < 0) return fail(NCF_EINVAL, "%s: rows %lld elements apart", name, (long long)ld);
+    return 0;
+}
+// an output: its rows may not overlap
+static int check_output(const char* name, const void* p, int64_t rows, int64_t cols, int64_t ld) {
+    if (int r = check_matrix(name, p, rows, cols, ld)) return r;
+    if (rows > 1 && ld < cols) return fail(NCF_EINVAL, "%s: rows of %lld elements only %lld apart", name,
+                                           (long long)cols, (long long)ld);
+    return 0;
+}
+static int check_dtype(int dtype) {
+    if (dtype != NCF_F32 && dtype != NCF_BF16 && dtype != NCF_F16)
+        return fail(NCF_EINVAL, "unknown element type %d", dtype);
+    return 0;
+}
+
+int ncf_quantize_blocks(const void* x, int32_t dtype, int64_t rows, int64_t cols, int64_t ld, int32_t tile, void* q,
+                        int64_t q_ld, float* scale, void* stream) {
+    if (int r = check_dtype(dtype)) return r;
+    if (rows < 0) return fail(NCF_EINVAL, "rows must be >= 0, got %lld", (long long)rows);
+    if (rows == 0) return 0;
+    if (int r = check_matrix("x", x, rows, cols, ld)) return r;
+    if (int r = check_output("q", q, rows, cols, q_ld)) return r;
+    if (!scale) return fail(NCF_EINVAL, "scale is NULL");
+    if ((rows + 127) / 128 > INT32_MAX / ((cols + 127) / 128))
+        return fail(NCF_EINVAL, "%lld x %lld is too large a matrix", (long long)rows, (long long)cols);
+    return hip_check(ncf::launch_quantize(x, dtype, rows, (int)cols, ld, tile != 0, static_cast<uint8_t*>(q), q_ld,
+                                          scale, (hipStream_t)stream),
+                     "ncf_quantize_blocks");
+}
+
+int ncf_matmul_blocks(const void* a, int64_t a_ld, const float* a_scale, const void* b, int64_t b_ld,
+                      const float* b_scale, int32_t b_tile, const float* bias, int64_t m, int64_t n, int64_t k,
+                      int32_t out_dtype, void* y, int64_t y_ld, void* stream) {
+    if (int r = check_dtype(out_dtype)) return r;
+    if (m < 0 || n < 0) return fail(NCF_EINVAL, "m and n must be >= 0, got %lld, %lld", (long long)m, (long long)n);
+    if (m == 0 || n == 0) return 0;
+    if (int r = check_matrix("a", a, m, k, a_ld)) return r;
+    if (int r = check_matrix("b", b, n, k, b_ld)) return r;
+    if (int r = check_output("y", y, m, n, y_ld)) return r;
+    if (!a_scale || !b_scale) return fail(NCF_EINVAL, "a scale is NULL");
+    // one workgroup for 16 rows x 64 columns is the finest grid of any variant
+    if ((m + 15) / 16 > INT32_MAX / ((n + 15) / 16))
+        return fail(NCF_EINVAL, "%lld x %lld is too large a product", (long long)m, (long long)n);
+    return hip_check(ncf::launch_matmul_blocks(static_cast<const uint8_t*>(a), a_ld, a_scale,
+                                               static_cast<const uint8_t*>(b), b_ld, b_scale, b_tile != 0, bias, m, n,
+                                               (int)k, out_dtype, y, y_ld, (hipStream_t)stream),
+                     "ncf_matmul_blocks");
+}
+
 int ncf_sample_batch(const ncf_sampler_data_t* d, const int32_t* order, int64_t first, int32_t n_pos, int32_t negs,
                      uint64_t seed, uint64_t stream_id, int32_t* x_user, int32_t* x_item, float* labels, int32_t* err,
                      void* stream) {

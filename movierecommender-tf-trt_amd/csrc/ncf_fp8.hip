@@ -1,0 +1,319 @@
+// Block-scaled 8-bit operands: the quantiser and the product that scores users against a catalogue.
+//
+// An operand is held as e4m3 values q with one fp32 scale s per 128 consecutive values of a row (or
+// per 128 x 128 tile): x ~ s q, s = max(max|x| / 448, 2^-126), q = e4m3(x / s), both roundings to
+// nearest even.  The product is
+//     y[m][n] = bias[n] + sum_j sa[m][j] sb[n][j] (sum over block j of qa[m][k] qb[n][k]),
+// a block's sum on MFMA from a zero accumulator, then added, scaled, to the fp32 total.  Two forms of
+// the block's sum, by the output's type:
+//   fp32 outputs    the e4m3 values widened to fp16 (exact) on v_mfma_f32_16x16x32_f16: products and
+//                   sums in fp32 (relative error of a random 128-block 9e-9)
+//   16-bit outputs  v_mfma_f32_16x16x128_f8f6f4, twice the rate.  It aligns the products of each 8
+//                   neighbouring k to the largest and drops what lies more than 13 binary places
+//                   below its exponent (measured: 448 * 448 + 4 gives 448 * 448; a random 128-block
+//                   is off by 1.5e-5) — below half a step of bf16 (2^-9) and fp16 (2^-12) but not of
+//                   fp32.  v_mfma_f32_16x16x32_fp8_fp8 drops the same.
+//
+// The reference scores one user against a list of items (movierec/trt_client.py:43-57).
+
+#include <cmath>
+#include <type_traits>
+
+#include "ncf_common.h"
+#include "ncf_internal.h"
+#include "ncf_types.h"
+
+namespace ncf {
+
+constexpr int kScaleBlock = 128;
+constexpr float kE4m3Max = 448.0f;
+constexpr float kMinScale = 0x1p-126f;  // the smallest normal number: a block of zeros divides by it
+
+// ----------------------------------------------------------------------------- quantiser
+
+template <typename T>
+__device__ __forceinline__ vf32x4 load4(const T* p, int valid) {
+    vf32x4 r = {0.0f, 0.0f, 0.0f, 0.0f};
+    if (valid >= 4) {
+        typedef T v4 __attribute__((ext_vector_type(4), aligned(sizeof(T))));
+        const v4 x = *reinterpret_cast<const v4*>(p);
+#pragma unroll
+        for (int e = 0; e < 4; ++e) r[e] = (float)x[e];
+    } else {
+#pragma unroll
+        for (int e = 0; e < 3; ++e)
+            if (e < valid) r[e] = (float)p[e];
+    }
+    return r;
+}
+
+// the largest magnitude as bits: above every finite number stand infinity, then NaN, so both stay
+__device__ __forceinline__ uint32_t mag4(vf32x4 x) {
+    uint32_t m = 0;
+#pragma unroll
+    for (int e = 0; e < 4; ++e) m = max(m, __float_as_uint(x[e]) & 0x7fffffffu);
+    return m;
+}
+
+// a NaN among the values makes the scale NaN (fmaxf would drop it)
+__device__ __forceinline__ float scale_of(uint32_t mag) {
+    const float a = __uint_as_float(mag) / kE4m3Max;
+    return a < kMinScale ? kMinScale : a;
+}
+
+__device__ __forceinline__ void store_q4(uint8_t* q, vf32x4 x, float s, int valid) {
+    int w = 0;
+    w = __builtin_amdgcn_cvt_pk_fp8_f32(x[0] / s, x[1] / s, w, false);
+    w = __builtin_amdgcn_cvt_pk_fp8_f32(x[2] / s, x[3] / s, w, true);
+    if (valid >= 4) {
+        typedef int iu __attribute__((aligned(1)));
+        *reinterpret_cast<iu*>(q) = w;
+    } else {
+#pragma unroll
+        for (int e = 0; e < 3; ++e)
+            if (e < valid) q[e] = (uint8_t)(w >> (8 * e));
+    }
+}
+
+// One scale per 128 values of a row: 32 lanes hold a block, four values each.
+template <typename T>
+__global__ __launch_bounds__(kBlock) void k_quantize_rows(const T* __restrict__ x, int64_t ld, int64_t blocks, int kb,
+                                                          int cols, uint8_t* __restrict__ q, int64_t q_ld,
+                                                          float* __restrict__ scale) {
+    const int l = threadIdx.x & 31;
+    const int64_t step = (int64_t)gridDim.x * (kBlock / 32);
+    for (int64_t b = (int64_t)blockIdx.x * (kBlock / 32) + (threadIdx.x >> 5); b < blocks; b += step) {
+        const int64_t row = b / kb;
+        const int c = (int)(b - row * kb) * kScaleBlock + 4 * l;
+        const vf32x4 v = load4(x + row * ld + c, cols - c);
+        uint32_t m = mag4(v);
+#pragma unroll
+        for (int d = 16; d >= 1; d >>= 1) m = max(m, (uint32_t)__shfl_xor((int)m, d, 32));
+        const float s = scale_of(m);
+        if (l == 0) scale[b] = s;
+        store_q4(q + row * q_ld + c, v, s, cols - c);
+    }
+}
+
+// One scale per 128 x 128 tile: a workgroup holds the tile in registers.
+template <typename T>
+__global__ __launch_bounds__(kBlock) void k_quantize_tiles(const T* __restrict__ x, int64_t ld, int64_t rows, int kb,
+                                                           int cols, uint8_t* __restrict__ q, int64_t q_ld,
+                                                           float* __restrict__ scale) {
+    __shared__ uint32_t red[kBlock / 64];
+    const int64_t rb = blockIdx.x / kb;
+    const int c = (int)(blockIdx.x - rb * kb) * kScaleBlock + 4 * (threadIdx.x & 31);
+    const int64_t r0 = rb * kScaleBlock + (threadIdx.x >> 5);
+    vf32x4 v[16];
+    uint32_t m = 0;
+#pragma unroll
+    for (int i = 0; i < 16; ++i) {
+        const int64_t row = r0 + 8 * i;
+        v[i] = load4(x + (row < rows ? row : 0) * ld + c, row < rows ? cols - c : 0);
+        m = max(m, mag4(v[i]));
+    }
+#pragma unroll
+    for (int d = 32; d >= 1; d >>= 1) m = max(m, (uint32_t)__shfl_xor((int)m, d, 64));
+    if ((threadIdx.x & 63) == 0) red[threadIdx.x >> 6] = m;
+    __syncthreads();
+    const float s = scale_of(max(max(red[0], red[1]), max(red[2], red[3])));
+    if (threadIdx.x == 0) scale[blockIdx.x] = s;
+#pragma unroll
+    for (int i = 0; i < 16; ++i) {
+        const int64_t row = r0 + 8 * i;
+        if (row < rows) store_q4(q + row * q_ld + c, v[i], s, cols - c);
+    }
+}
+
+template <typename T>
+static hipError_t quantize_t(const T* x, int64_t rows, int cols, int64_t ld, int tile, uint8_t* q, int64_t q_ld,
+                             float* scale, hipStream_t st) {
+    const int kb = (cols + kScaleBlock - 1) / kScaleBlock;
+    if (tile) {
+        const int64_t grid = (rows + kScaleBlock - 1) / kScaleBlock * kb;
+        launch(k_quantize_tiles<T>, dim3((unsigned)grid), kBlock, 0, st, x, ld, rows, kb, cols, q, q_ld, scale);
+    } else {
+        const int64_t blocks = rows * kb;
+        int64_t grid = (blocks + kBlock / 32 - 1) / (kBlock / 32);
+        if (grid > 256 * 64) grid = 256 * 64;
+        launch(k_quantize_rows<T>, dim3((unsigned)grid), kBlock, 0, st, x, ld, blocks, kb, cols, q, q_ld, scale);
+    }
+    return hipGetLastError();
+}
+
+hipError_t launch_quantize(const void* x, int dtype, int64_t rows, int cols, int64_t ld, int tile, uint8_t* q,
+                           int64_t q_ld, float* scale, hipStream_t st) {
+    if (rows <= 0) return hipSuccess;
+    if (dtype == NCF_F32)
+        return quantize_t(static_cast<const float*>(x), rows, cols, ld, tile, q, q_ld, scale, st);
+    if (dtype == NCF_BF16)
+        return quantize_t(static_cast<const __bf16*>(x), rows, cols, ld, tile, q, q_ld, scale, st);
+    return quantize_t(static_cast<const _Float16*>(x), rows, cols, ld, tile, q, q_ld, scale, st);
+}
+
+// ----------------------------------------------------------------------------- product
+
+typedef int mi32x8 __attribute__((ext_vector_type(8)));
+
+typedef _Float16 mf16x8 __attribute__((ext_vector_type(8)));
+typedef _Float16 mf16x2 __attribute__((ext_vector_type(2)));
+
+// 8 of a fragment's 32 values in fp16
+__device__ __forceinline__ mf16x8 widen(mi32x8 f, int e) {
+    mf16x8 r;
+#pragma unroll
+    for (int w = 0; w < 2; ++w) {
+        const mf16x2 lo = __builtin_amdgcn_cvt_scalef32_pk_f16_fp8(f[2 * e + w], 1.0f, false);
+        const mf16x2 hi = __builtin_amdgcn_cvt_scalef32_pk_f16_fp8(f[2 * e + w], 1.0f, true);
+        r[4 * w + 0] = lo[0];
+        r[4 * w + 1] = lo[1];
+        r[4 * w + 2] = hi[0];
+        r[4 * w + 3] = hi[1];
+    }
+    return r;
+}
+
+// One block of 128: both operands hold lane l's row l & 15 and its 32 values from 32 (l >> 4) on (which
+// of them share an instruction is the same in both, so the order of k does not matter).
+template <bool WIDE>
+__device__ __forceinline__ vf32x4 mfma_block(mi32x8 a, mi32x8 b) {
+    vf32x4 d = {0.0f, 0.0f, 0.0f, 0.0f};
+    if constexpr (WIDE) {
+#pragma unroll
+        for (int e = 0; e < 4; ++e) d = __builtin_amdgcn_mfma_f32_16x16x32_f16(widen(a, e), widen(b, e), d, 0, 0, 0);
+    } else {
+        d = __builtin_amdgcn_mfma_scale_f32_16x16x128_f8f6f4(a, b, d, 0, 0, 0, 0, 0, 0);
+    }
+    return d;
+}
+
+// 16 values from column c on of a row of k values, zero past its end
+__device__ __forceinline__ vu32x4 load_q16(const uint8_t* row, int c, int k) {
+    if (c + 16 <= k) return load16(row + c);
+    vu32x4 r = {0, 0, 0, 0};
+    for (int e = 0; c + e < k; ++e) r[e >> 2] |= (uint32_t)row[c + e] << (8 * (e & 3));
+    return r;
+}
+
+__device__ __forceinline__ mi32x8 load_frag(const uint8_t* row, int c, int k) {
+    const vu32x4 lo = load_q16(row, c, k), hi = load_q16(row, c + 16, k);
+    return mi32x8{(int)lo[0], (int)lo[1], (int)lo[2], (int)lo[3], (int)hi[0], (int)hi[1], (int)hi[2], (int)hi[3]};
+}
+
+struct MmArgs {
+    const uint8_t* a;
+    const uint8_t* b;
+    const float* sa;    // [m][kb]
+    const float* sb;    // [n][kb], or [ceil(n / 128)][kb] with b_tile
+    const float* bias;  // [n] or NULL
+    void* y;
+    int64_t lda, ldb, ldy;
+    int64_t m, n;
+    int k, kb, b_tile;
+    int64_t mt, nt;     // tiles along m and n
+};
+
+// y[m][n .. n + 4), the lane's four neighbouring columns
+template <typename TO>
+__device__ __forceinline__ void store_y4(TO* p, vf32x4 v, int valid) {
+    typedef TO o4 __attribute__((ext_vector_type(4), aligned(sizeof(TO))));
+    if (valid >= 4) {
+        o4 o;
+#pragma unroll
+        for (int e = 0; e < 4; ++e) o[e] = (TO)v[e];
+        *reinterpret_cast<o4*>(p) = o;
+    } else {
+#pragma unroll
+        for (int e = 0; e < 3; ++e)
+            if (e < valid) p[e] = (TO)v[e];
+    }
+}
+
+// Operands straight from memory to registers.  A wave computes 16 MI rows of y by 16 NI columns; the
+// rows of b are the MFMA's A operand, so a lane ends with four neighbouring columns of one row of y.
+template <int MI, int NI, typename TO>
+__global__ __launch_bounds__(kBlock) void k_mm_direct(MmArgs p) {
+    const int lane = threadIdx.x & 63, g = lane >> 4, i = lane & 15;
+    const int64_t wave = (int64_t)blockIdx.x * (kBlock / 64) + (threadIdx.x >> 6);
+    if (wave >= p.mt * p.nt) return;
+    const int64_t m0 = wave / p.nt * (16 * MI), n0 = wave % p.nt * (16 * NI);
+    vf32x4 acc[MI][NI];
+#pragma unroll
+    for (int x = 0; x < MI; ++x)
+#pragma unroll
+        for (int j = 0; j < NI; ++j) acc[x][j] = vf32x4{0.0f, 0.0f, 0.0f, 0.0f};
+    // rows past the end repeat the last one: what they give is not stored
+    const uint8_t* ar[MI];
+    const uint8_t* br[NI];
+#pragma unroll
+    for (int x = 0; x < MI; ++x) ar[x] = p.a + min(m0 + 16 * x + i, p.m - 1) * p.lda;
+#pragma unroll
+    for (int j = 0; j < NI; ++j) br[j] = p.b + min(n0 + 16 * j + i, p.n - 1) * p.ldb;
+    for (int kb = 0; kb < p.kb; ++kb) {
+        const int c = kb * kScaleBlock + 32 * g;
+        mi32x8 fb[NI];
+        vf32x4 sb[NI];
+#pragma unroll
+        for (int j = 0; j < NI; ++j) {
+            fb[j] = load_frag(br[j], c, p.k);
+#pragma unroll
+            for (int r = 0; r < 4; ++r) {
+                const int64_t n = min(n0 + 16 * j + 4 * g + r, p.n - 1);
+                sb[j][r] = p.sb[(p.b_tile ? n / kScaleBlock : n) * p.kb + kb];
+            }
+        }
+#pragma unroll
+        for (int x = 0; x < MI; ++x) {
+            const mi32x8 fa = load_frag(ar[x], c, p.k);
+            const float sa = p.sa[min(m0 + 16 * x + i, p.m - 1) * p.kb + kb];
+#pragma unroll
+            for (int j = 0; j < NI; ++j) {
+                const vf32x4 d = mfma_block<std::is_same<TO, float>::value>(fb[j], fa);
+#pragma unroll
+                for (int r = 0; r < 4; ++r) acc[x][j][r] = fmaf(sa * sb[j][r], d[r], acc[x][j][r]);
+            }
+        }
+    }
+#pragma unroll
+    for (int j = 0; j < NI; ++j) {
+        const int64_t n = n0 + 16 * j + 4 * g;
+        const int valid = (int)min((int64_t)4, p.n - n);
+        if (valid <= 0) continue;
+        vf32x4 bias = {0.0f, 0.0f, 0.0f, 0.0f};
+        if (p.bias)
+#pragma unroll
+            for (int r = 0; r < 4; ++r)
+                if (r < valid) bias[r] = p.bias[n + r];
+#pragma unroll
+        for (int x = 0; x < MI; ++x) {
+            const int64_t m = m0 + 16 * x + i;
+            if (m < p.m) store_y4(static_cast<TO*>(p.y) + m * p.ldy + n, acc[x][j] + bias, valid);
+        }
+    }
+}
+
+template <typename TO>
+static hipError_t mm_t(MmArgs p, hipStream_t st) {
+    if (p.m <= 16) {
+        p.mt = 1;
+        p.nt = (p.n + 15) / 16;
+        launch(k_mm_direct<1, 1, TO>, dim3((unsigned)((p.nt + 3) / 4)), kBlock, 0, st, p);
+    } else {
+        p.mt = (p.m + 63) / 64;
+        p.nt = (p.n + 63) / 64;
+        launch(k_mm_direct<4, 4, TO>, dim3((unsigned)((p.mt * p.nt + 3) / 4)), kBlock, 0, st, p);
+    }
+    return hipGetLastError();
+}
+
+hipError_t launch_matmul_blocks(const uint8_t* a, int64_t lda, const float* sa, const uint8_t* b, int64_t ldb,
+                                const float* sb, int b_tile, const float* bias, int64_t m, int64_t n, int k,
+                                int out_dtype, void* y, int64_t ldy, hipStream_t st) {
+    if (m <= 0 || n <= 0) return hipSuccess;
+    MmArgs p{a, b, sa, sb, bias, y, lda, ldb, ldy, m, n, k, (k + kScaleBlock - 1) / kScaleBlock, b_tile, 0, 0};
+    if (out_dtype == NCF_F32) return mm_t<float>(p, st);
+    if (out_dtype == NCF_BF16) return mm_t<__bf16>(p, st);
+    return mm_t<_Float16>(p, st);
+}
+
+}  // namespace ncf

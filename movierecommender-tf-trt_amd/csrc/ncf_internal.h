@@ -994,4 +994,11 @@ hipError_t launch_score_pairs(const int32_t* users, int64_t nq, int I, int32_t* 
 hipError_t launch_topk_rows(const float* probs, int64_t rows, int I, int k, int32_t* top_items, float* top_scores,
                             hipStream_t st);
 
+// Catalogue operators (ncf_fp8.hip): block-scaled 8-bit operands and their product
+hipError_t launch_quantize(const void* x, int dtype, int64_t rows, int cols, int64_t ld, int tile, uint8_t* q,
+                           int64_t q_ld, float* scale, hipStream_t st);
+hipError_t launch_matmul_blocks(const uint8_t* a, int64_t lda, const float* sa, const uint8_t* b, int64_t ldb,
+                                const float* sb, int b_tile, const float* bias, int64_t m, int64_t n, int k,
+                                int out_dtype, void* y, int64_t ldy, hipStream_t st);
+
 }  // namespace ncf
