@@ -531,6 +531,76 @@ int ncf_matmul_blocks(const void* a, int64_t a_ld, const float* a_scale, const v
                       const float* b_scale, int32_t b_tile, const float* bias, int64_t m, int64_t n, int64_t k,
                       int32_t out_dtype, void* y, int64_t y_ld, void* stream);
 
+/* Drawing items from logits by given uniform numbers.  For a row of n logits, its allowed items are
+ * those whose mask byte is not 0 (mask may be NULL) and whose logit is neither NaN nor -inf; m is the
+ * largest of them.
+ *   1. the top_k best, best first, equals in the order of their ids (top_k <= 0: all;
+ *      temperature <= 0 or NaN: one)
+ *   2. weights exp((x - m) / temperature), 1 where x = m
+ *   3. of them the shortest leading list with at least top_p of their weight (<= 0: one item, >= 1: all)
+ *   4. of it the items of weight >= min_p (<= 0: all, >= 1: those that equal the best)
+ *   5. draw d: the first item, in the order of the ids, at which the running sum of the weights passes
+ *      u[row][d] times their total (u outside [0, 1): the nearest end)
+ * items[row][d] = that item, probs[row][d] = its share of the total; -1 and 0 where no item is allowed.
+ * Weights are summed as integers in units of 2^-min(51, 62 - ceil(log2 n)): a result does not depend
+ * on the launch.  temperature / top_k / top_p / min_p: one value, or, where the pointer is not NULL,
+ * one per row (float32, top_k int32).  u is float32 (u64 == 0) or float64. */
+typedef struct ncf_draw {
+    const void* logits;
+    int32_t dtype;              /* NCF_F32 / NCF_BF16 / NCF_F16 */
+    int32_t u64;
+    int64_t rows, n, ld;
+    const uint8_t* mask;
+    int64_t mask_ld;
+    const void* u;              /* [rows][draws] */
+    int64_t draws;
+    const float* temperature_rows;
+    const int32_t* top_k_rows;
+    const float* top_p_rows;
+    const float* min_p_rows;
+    double temperature, top_p, min_p;
+    int64_t top_k;
+    int32_t* items;             /* [rows][draws] */
+    float* probs;               /* [rows][draws] */
+} ncf_draw_t;
+int ncf_draw_items(const ncf_draw_t* draw, void* stream);
+
+/* Distillation from a teacher's best items (k <= NCF_DISTILL_MAX_K a row; item ids outside [0, v) are
+ * padding).  With p = softmax(logits / temperature) and q_i = exp(teacher_logits_i / temperature - ref),
+ *   loss[row] = sum_i q_i (log q_i - log p[item_i])
+ * where ref is the log-sum-exp of the row's list, or teacher_lse[row] (the teacher's log-sum-exp of
+ * logits / temperature over its whole catalogue), which adds the mass outside the list as one more
+ * class: q0 (log q0 - log p0), q0 = 1 - sum q, p0 = the student's mass outside (left out where one of
+ * them is 0).  grad = d (sum over rows of grad_loss[row] loss[row]) / d logits.  A row with no entry, or
+ * whose logits are all -inf, has loss and gradient 0.
+ *   ncf_distill_loss       writes loss and state (double[rows][NCF_DISTILL_STATE])
+ *   ncf_distill_grad       writes grad from the state of the same inputs (no workspace)
+ *   ncf_distill_loss_grad  both
+ * ws: ncf_distill_workspace_size bytes; nothing persists in it between calls. */
+#define NCF_DISTILL_MAX_K 1024
+#define NCF_DISTILL_STATE 5
+typedef struct ncf_distill {
+    const void* logits;
+    int32_t dtype;
+    int32_t items64;            /* teacher_items: 0 int32, 1 int64 */
+    int64_t rows, v, ld;
+    const void* teacher_items;  /* [rows][k], rows items_ld apart */
+    const float* teacher_logits;
+    int64_t k, items_ld, teacher_ld;
+    const float* teacher_lse;   /* [rows] or NULL */
+    double temperature;         /* > 0 */
+    const float* grad_loss;     /* [rows] or NULL: grad_loss_value */
+    float grad_loss_value;
+    float* loss;                /* [rows] */
+    double* state;
+    void* grad;                 /* [rows][v] of dtype, rows grad_ld apart */
+    int64_t grad_ld;
+} ncf_distill_t;
+int ncf_distill_workspace_size(int64_t rows, int64_t v, size_t* bytes);
+int ncf_distill_loss(const ncf_distill_t* d, void* ws, size_t ws_bytes, void* stream);
+int ncf_distill_grad(const ncf_distill_t* d, void* stream);
+int ncf_distill_loss_grad(const ncf_distill_t* d, void* ws, size_t ws_bytes, void* stream);
+
 /* On-device negative sampling + batch assembly.  Replaces
  * MovieLensDataGenerator.__getitem__ (data_pipeline.py:115-150): for the n_pos positives
  * order[first .. first+n_pos) (indexes into pos_users/pos_items, the epoch's shuffled order,

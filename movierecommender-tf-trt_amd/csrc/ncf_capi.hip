@@ -1,6 +1,7 @@
 // C ABI entry points (include/movierec_ncf.h).  Host orchestration only:
 // argument validation, workspace carving and the launch sequence of each call.
 
+#include <cmath>
 #include <cstdarg>
 #include <cstdio>
 #include <cstdlib>
@@ -1529,6 +1530,61 @@ int ncf_matmul_blocks(const void* a, int64_t a_ld, const float* a_scale, const v
                                                static_cast<const uint8_t*>(b), b_ld, b_scale, b_tile != 0, bias, m, n,
                                                (int)k, out_dtype, y, y_ld, (hipStream_t)stream),
                      "ncf_matmul_blocks");
+}
+
+int ncf_draw_items(const ncf_draw_t* d, void* stream) {
+    if (!d) return fail(NCF_EINVAL, "draw is NULL");
+    if (int r = check_dtype(d->dtype)) return r;
+    if (d->rows < 0 || d->draws < 0)
+        return fail(NCF_EINVAL, "rows and draws must be >= 0, got %lld, %lld", (long long)d->rows, (long long)d->draws);
+    if (d->rows == 0 || d->draws == 0) return 0;
+    if (int r = check_matrix("logits", d->logits, d->rows, d->n, d->ld)) return r;
+    if (d->mask)
+        if (int r = check_matrix("mask", d->mask, d->rows, d->n, d->mask_ld)) return r;
+    if (!d->u || !d->items || !d->probs) return fail(NCF_EINVAL, "NULL device pointer");
+    if (d->rows > INT32_MAX || d->draws > INT32_MAX / d->rows)
+        return fail(NCF_EINVAL, "%lld rows of %lld draws are too many", (long long)d->rows, (long long)d->draws);
+    return hip_check(ncf::launch_draw(*d, (hipStream_t)stream), "ncf_draw_items");
+}
+
+int ncf_distill_workspace_size(int64_t rows, int64_t v, size_t* bytes) {
+    if (!bytes) return fail(NCF_EINVAL, "bytes is NULL");
+    if (rows < 0 || v < 1 || v > INT32_MAX - 128)
+        return fail(NCF_EINVAL, "no workspace for %lld rows of %lld items", (long long)rows, (long long)v);
+    if (ncf::distill_blocks(rows, (int)v) > INT32_MAX)
+        return fail(NCF_EINVAL, "%lld rows of %lld items are too many", (long long)rows, (long long)v);
+    *bytes = ncf::distill_workspace(rows, (int)v);
+    return 0;
+}
+
+static int distill(const ncf_distill_t* d, void* ws, size_t ws_bytes, bool forward, bool backward, void* stream) {
+    if (!d) return fail(NCF_EINVAL, "distill is NULL");
+    if (int r = check_dtype(d->dtype)) return r;
+    if (d->rows < 0) return fail(NCF_EINVAL, "rows must be >= 0, got %lld", (long long)d->rows);
+    if (d->rows == 0) return 0;
+    if (int r = check_matrix("logits", d->logits, d->rows, d->v, d->ld)) return r;
+    if (int r = check_matrix("teacher_items", d->teacher_items, d->rows, d->k, d->items_ld)) return r;
+    if (int r = check_matrix("teacher_logits", d->teacher_logits, d->rows, d->k, d->teacher_ld)) return r;
+    if (d->k > NCF_DISTILL_MAX_K)
+        return fail(NCF_EINVAL, "k must be in [1, %d], got %lld", NCF_DISTILL_MAX_K, (long long)d->k);
+    if (!(d->temperature > 0.0) || std::isinf(d->temperature))
+        return fail(NCF_EINVAL, "temperature must be positive and finite, got %g", d->temperature);
+    if (!d->state || (forward && !d->loss)) return fail(NCF_EINVAL, "NULL device pointer");
+    size_t need = 0;
+    if (int r = ncf_distill_workspace_size(d->rows, d->v, &need)) return r;
+    if (forward && (!ws || ws_bytes < need))
+        return fail(NCF_EINVAL, "workspace of %zu bytes, need %zu", ws ? ws_bytes : (size_t)0, need);
+    if (backward)
+        if (int r = check_output("grad", d->grad, d->rows, d->v, d->grad_ld)) return r;
+    return hip_check(ncf::launch_distill(*d, ws, forward, backward, (hipStream_t)stream), "ncf_distill");
+}
+
+int ncf_distill_loss(const ncf_distill_t* d, void* ws, size_t ws_bytes, void* stream) {
+    return distill(d, ws, ws_bytes, true, false, stream);
+}
+int ncf_distill_grad(const ncf_distill_t* d, void* stream) { return distill(d, nullptr, 0, false, true, stream); }
+int ncf_distill_loss_grad(const ncf_distill_t* d, void* ws, size_t ws_bytes, void* stream) {
+    return distill(d, ws, ws_bytes, true, true, stream);
 }
 
 int ncf_sample_batch(const ncf_sampler_data_t* d, const int32_t* order, int64_t first, int32_t n_pos, int32_t negs,

@@ -67,6 +67,21 @@ class NcfSamplerData(ctypes.Structure):
                 ("num_users", _i32), ("num_items", _i32)]
 
 
+class NcfDraw(ctypes.Structure):
+    _fields_ = [("logits", _vp), ("dtype", _i32), ("u64", _i32), ("rows", _i64), ("n", _i64), ("ld", _i64),
+                ("mask", _vp), ("mask_ld", _i64), ("u", _vp), ("draws", _i64), ("temperature_rows", _vp),
+                ("top_k_rows", _vp), ("top_p_rows", _vp), ("min_p_rows", _vp), ("temperature", ctypes.c_double),
+                ("top_p", ctypes.c_double), ("min_p", ctypes.c_double), ("top_k", _i64), ("items", _vp),
+                ("probs", _vp)]
+
+
+class NcfDistill(ctypes.Structure):
+    _fields_ = [("logits", _vp), ("dtype", _i32), ("items64", _i32), ("rows", _i64), ("v", _i64), ("ld", _i64),
+                ("teacher_items", _vp), ("teacher_logits", _vp), ("k", _i64), ("items_ld", _i64),
+                ("teacher_ld", _i64), ("teacher_lse", _vp), ("temperature", ctypes.c_double), ("grad_loss", _vp),
+                ("grad_loss_value", _f32), ("loss", _vp), ("state", _vp), ("grad", _vp), ("grad_ld", _i64)]
+
+
 _P = ctypes.POINTER
 _SIGNATURES = {
     "ncf_abi_version": (ctypes.c_int, []),
@@ -140,6 +155,11 @@ _SIGNATURES = {
     "ncf_quantize_blocks": (ctypes.c_int, [_vp, _i32, _i64, _i64, _i64, _i32, _vp, _i64, _vp, _vp]),
     "ncf_matmul_blocks": (ctypes.c_int, [_vp, _i64, _vp, _vp, _i64, _vp, _i32, _vp, _i64, _i64, _i64, _i32, _vp,
                                          _i64, _vp]),
+    "ncf_draw_items": (ctypes.c_int, [_P(NcfDraw), _vp]),
+    "ncf_distill_workspace_size": (ctypes.c_int, [_i64, _i64, _P(ctypes.c_size_t)]),
+    "ncf_distill_loss": (ctypes.c_int, [_P(NcfDistill), _vp, ctypes.c_size_t, _vp]),
+    "ncf_distill_grad": (ctypes.c_int, [_P(NcfDistill), _vp]),
+    "ncf_distill_loss_grad": (ctypes.c_int, [_P(NcfDistill), _vp, ctypes.c_size_t, _vp]),
     "ncf_profile_enable": (ctypes.c_int, [_i32, _i32]),
     "ncf_profile_read": (ctypes.c_int, [_i32, _P(ctypes.c_double), _P(_i64)]),
     "ncf_profile_pause": (ctypes.c_int, [_i32]),
@@ -148,6 +168,7 @@ _SIGNATURES = {
 EXPORTED = sorted(_SIGNATURES)
 K_INDEX, K_FWD_BWD, K_EMB_UPDATE, K_MLP_UPDATE, K_METRICS, K_SCORE, K_SAMPLE, K_CATCHUP = 1, 2, 3, 4, 5, 6, 7, 8
 NCF_F32, NCF_BF16, NCF_F16 = 0, 1, 2
+NCF_DISTILL_MAX_K, NCF_DISTILL_STATE = 1024, 5
 NCF_SCORE_FP16, NCF_SCORE_FP32, NCF_SCORE_MAX_K = 0, 1, 32
 
 

@@ -2,6 +2,9 @@
 
 ``quantize_blocks`` / ``matmul_blocks``  logits as a product of 8-bit operands with a scale for each
                                         block of 128 values (GMF models: user factors x item factors)
+``sample_items``                        items drawn from the logits: temperature, top-k, top-p, min-p
+``distill_loss`` / ``distill_grad`` / ``distill_loss_grad``
+                                        a student's logits against a teacher's list of best items
 
 Every tensor lives on one HIP device and the work is enqueued on that device's current stream; no
 call synchronises, and what a call needs beside its outputs it allocates from torch's caching
@@ -10,6 +13,9 @@ over their rows; their last dimension is dense.  A wrong argument raises ``Value
 
 The reference scores a list of items for one user and keeps the best (movierec/trt_client.py:43-57).
 """
+
+import ctypes
+import math
 
 import torch
 
@@ -113,3 +119,163 @@ def matmul_blocks(a, a_scale, b, b_scale, bias=None, out_dtype=torch.float32):
         _call(N.lib().ncf_matmul_blocks, a.device, a.data_ptr(), lda, a_scale.data_ptr(), b.data_ptr(), ldb,
               b_scale.data_ptr(), 1 if tile else 0, N.ptr(bias), m, n, k, code, y.data_ptr(), n)
     return y
+
+
+def _setting(name, value, rows, dtype, device, low, high):
+    """One number for all rows, or a tensor with one per row: (number, address or None)."""
+    if torch.is_tensor(value):
+        return 0, _dense(name, value, (rows,), dtype, device).data_ptr()
+    if not low <= value <= high:   # (a NaN fails too)
+        raise ValueError("%s must be in [%g, %g], got %r" % (name, low, high, value))
+    return value, None
+
+
+def sample_items(logits, u, temperature=1.0, top_k=0, top_p=1.0, min_p=0.0, mask=None):
+    """Draws items from ``logits`` (rows, n; float32, bfloat16 or float16) by the given uniform numbers
+    ``u`` (rows,) or (rows, draws), float32 or float64 in [0, 1): ``(items, probs)`` of u's shape, int32
+    and float32.  A row keeps its ``top_k`` best items (0: all), of them the shortest leading list with
+    at least ``top_p`` of the weight exp(logit / temperature), of it the items with at least ``min_p``
+    of the best one's weight; equals rank by the lower id.  A draw takes the first kept item, in the
+    order of the ids, at which the running sum of the weights passes u times their total; its
+    probability is its share.  Draws of a row are independent (with replacement).  temperature 0 is
+    the best item alone.
+
+    ``mask`` (rows, n) or (n,) for every row, bool or uint8: False/0 items are never drawn, whatever
+    their logits; neither are NaN and -inf.  A row with nothing to draw gives item -1, probability 0.
+    Each setting is a number or a tensor with one per row (float32; top_k int32), where values outside
+    the range act as its nearest end."""
+    ld = _matrix("logits", logits)
+    dev = logits.device
+    rows, n = logits.shape
+    d = N.NcfDraw()
+    d.dtype = _dtype_code("logits", logits.dtype)
+    if n < 1:
+        raise ValueError("logits has no columns")
+    if not torch.is_tensor(u) or u.dim() not in (1, 2) or u.shape[0] != rows:
+        raise ValueError("u must have shape (%d,) or (%d, draws)" % (rows, rows))
+    if u.dtype not in (torch.float32, torch.float64):
+        raise ValueError("u must be float32 or float64, got %s" % u.dtype)
+    _dense("u", u, u.shape, u.dtype, dev)
+    d.temperature, d.temperature_rows = _setting("temperature", temperature, rows, torch.float32, dev, 0, math.inf)
+    d.top_k, d.top_k_rows = _setting("top_k", top_k, rows, torch.int32, dev, 0, 2 ** 62)
+    d.top_p, d.top_p_rows = _setting("top_p", top_p, rows, torch.float32, dev, 0, 1)
+    d.min_p, d.min_p_rows = _setting("min_p", min_p, rows, torch.float32, dev, 0, 1)
+    if mask is not None:
+        if not torch.is_tensor(mask) or mask.dtype not in (torch.bool, torch.uint8):
+            raise ValueError("mask must be a bool or uint8 tensor")
+        if tuple(mask.shape) == (n,):
+            mask = mask.view(1, n).expand(rows, n) if mask.is_contiguous() else mask.contiguous().expand(rows, n)
+        if tuple(mask.shape) != (rows, n):
+            raise ValueError("mask must have shape (%d, %d) or (%d,), got %s" % (rows, n, n, tuple(mask.shape)))
+        d.mask_ld = _matrix("mask", mask, dev)
+        d.mask = mask.data_ptr()
+    with torch.cuda.device(dev):
+        items = torch.empty(u.shape, dtype=torch.int32, device=dev)
+        probs = torch.empty(u.shape, dtype=torch.float32, device=dev)
+    d.draws = 1 if u.dim() == 1 else u.shape[1]
+    if rows and d.draws:
+        d.logits, d.rows, d.n, d.ld = logits.data_ptr(), rows, n, ld
+        d.u, d.u64 = u.data_ptr(), 1 if u.dtype == torch.float64 else 0
+        d.items, d.probs = items.data_ptr(), probs.data_ptr()
+        _call(N.lib().ncf_draw_items, dev, ctypes.byref(d))
+    return items, probs
+
+
+def _distill(logits, teacher_items, teacher_logits, temperature, teacher_lse):
+    """Checks what every distillation call takes; the filled argument struct."""
+    d = N.NcfDistill()
+    d.ld = _matrix("logits", logits)
+    dev = logits.device
+    d.dtype = _dtype_code("logits", logits.dtype)
+    d.rows, d.v = logits.shape
+    if d.v < 1:
+        raise ValueError("logits has no columns")
+    d.items_ld = _matrix("teacher_items", teacher_items, dev)
+    if teacher_items.dtype not in (torch.int32, torch.int64):
+        raise ValueError("teacher_items must be int32 or int64, got %s" % teacher_items.dtype)
+    d.k = teacher_items.shape[1]
+    if teacher_items.shape[0] != d.rows or not 1 <= d.k <= N.NCF_DISTILL_MAX_K:
+        raise ValueError("teacher_items must have shape (%d, 1..%d), got %s"
+                         % (d.rows, N.NCF_DISTILL_MAX_K, tuple(teacher_items.shape)))
+    d.teacher_ld = _matrix("teacher_logits", teacher_logits, dev)
+    if teacher_logits.shape != teacher_items.shape or teacher_logits.dtype != torch.float32:
+        raise ValueError("teacher_logits must be float32 of shape %s, got %s of %s"
+                         % (tuple(teacher_items.shape), teacher_logits.dtype, tuple(teacher_logits.shape)))
+    if teacher_lse is not None:
+        d.teacher_lse = _dense("teacher_lse", teacher_lse, (d.rows,), torch.float32, dev).data_ptr()
+    if not 0 < temperature < math.inf:
+        raise ValueError("temperature must be positive and finite, got %r" % (temperature,))
+    d.temperature = temperature
+    d.logits, d.teacher_items, d.teacher_logits = logits.data_ptr(), teacher_items.data_ptr(), teacher_logits.data_ptr()
+    d.items64 = 1 if teacher_items.dtype == torch.int64 else 0
+    return d
+
+
+def _distill_outputs(d, logits, grad_loss):
+    if torch.is_tensor(grad_loss):
+        d.grad_loss = _dense("grad_loss", grad_loss, (d.rows,), torch.float32, logits.device).data_ptr()
+    else:
+        d.grad_loss_value = grad_loss
+    grad = torch.empty(d.rows, d.v, dtype=logits.dtype, device=logits.device)
+    d.grad, d.grad_ld = grad.data_ptr(), d.v
+    return grad
+
+
+def _distill_workspace(d, device):
+    nbytes = ctypes.c_size_t()
+    N.check(N.lib().ncf_distill_workspace_size(d.rows, d.v, ctypes.byref(nbytes)))
+    return torch.empty(nbytes.value, dtype=torch.uint8, device=device)
+
+
+def distill_loss(logits, teacher_items, teacher_logits, temperature=1.0, teacher_lse=None):
+    """Per row, the divergence of a student's softmax over the catalogue from a teacher's list of its
+    best items: ``(loss, state)``, loss float32 (rows,), state for :func:`distill_grad`.
+
+    ``logits`` (rows, v; float32, bfloat16 or float16) are the student's; ``teacher_items`` (rows, k;
+    int32 or int64, k <= 1024) and ``teacher_logits`` (rows, k; float32) the teacher's list, as
+    ``NCFEngine.score_topk`` gives items (ids outside [0, v), such as -1, are padding).  With
+    p = softmax(logits / temperature) and q = softmax(teacher_logits / temperature) over the list,
+    loss = sum q (log q - log p[items]).  ``teacher_lse`` (rows,) float32, the teacher's
+    logsumexp(logits / temperature) over its whole catalogue, makes q the teacher's probabilities
+    and adds the mass outside the list as one more class.  A row without an entry, or whose logits
+    are all -inf, has loss 0.  (Gradients by soft targets usually carry a factor temperature ** 2:
+    pass it in ``grad_loss``.)"""
+    d = _distill(logits, teacher_items, teacher_logits, temperature, teacher_lse)
+    dev = logits.device
+    with torch.cuda.device(dev):
+        loss = torch.empty(d.rows, dtype=torch.float32, device=dev)
+        state = torch.empty(d.rows, N.NCF_DISTILL_STATE, dtype=torch.float64, device=dev)
+        ws = _distill_workspace(d, dev)
+    d.loss, d.state = loss.data_ptr(), state.data_ptr()
+    if d.rows:
+        _call(N.lib().ncf_distill_loss, dev, ctypes.byref(d), ws.data_ptr(), ws.numel())
+    return loss, state
+
+
+def distill_grad(logits, teacher_items, teacher_logits, state, grad_loss=1.0, temperature=1.0, teacher_lse=None):
+    """d sum(grad_loss * loss) / d logits, of logits' type and shape, from the ``state`` that
+    :func:`distill_loss` gave for the same inputs.  ``grad_loss``: a number or float32 (rows,)."""
+    d = _distill(logits, teacher_items, teacher_logits, temperature, teacher_lse)
+    dev = logits.device
+    _dense("state", state, (d.rows, N.NCF_DISTILL_STATE), torch.float64, dev)
+    with torch.cuda.device(dev):
+        grad = _distill_outputs(d, logits, grad_loss)
+    d.state = state.data_ptr()
+    if d.rows:
+        _call(N.lib().ncf_distill_grad, dev, ctypes.byref(d))
+    return grad
+
+
+def distill_loss_grad(logits, teacher_items, teacher_logits, grad_loss=1.0, temperature=1.0, teacher_lse=None):
+    """:func:`distill_loss` and :func:`distill_grad` in one call: ``(loss, grad)``."""
+    d = _distill(logits, teacher_items, teacher_logits, temperature, teacher_lse)
+    dev = logits.device
+    with torch.cuda.device(dev):
+        loss = torch.empty(d.rows, dtype=torch.float32, device=dev)
+        state = torch.empty(d.rows, N.NCF_DISTILL_STATE, dtype=torch.float64, device=dev)
+        grad = _distill_outputs(d, logits, grad_loss)
+        ws = _distill_workspace(d, dev)
+    d.loss, d.state = loss.data_ptr(), state.data_ptr()
+    if d.rows:
+        _call(N.lib().ncf_distill_loss_grad, dev, ctypes.byref(d), ws.data_ptr(), ws.numel())
+    return loss, grad
