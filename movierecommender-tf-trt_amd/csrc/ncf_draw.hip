@@ -42,7 +42,7 @@ struct DrawArgs {
     const float* min_p;
     double temperature_v, top_p_v, min_p_v;
     int32_t top_k_v;
-    int shift;                // S
+    double unit;              // 2^S
     int32_t* items;
     float* probs;
 };
@@ -65,15 +65,37 @@ __device__ __forceinline__ uint32_t item_key(T x, bool allowed) {
     return (allowed && f > -INFINITY) ? ukey(f) : 0u;   // (a NaN compares false)
 }
 
-struct Weigher {
-    double m, t, scale;
-    uint32_t top;  // key of the best item
+// 2^(j / 64), filled by the compiler's exp2
+constexpr int kPowers = 64;
 
-    __device__ __forceinline__ double real(uint32_t key) const {
-        if (key == top) return 1.0;
-        return fmax(exp(((double)unukey(key) - m) / t), 0.0);   // (infinities in both: NaN, no weight)
+// w = exp((x - m) / t) as an integer in units of 2^-S.  With y = (x - m) log2(e) / t = j / 64 + f,
+// w = 2^(j / 64) e^(f ln 2): the powers of two from a table in LDS, the rest, |f ln 2| <= ln 2 / 128, by
+// its Taylor polynomial to the fifth power (the next term is below 2^-54).  Adding 2^52 rounds to an
+// integer.  About 14 instructions of 64 bits against about 40 of exp().
+struct Weigher {
+    double m, c, unit;
+    float top;
+    const double* power;   // [kPowers]
+
+    // w 2^S, not rounded
+    __device__ __forceinline__ double real(float x) const {
+        if (x == top) return unit;
+        double y = ((double)x - m) * c;
+        y = fmax(y, -200.0);   // (below every unit; also where infinities in both made a NaN)
+        const double j = rint(y * 64.0);
+        const double r = (y - j * 0x1p-6) * 0.69314718055994530942;
+        double e = fma(r, 1.0 / 120.0, 1.0 / 24.0);
+        e = fma(r, e, 1.0 / 6.0);
+        e = fma(r, e, 0.5);
+        e = fma(r, e, 1.0);
+        e = fma(r, e, 1.0);
+        const int n = (int)j;
+        return ldexp(power[n & (kPowers - 1)] * e, n >> 6) * unit;
     }
-    __device__ __forceinline__ uint64_t fixed(double w) const { return (uint64_t)rint(w * scale); }
+    __device__ __forceinline__ unsigned long long fixed(float x) const { return round(real(x)); }
+    __device__ __forceinline__ static unsigned long long round(double w) {
+        return (unsigned long long)__double_as_longlong(w + 0x1p52) & 0xfffffffffffffull;
+    }
 };
 
 // ----------------------------------------------------------------------------- one workgroup per row
@@ -90,7 +112,12 @@ struct DrawShared {
     uint32_t wave32[kDrawThreads / 64];
     unsigned long long pick64;
     uint32_t pick_bin;
+    double power[kPowers];
 };
+
+__device__ __forceinline__ void fill_powers(double* power, int threads) {
+    for (int j = threadIdx.x; j < kPowers; j += threads) power[j] = exp2(j * (1.0 / kPowers));
+}
 
 __device__ __forceinline__ unsigned long long shfl_up64(unsigned long long v, int d) {
     return (unsigned long long)__shfl_up((long long)v, d, 64);
@@ -196,7 +223,10 @@ __global__ __launch_bounds__(kDrawThreads) void k_draw(DrawArgs a) {
         }
         return;
     }
-    const Weigher wt{(double)unukey(top), t > 0.0 ? t : 1.0, exp2((double)a.shift), top};
+    fill_powers(s.power, kDrawThreads);
+    __syncthreads();
+    const Weigher wt{(double)unukey(top), 1.4426950408889634074 / (t > 0.0 ? t : 1.0), a.unit, unukey(top), s.power};
+    const double min_w = min_p * a.unit;
 
     // top-k: the k-th largest key, digit by digit
     uint32_t bound = 1, ties = 0xffffffffu;   // all allowed items
@@ -237,7 +267,7 @@ __global__ __launch_bounds__(kDrawThreads) void k_draw(DrawArgs a) {
             block_before32(equal, s, &equal);
         }
         const unsigned long long over =
-            ties != 0xffffffffu ? (unsigned long long)(equal - ties) * wt.fixed(wt.real(bound)) : 0;
+            ties != 0xffffffffu ? (unsigned long long)(equal - ties) * wt.fixed(unukey(bound)) : 0;
         uint32_t prefix = 0;
         unsigned long long above = 0;
         double total = 0.0;
@@ -248,7 +278,7 @@ __global__ __launch_bounds__(kDrawThreads) void k_draw(DrawArgs a) {
                 const uint32_t key = r.key(i);
                 if (key >= bound && same_prefix(key, prefix, level))
                     atomicAdd(&s.weight[(key >> digit_shift(level)) & digit_mask(level)],
-                              (unsigned long long)wt.fixed(wt.real(key)));
+                              wt.fixed(unukey(key)));
             }
             __syncthreads();
             if (tid == 0 && over && same_prefix(bound, prefix, level))
@@ -269,7 +299,7 @@ __global__ __launch_bounds__(kDrawThreads) void k_draw(DrawArgs a) {
             __syncthreads();
         }
         // of the equals of this key, as many as it takes
-        const unsigned long long w = wt.fixed(wt.real(prefix));
+        const unsigned long long w = wt.fixed(unukey(prefix));
         double want = ceil((p * total - (double)above) / (double)w);
         uint32_t j = want < 1.0 ? 1u : want > (double)a.n ? (uint32_t)a.n : (uint32_t)want;
         while (j > 1 && reaches(above + (unsigned long long)(j - 1) * w, p, total)) --j;
@@ -292,8 +322,8 @@ __global__ __launch_bounds__(kDrawThreads) void k_draw(DrawArgs a) {
         const uint32_t key = r.key(i);
         if (key < bound || key == 0) return 0;
         if (key == bound && seen++ >= ties) return 0;
-        const double w = wt.real(key);
-        return w >= min_p || !(min_p > 0.0) ? (unsigned long long)wt.fixed(w) : 0ull;
+        const double w = wt.real(unukey(key));
+        return w >= min_w || !(min_w > 0.0) ? Weigher::round(w) : 0ull;
     };
     unsigned long long mine = 0, total;
     {
@@ -324,6 +354,738 @@ __global__ __launch_bounds__(kDrawThreads) void k_draw(DrawArgs a) {
     }
 }
 
+// ----------------------------------------------------------------------------- rows held in registers
+//
+// A workgroup of NT threads holds a row of up to EPT NT logits in registers (-inf: not allowed), each
+// wave a contiguous part of it, reads it once, and works from there.  The bound of top-k (top-p) is
+// found in two steps: a histogram of counts (weights) over 2 NT bins that are equal steps of the logit
+// from the best down, which names the bin where the k-th item (the p-th part of the weight) lies; then
+// that bin's few items are ranked against each other, one a thread.  A bin with more than NT items (many
+// equal logits) goes digit by digit of the key instead.
+// For top-k with k <= 4 NT the histogram sees one of V neighbours only and gives a limit that the k best
+// most likely pass; the items that pass it, if they are at least k and at most 4 NT, move to a list in LDS
+// in the order of the ids, and the row is not looked at again.  (Otherwise the whole row is counted.)
+
+__device__ __forceinline__ int lane_count(uint64_t mask) { return (int)__popcll(mask); }
+// set bits of the mask below this lane, plus `more`
+__device__ __forceinline__ uint32_t lanes_before(uint64_t mask, uint32_t more) {
+    return __builtin_amdgcn_mbcnt_hi((uint32_t)(mask >> 32), __builtin_amdgcn_mbcnt_lo((uint32_t)mask, more));
+}
+
+// inclusive sums over the lanes of a wave by data-parallel moves: within rows of 16, then across rows
+template <int CTRL, int ROWS>
+__device__ __forceinline__ uint32_t moved32(uint32_t x) {
+    return (uint32_t)__builtin_amdgcn_update_dpp(0, (int)x, CTRL, ROWS, 0xf, false);
+}
+__device__ __forceinline__ uint32_t lane_sums32(uint32_t x) {
+    x += moved32<0x111, 0xf>(x);
+    x += moved32<0x112, 0xf>(x);
+    x += moved32<0x114, 0xf>(x);
+    x += moved32<0x118, 0xf>(x);
+    x += moved32<0x142, 0xa>(x);
+    x += moved32<0x143, 0xc>(x);
+    return x;
+}
+template <int CTRL, int ROWS>
+__device__ __forceinline__ unsigned long long moved64(unsigned long long x) {
+    return (unsigned long long)moved32<CTRL, ROWS>((uint32_t)(x >> 32)) << 32 | moved32<CTRL, ROWS>((uint32_t)x);
+}
+__device__ __forceinline__ unsigned long long lane_sums64(unsigned long long x) {
+    x += moved64<0x111, 0xf>(x);
+    x += moved64<0x112, 0xf>(x);
+    x += moved64<0x114, 0xf>(x);
+    x += moved64<0x118, 0xf>(x);
+    x += moved64<0x142, 0xa>(x);
+    x += moved64<0x143, 0xc>(x);
+    return x;
+}
+__device__ __forceinline__ uint32_t lane63(uint32_t x) { return (uint32_t)__builtin_amdgcn_readlane((int)x, 63); }
+__device__ __forceinline__ unsigned long long lane63(unsigned long long x) {
+    return (unsigned long long)lane63((uint32_t)(x >> 32)) << 32 | lane63((uint32_t)x);
+}
+
+template <int NT>
+struct RowShared {
+    static constexpr int kBins = 2 * NT, kWaves = NT / 64, kPer = 4, kList = kPer * NT;
+    union {
+        uint32_t count[kBins];
+        unsigned long long weight[kBins];
+        unsigned long long before[kList];   // the list's running sums
+    };
+    float list_x[kList];
+    uint32_t list_id[kList];
+    unsigned long long member_w[NT];
+    float member_x[NT];
+    uint32_t member_id[NT];
+    uint32_t members;
+    float bound;
+    uint32_t pick_bin, ties, equal;
+    unsigned long long pick;
+    unsigned long long wave64[kWaves];
+    uint32_t wave32[kWaves];
+    float wave_top[kWaves], wave_sum[kWaves], wave_n[kWaves];
+    unsigned long long seg[NT / 4];         // weights ahead of each segment of the row: a wave's vector j
+    uint32_t seg_ties[NT / 4];              // equals of the bound ahead of it
+    double power[kPowers];
+};
+
+// exclusive sums over the workgroup, the total to *sum
+template <int NT>
+__device__ __forceinline__ unsigned long long before64(unsigned long long v, RowShared<NT>& s,
+                                                       unsigned long long* sum) {
+    const int lane = threadIdx.x & 63, w = threadIdx.x >> 6;
+    const unsigned long long inc = lane_sums64(v);
+    if constexpr (NT == 64) {
+        *sum = lane63(inc);
+        return inc - v;
+    }
+    __syncthreads();
+    if (lane == 63) s.wave64[w] = inc;
+    __syncthreads();
+    unsigned long long before = 0, all = 0;
+#pragma unroll
+    for (int j = 0; j < NT / 64; ++j) {
+        const unsigned long long o = s.wave64[j];
+        before += j < w ? o : 0ull;
+        all += o;
+    }
+    *sum = all;
+    return before + inc - v;
+}
+
+template <int NT>
+__device__ __forceinline__ uint32_t before32(uint32_t v, RowShared<NT>& s, uint32_t* sum) {
+    const int lane = threadIdx.x & 63, w = threadIdx.x >> 6;
+    const uint32_t inc = lane_sums32(v);
+    if constexpr (NT == 64) {
+        *sum = lane63(inc);
+        return inc - v;
+    }
+    __syncthreads();
+    if (lane == 63) s.wave32[w] = inc;
+    __syncthreads();
+    uint32_t before = 0, all = 0;
+#pragma unroll
+    for (int j = 0; j < NT / 64; ++j) {
+        const uint32_t o = s.wave32[j];
+        before += j < w ? o : 0u;
+        all += o;
+    }
+    *sum = all;
+    return before + inc - v;
+}
+
+// bins of equal width from the best logit down; what lies below the range shares the last
+struct Bins {
+    float top, scale, last;
+    __device__ __forceinline__ int of(float x) const {
+        return (int)fminf((top - x) * scale, last);   // (infinities on both sides: NaN, the last bin)
+    }
+    // every item of a bin up to b lies above this: the bin's lower edge, less the roundings of of()
+    __device__ __forceinline__ float below(int b) const {
+        if ((float)b >= last) return -3.402823466e38f;
+        const float width = (float)(b + 1) / scale;
+        return top - width - (fabsf(top) + width) * 0x1p-21f;
+    }
+};
+__device__ __forceinline__ Bins make_bins(float top, float range, int bins) {
+    range = range > 1e-30f && range < 1e30f ? range : 1.0f;
+    return Bins{top, (float)bins / range, (float)(bins - 1)};
+}
+
+// what a row keeps: every item above `bound` and the first `ties` (in the order of the ids) equal to it
+struct Cut {
+    float bound;
+    uint32_t ties;
+    bool partial;   // more items equal the bound than `ties`
+};
+constexpr uint32_t kAllTies = 0xffffffffu;
+__device__ __forceinline__ Cut keep_all() { return Cut{-3.402823466e38f, kAllTies, false}; }
+
+// Threads' sums of two neighbouring bins, from bin 0 (the best) up, in c0 and c1: the bin at which
+// `found(before, before + bin)` holds goes to s.pick_bin, what lies before it to s.pick.
+template <int NT, typename Found>
+__device__ __forceinline__ void find_bin(unsigned long long b, unsigned long long c0, unsigned long long c1,
+                                         RowShared<NT>& s, Found found) {
+    if (found(b, b + c0)) {
+        s.pick_bin = 2 * threadIdx.x;
+        s.pick = b;
+    } else if (found(b + c0, b + c0 + c1)) {
+        s.pick_bin = 2 * threadIdx.x + 1;
+        s.pick = b + c0;
+    }
+    __syncthreads();
+}
+
+// digits of a key, best first, log2(2 NT) bits each
+template <int NT>
+struct Digits {
+    static constexpr int kBits = NT == 1024 ? 11 : NT == 512 ? 10 : NT == 256 ? 9 : 7;
+    static constexpr int kLevels = (32 + kBits - 1) / kBits;
+    static_assert(1 << kBits == 2 * NT, "a bin for every digit");
+    __device__ static int shift(int level) { return 32 - kBits * (level + 1) > 0 ? 32 - kBits * (level + 1) : 0; }
+    __device__ static uint32_t mask(int level) {
+        return (1u << (level == kLevels - 1 ? 32 - kBits * (kLevels - 1) : kBits)) - 1u;
+    }
+    __device__ static bool same(uint32_t a, uint32_t b, int level) {
+        return level == 0 || (a >> shift(level - 1)) == (b >> shift(level - 1));
+    }
+};
+
+// The bin that holds the k-th best: returns false where all allowed items are no more than k.
+// each(f) calls f(x, id) for the thread's items (-inf: not allowed).
+struct CountBin {
+    int bin;
+    uint32_t above, in;   // items in better bins, and in this
+};
+template <int NT, typename Each>
+__device__ __forceinline__ bool count_bin(uint32_t k, const Bins& bins, RowShared<NT>& s, Each each, CountBin* r) {
+    const int tid = threadIdx.x;
+    s.count[2 * tid] = s.count[2 * tid + 1] = 0;
+    if (tid == 0) s.members = 0;
+    __syncthreads();
+    each([&](float x, uint32_t) {
+        if (x > -INFINITY) atomicAdd(&s.count[bins.of(x)], 1u);
+    });
+    __syncthreads();
+    const uint32_t c0 = s.count[2 * tid], c1 = s.count[2 * tid + 1];
+    uint32_t all;
+    const uint32_t b = before32(c0 + c1, s, &all);
+    if (all <= k) return false;
+    find_bin(b, c0, c1, s, [&](unsigned long long x, unsigned long long e) { return x < k && e >= k; });
+    r->bin = (int)s.pick_bin;
+    r->above = (uint32_t)s.pick;
+    r->in = s.count[r->bin];
+    return true;
+}
+
+// Its bound.
+template <int NT, typename Each>
+__device__ __forceinline__ Cut cut_count(uint32_t k, const CountBin& in, const Bins& bins, RowShared<NT>& s,
+                                         Each each) {
+    const int tid = threadIdx.x;
+    if (in.in <= NT) {
+        each([&](float x, uint32_t id) {
+            if (x > -INFINITY && bins.of(x) == in.bin) {
+                const uint32_t at = atomicAdd(&s.members, 1u);
+                s.member_x[at] = x;
+                s.member_id[at] = id;
+            }
+        });
+        __syncthreads();
+        if (tid < (int)in.in) {
+            const float x = s.member_x[tid];
+            const uint32_t id = s.member_id[tid];
+            uint32_t rank = in.above, same = 0, equal = 0;
+#pragma unroll 4
+            for (uint32_t j = 0; j < in.in; ++j) {
+                const float o = s.member_x[j];
+                rank += o > x;
+                equal += o == x;
+                same += o == x && s.member_id[j] < id;
+            }
+            if (rank + same == k - 1) {
+                s.bound = x;
+                s.ties = same + 1;
+                s.equal = equal;
+            }
+        }
+        __syncthreads();
+        return Cut{s.bound, s.ties, s.equal > s.ties};
+    }
+    uint32_t prefix = 0, equal = 0, left = k;
+    for (int level = 0; level < Digits<NT>::kLevels; ++level) {
+        __syncthreads();
+        s.count[2 * tid] = s.count[2 * tid + 1] = 0;
+        __syncthreads();
+        const uint32_t mask = Digits<NT>::mask(level);
+        each([&](float x, uint32_t) {
+            const uint32_t key = ukey(x + 0.0f);   // (-0 equals 0)
+            if (x > -INFINITY && Digits<NT>::same(key, prefix, level))
+                atomicAdd(&s.count[mask - ((key >> Digits<NT>::shift(level)) & mask)], 1u);
+        });
+        __syncthreads();
+        const uint32_t c0 = s.count[2 * tid], c1 = s.count[2 * tid + 1];
+        uint32_t all;
+        const uint32_t before = before32(c0 + c1, s, &all);
+        find_bin(before, c0, c1, s, [&](unsigned long long x, unsigned long long e) { return x < left && e >= left; });
+        prefix |= (mask - s.pick_bin) << Digits<NT>::shift(level);
+        left -= (uint32_t)s.pick;
+        equal = s.count[s.pick_bin];
+    }
+    return Cut{unukey(prefix), left, equal > left};
+}
+
+// The shortest leading list with at least p of the weight, inside what `was` keeps.
+template <int NT, typename Each>
+__device__ __forceinline__ Cut cut_weight(double p, Cut was, const Bins& bins, const Weigher& wt, RowShared<NT>& s,
+                                          Each each) {
+    const int tid = threadIdx.x;
+    // equals of the bound beyond its ties: counted with the others, then taken off
+    uint32_t extra = 0;
+    if (was.partial) {
+        each([&](float x, uint32_t) { extra += x == was.bound; });
+        before32(extra, s, &extra);
+        extra -= was.ties;
+    }
+    const unsigned long long over = (unsigned long long)extra * wt.fixed(was.bound);
+    __syncthreads();
+    s.weight[2 * tid] = s.weight[2 * tid + 1] = 0;
+    if (tid == 0) s.members = 0;
+    __syncthreads();
+    each([&](float x, uint32_t) {
+        if (x >= was.bound) atomicAdd(&s.weight[bins.of(x)], wt.fixed(x));
+    });
+    __syncthreads();
+    if (was.partial) {
+        if (tid == 0) s.weight[bins.of(was.bound)] -= over;
+        __syncthreads();
+    }
+    unsigned long long c0 = s.weight[2 * tid], c1 = s.weight[2 * tid + 1], total;
+    const unsigned long long b = before64(c0 + c1, s, &total);
+    const double all = (double)total;
+    auto found = [&](unsigned long long x, unsigned long long e) { return !reaches(x, p, all) && reaches(e, p, all); };
+    find_bin(b, c0, c1, s, found);
+    const int bin = (int)s.pick_bin;
+    const unsigned long long above = s.pick;
+    each([&](float x, uint32_t id) {
+        if (x >= was.bound && bins.of(x) == bin) {
+            const uint32_t at = atomicAdd(&s.members, 1u);
+            if (at < NT) {
+                s.member_x[at] = x;
+                s.member_id[at] = id;
+                s.member_w[at] = wt.fixed(x);
+            }
+        }
+    });
+    __syncthreads();
+    const uint32_t in_bin = s.members;
+    if (in_bin <= NT) {
+        if (tid < (int)in_bin) {
+            const float x = s.member_x[tid];
+            const uint32_t id = s.member_id[tid];
+            unsigned long long ahead = above;
+            uint32_t same = 0, equal = 0;
+#pragma unroll 4
+            for (uint32_t j = 0; j < in_bin; ++j) {
+                const float o = s.member_x[j];
+                const bool before = o == x && s.member_id[j] < id;
+                ahead += o > x || before ? s.member_w[j] : 0ull;
+                equal += o == x;
+                same += before;
+            }
+            if (!(x == was.bound && same >= was.ties) && found(ahead, ahead + s.member_w[tid])) {
+                s.bound = x;
+                s.ties = same + 1;
+                s.equal = equal;
+            }
+        }
+        __syncthreads();
+        return Cut{s.bound, s.ties, s.equal > s.ties};
+    }
+    uint32_t prefix = 0;
+    unsigned long long ahead = 0;
+    const uint32_t bound_key = ukey(was.bound + 0.0f);
+    for (int level = 0; level < Digits<NT>::kLevels; ++level) {
+        __syncthreads();
+        s.weight[2 * tid] = s.weight[2 * tid + 1] = 0;
+        __syncthreads();
+        const uint32_t mask = Digits<NT>::mask(level);
+        each([&](float x, uint32_t) {
+            const uint32_t key = ukey(x + 0.0f);   // (-0 equals 0)
+            if (x >= was.bound && Digits<NT>::same(key, prefix, level))
+                atomicAdd(&s.weight[mask - ((key >> Digits<NT>::shift(level)) & mask)], wt.fixed(x));
+        });
+        __syncthreads();
+        if (tid == 0 && over && Digits<NT>::same(bound_key, prefix, level))
+            s.weight[mask - ((bound_key >> Digits<NT>::shift(level)) & mask)] -= over;
+        __syncthreads();
+        c0 = s.weight[2 * tid];
+        c1 = s.weight[2 * tid + 1];
+        unsigned long long level_sum;
+        const unsigned long long before = ahead + before64(c0 + c1, s, &level_sum);
+        find_bin(before, c0, c1, s, found);
+        prefix |= (mask - s.pick_bin) << Digits<NT>::shift(level);
+        ahead = s.pick;
+    }
+    const float bound = unukey(prefix);
+    uint32_t equal = 0;
+    each([&](float x, uint32_t) { equal += x == bound; });
+    before32(equal, s, &equal);
+    // of the equals of this logit, as many as it takes
+    const uint32_t most = bound == was.bound && was.partial ? was.ties : equal;
+    const unsigned long long w = wt.fixed(bound);
+    const double want = ceil((p * all - (double)ahead) / (double)w);
+    uint32_t j = want < 1.0 ? 1u : want > (double)most ? most : (uint32_t)want;
+    while (j > 1 && reaches(ahead + (unsigned long long)(j - 1) * w, p, all)) --j;
+    while (j < most && !reaches(ahead + (unsigned long long)j * w, p, all)) ++j;
+    return Cut{bound, j, equal > j};
+}
+
+struct RowSettings {
+    double t, p, min_p;
+    uint32_t k;     // 0: all
+    bool all_p;     // top-p keeps everything
+};
+__device__ __forceinline__ RowSettings row_settings(const DrawArgs& a, int64_t row) {
+    RowSettings r;
+    r.t = a.temperature ? (double)a.temperature[row] : a.temperature_v;
+    r.p = a.top_p ? (double)a.top_p[row] : a.top_p_v;
+    r.min_p = a.min_p ? (double)a.min_p[row] : a.min_p_v;
+    r.min_p = r.min_p > 1.0 ? 1.0 : r.min_p;   // the best item always stays
+    const int k = a.top_k ? a.top_k[row] : a.top_k_v;
+    r.k = k > 0 ? (uint32_t)k : 0u;
+    if (!(r.t > 0.0) || r.p <= 0.0) r.k = 1;
+    if (!(r.t > 0.0)) r.t = 1.0;
+    r.all_p = !(r.p > 0.0 && r.p < 1.0);
+    return r;
+}
+
+// u total, held inside [0, total)
+__device__ __forceinline__ unsigned long long draw_target(const DrawArgs& a, int64_t o, unsigned long long total) {
+    const double at = (a.u ? a.u[o] : (double)a.u32[o]) * (double)total;
+    const unsigned long long t = at > 0.0 ? (at >= 9.2e18 ? ~0ull >> 1 : (unsigned long long)at) : 0ull;
+    return t >= total ? total - 1 : t;
+}
+
+// V neighbours' logits from item i on; -inf where not allowed or past the row's end
+template <typename T>
+__device__ __forceinline__ void load_logits(const DrawArgs& a, int64_t row, int i, float* r) {
+    constexpr int V = Elem<T>::kVec;
+    const T* x = static_cast<const T*>(a.logits) + row * a.ld;
+    const uint8_t* mask = a.mask ? a.mask + row * a.mask_ld : nullptr;
+    if (i + V <= a.n) {
+        const typename Elem<T>::vec w = *reinterpret_cast<const typename Elem<T>::vec*>(x + i);
+#pragma unroll
+        for (int e = 0; e < V; ++e) r[e] = fmaxf((float)w[e], -INFINITY);   // (a NaN becomes -inf)
+        if (mask) {
+            uint32_t on[V / 4];
+            __builtin_memcpy(on, mask + i, V);
+#pragma unroll
+            for (int e = 0; e < V; ++e) r[e] = (on[e / 4] >> (8 * (e & 3)) & 0xffu) ? r[e] : -INFINITY;
+        }
+    } else {
+#pragma unroll
+        for (int e = 0; e < V; ++e)
+            r[e] = i + e < a.n && (mask == nullptr || mask[i + e] != 0) ? fmaxf((float)x[i + e], -INFINITY) : -INFINITY;
+    }
+}
+
+// a copy the compiler takes for a new value: what one pass over the row derives from its logits (bins,
+// weights) is computed again by the next and not kept in registers, for which there is no room
+__device__ __forceinline__ float fresh(float x) {
+    asm volatile("" : "+v"(x));
+    return x;
+}
+
+template <typename T, int NT, int EPT>
+__global__ __launch_bounds__(NT) void k_draw_row(DrawArgs a) {
+    __shared__ RowShared<NT> s;
+    constexpr int V = Elem<T>::kVec, J = EPT / V, W = NT / 64, P = RowShared<NT>::kPer;
+    static_assert(J * W <= NT / 4, "a thread and a place for every segment");
+    const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
+    const int64_t row = blockIdx.x;
+    const RowSettings set = row_settings(a, row);
+    // a wave's vectors, of 64 V neighbours each: the row spread evenly over the waves
+    const int jn = (a.n + NT * V - 1) / (NT * V), segs = jn * W;
+    const int first = wave * jn * 64 * V + lane * V;   // of the thread's vector 0; vector j: 64 V j further
+    float x[EPT];
+#pragma unroll
+    for (int j = 0; j < J; ++j) {
+        if (j < jn) {
+            load_logits<T>(a, row, first + 64 * V * j, x + V * j);
+        } else {
+#pragma unroll
+            for (int e = 0; e < V; ++e) x[V * j + e] = -INFINITY;
+        }
+    }
+    fill_powers(s.power, NT);
+
+    // the best item, and the mean of the first logits of every thread for the bins' range
+    float top = -INFINITY, sum = 0.0f, num = 0.0f;
+#pragma unroll
+    for (int e = 0; e < EPT; ++e) top = fmaxf(top, x[e]);
+#pragma unroll
+    for (int e = 0; e < V; ++e) {
+        const bool usual = fabsf(x[e]) < 1e30f;   // (no mask by the lowest value)
+        sum += usual ? x[e] : 0.0f;
+        num += usual ? 1.0f : 0.0f;
+    }
+#pragma unroll
+    for (int d = 32; d >= 1; d >>= 1) {
+        top = fmaxf(top, __shfl_xor(top, d, 64));
+        sum += __shfl_xor(sum, d, 64);
+        num += __shfl_xor(num, d, 64);
+    }
+    if constexpr (NT > 64) {
+        if (lane == 0) {
+            s.wave_top[wave] = top;
+            s.wave_sum[wave] = sum;
+            s.wave_n[wave] = num;
+        }
+        __syncthreads();
+        sum = num = 0.0f;
+#pragma unroll
+        for (int j = 0; j < W; ++j) {
+            top = fmaxf(top, s.wave_top[j]);
+            sum += s.wave_sum[j];
+            num += s.wave_n[j];
+        }
+    }
+    __syncthreads();
+    if (!(top > -INFINITY)) {
+        for (int d = tid; d < a.draws; d += NT) {
+            a.items[row * a.draws + d] = -1;
+            a.probs[row * a.draws + d] = 0.0f;
+        }
+        return;
+    }
+    const Weigher wt{(double)top, 1.4426950408889634074 / set.t, a.unit, top, s.power};
+    const double min_w = set.min_p * a.unit;
+    // twice the way from the best to the mean holds what top-k and top-p cut between
+    const float range = 2.0f * (top - sum / num);
+    const Bins bins = make_bins(top, range, 2 * NT);
+
+    auto each = [&](auto f) {
+#pragma unroll
+        for (int j = 0; j < J; ++j) {
+            if (j < jn) {
+#pragma unroll
+                for (int e = 0; e < V; ++e) f(fresh(x[V * j + e]), (uint32_t)(first + 64 * V * j + e));
+            }
+            __builtin_amdgcn_sched_barrier(0);   // (a vector at a time: registers for one)
+        }
+    };
+    constexpr int kList = RowShared<NT>::kList;
+    constexpr float kLowest = -3.402823466e38f;
+    const bool top_k = set.k > 0 && set.k < (uint32_t)a.n;
+    // items not below a limit: in the workgroup, and (at) in the waves ahead of this one
+    uint32_t at = 0;
+    auto count_from = [&](float limit) {
+        int mine = 0;
+#pragma unroll
+        for (int j = 0; j < J; ++j) {
+            if (j < jn) {
+#pragma unroll
+                for (int e = 0; e < V; ++e) mine += lane_count(__ballot(x[V * j + e] >= limit));
+            }
+            __builtin_amdgcn_sched_barrier(0);
+        }
+        if constexpr (NT == 64) return (uint32_t)mine;
+        __syncthreads();
+        if (lane == 0) s.wave32[wave] = (uint32_t)mine;
+        __syncthreads();
+        uint32_t all = 0;
+        at = 0;
+#pragma unroll
+        for (int w = 0; w < W; ++w) {
+            const uint32_t o = s.wave32[w];
+            at += w < wave ? o : 0u;
+            all += o;
+        }
+        return all;
+    };
+    float limit = kLowest;
+    uint32_t count = kList + 1;   // of the list
+    if (a.n <= kList) {
+        count = count_from(limit);
+    } else if (top_k && set.k <= (uint32_t)kList) {
+        auto sample = [&](auto f) {
+#pragma unroll
+            for (int j = 0; j < J; ++j)
+                if (j < jn) f(fresh(x[V * j + j % V]), 0u);
+        };
+        // k / V of the sample, and four deviations more
+        const float part = (float)set.k / V;
+        CountBin cb;
+        if (count_bin((uint32_t)(part + 4.0f * sqrtf(part) + 4.0f), bins, s, sample, &cb)) limit = bins.below(cb.bin);
+        count = count_from(limit);
+        if (count < set.k && limit > kLowest) count = kList + 1;
+    }
+    Cut cut = keep_all();
+    if (top_k && count > (uint32_t)kList) {
+        CountBin cb;
+        if (count_bin(set.k, bins, s, each, &cb)) {
+            limit = bins.below(cb.bin);
+            if (cb.above + cb.in <= (uint32_t)kList) count = count_from(limit);
+            if (count > (uint32_t)kList) cut = cut_count(set.k, cb, bins, s, each);
+        }
+    }
+    if (count <= (uint32_t)kList) {
+        // ---- from a list in LDS
+#pragma unroll
+        for (int j = 0; j < J; ++j) {
+            if (j < jn) {
+                uint64_t m[V], any = 0;
+#pragma unroll
+                for (int e = 0; e < V; ++e) any |= m[e] = __ballot(x[V * j + e] >= limit);
+                if (any != 0) {
+                    uint32_t mine = at;
+#pragma unroll
+                    for (int e = 0; e < V; ++e) {
+                        mine = lanes_before(m[e], mine);
+                        at += (uint32_t)lane_count(m[e]);
+                    }
+#pragma unroll
+                    for (int e = 0; e < V; ++e)
+                        if (x[V * j + e] >= limit) {
+                            s.list_x[mine] = x[V * j + e];
+                            s.list_id[mine] = (uint32_t)(first + 64 * V * j + e);
+                            ++mine;
+                        }
+                }
+            }
+            __builtin_amdgcn_sched_barrier(0);
+        }
+        __syncthreads();
+        float y[P];   // the thread's neighbours in the list
+#pragma unroll
+        for (int e = 0; e < P; ++e) y[e] = P * tid + e < (int)count ? s.list_x[P * tid + e] : -INFINITY;
+        auto each_listed = [&](auto f) {
+#pragma unroll
+            for (int e = 0; e < P; ++e) f(y[e], (uint32_t)(P * tid + e));
+        };
+        const Bins fine = make_bins(top, limit > kLowest ? top - limit : range, 2 * NT);
+        Cut in = keep_all();
+        CountBin cb;
+        if (top_k && count > set.k && count_bin(set.k, fine, s, each_listed, &cb))
+            in = cut_count(set.k, cb, fine, s, each_listed);
+        if (!set.all_p) in = cut_weight(set.p, in, fine, wt, s, each_listed);
+        __syncthreads();
+        // weights in the order of the ids, which is the list's
+        uint32_t seen = 0;
+        if (in.partial) {
+            uint32_t mine = 0, ties;
+#pragma unroll
+            for (int e = 0; e < P; ++e) mine += y[e] == in.bound;
+            seen = before32(mine, s, &ties);
+        }
+        unsigned long long w[P], mine = 0, total;
+#pragma unroll
+        for (int e = 0; e < P; ++e) {
+            const bool out = y[e] < in.bound || (in.partial && y[e] == in.bound && seen++ >= in.ties);
+            const double real = wt.real(y[e]);
+            w[e] = !out && (real >= min_w || !(min_w > 0.0)) ? Weigher::round(real) : 0ull;
+            mine += w[e];
+        }
+        unsigned long long c = before64(mine, s, &total);
+        __syncthreads();
+#pragma unroll
+        for (int e = 0; e < P; ++e) s.before[P * tid + e] = c += w[e];   // running sums
+        __syncthreads();
+        for (int d = tid; d < a.draws; d += NT) {
+            const int64_t o = row * a.draws + d;
+            const unsigned long long target = draw_target(a, o, total);
+            int lo = 0, hi = (int)count - 1;   // the first running sum above the target
+            while (lo < hi) {
+                const int mid = (lo + hi) >> 1;
+                if (s.before[mid] > target) hi = mid;
+                else lo = mid + 1;
+            }
+            const unsigned long long got = s.before[lo] - (lo ? s.before[lo - 1] : 0ull);
+            a.items[o] = (int32_t)s.list_id[lo];
+            a.probs[o] = (float)((double)got / (double)total);
+        }
+        return;
+    }
+
+    // ---- from the registers
+    if (!set.all_p) cut = cut_weight(set.p, cut, bins, wt, s, each);
+    // equals of the bound ahead of the lane's first of V neighbours
+    auto ties_before = [&](const float* y, uint32_t ahead) {
+#pragma unroll
+        for (int e = 0; e < V; ++e) ahead = lanes_before(__ballot(y[e] == cut.bound), ahead);
+        return ahead;
+    };
+    if (cut.partial) {   // s.seg_ties: equals of the bound ahead of each segment
+        __syncthreads();
+#pragma unroll
+        for (int j = 0; j < J; ++j) {
+            if (j < jn) {
+                int mine = 0;
+#pragma unroll
+                for (int e = 0; e < V; ++e) mine += lane_count(__ballot(fresh(x[V * j + e]) == cut.bound));
+                if (lane == 0) s.seg_ties[wave * jn + j] = (uint32_t)mine;
+            }
+            __builtin_amdgcn_sched_barrier(0);
+        }
+        __syncthreads();
+        uint32_t all;
+        const uint32_t b = before32(tid < segs ? s.seg_ties[tid] : 0u, s, &all);
+        __syncthreads();
+        if (tid < segs) s.seg_ties[tid] = b;
+    }
+    __syncthreads();
+    auto weigh = [&](float y, uint32_t& seen) -> unsigned long long {
+        if (y < cut.bound) return 0;   // (-inf too)
+        if (cut.partial && y == cut.bound && seen++ >= cut.ties) return 0;
+        const double real = wt.real(y);
+        return real >= min_w || !(min_w > 0.0) ? Weigher::round(real) : 0ull;
+    };
+#pragma unroll
+    for (int j = 0; j < J; ++j) {
+        if (j < jn) {
+            uint32_t seen = cut.partial ? ties_before(x + V * j, s.seg_ties[wave * jn + j]) : 0u;
+            unsigned long long mine = 0;
+#pragma unroll
+            for (int e = 0; e < V; ++e) mine += weigh(fresh(x[V * j + e]), seen);
+            mine = lane_sums64(mine);
+            if (lane == 63) s.seg[wave * jn + j] = mine;
+        }
+        __builtin_amdgcn_sched_barrier(0);
+    }
+    __syncthreads();
+    unsigned long long total;
+    const unsigned long long seg_b = before64(tid < segs ? s.seg[tid] : 0ull, s, &total);
+    __syncthreads();
+    if (tid < segs) s.seg[tid] = seg_b;
+    __syncthreads();
+    // a wave takes a draw: the segment in which its sum passes the target, read once more
+    for (int d = wave; d < a.draws; d += W) {
+        const int64_t o = row * a.draws + d;
+        const unsigned long long target = draw_target(a, o, total);
+        int lo = 0, hi = segs - 1;   // the last segment with no more than the target ahead of it
+        while (lo < hi) {
+            const int mid = (lo + hi + 1) >> 1;
+            if (s.seg[mid] <= target) lo = mid;
+            else hi = mid - 1;
+        }
+        const int at = (lo * 64 + lane) * V;
+        float y[V];
+        load_logits<T>(a, row, at, y);
+        uint32_t seen = cut.partial ? ties_before(y, s.seg_ties[lo]) : 0u;
+        unsigned long long w[V], mine = 0;
+#pragma unroll
+        for (int e = 0; e < V; ++e) {
+            w[e] = weigh(y[e], seen);
+            mine += w[e];
+        }
+        unsigned long long c = s.seg[lo] + lane_sums64(mine) - mine;
+        if (c <= target && target < c + mine) {
+            bool open = true;
+#pragma unroll
+            for (int e = 0; e < V; ++e) {
+                if (open && target < c + w[e]) {
+                    open = false;
+                    a.items[o] = at + e;
+                    a.probs[o] = (float)((double)w[e] / (double)total);
+                }
+                c += w[e];
+            }
+        }
+    }
+}
+
+template <typename T>
+static void draw_t(const DrawArgs& a, hipStream_t st) {
+    const dim3 grid((unsigned)a.rows);
+    if (a.n <= 64 * 8) launch(k_draw_row<T, 64, 8>, grid, 64, 0, st, a);
+    else if (a.n <= 64 * 32) launch(k_draw_row<T, 64, 32>, grid, 64, 0, st, a);
+    else if (a.n <= 256 * 32) launch(k_draw_row<T, 256, 32>, grid, 256, 0, st, a);
+    else if (a.n <= 512 * 56) launch(k_draw_row<T, 512, 56>, grid, 512, 0, st, a);
+    else launch(k_draw<T>, grid, kDrawThreads, 0, st, a);
+}
+
 hipError_t launch_draw(const ncf_draw_t& c, hipStream_t st) {
     if (c.rows <= 0 || c.draws <= 0) return hipSuccess;
     DrawArgs a{};
@@ -348,11 +1110,10 @@ hipError_t launch_draw(const ncf_draw_t& c, hipStream_t st) {
     a.probs = c.probs;
     int bits = 0;
     while ((int64_t)1 << bits < c.n) ++bits;
-    a.shift = 62 - bits < 51 ? 62 - bits : 51;
-    const dim3 grid((unsigned)c.rows);
-    if (c.dtype == NCF_F32) launch(k_draw<float>, grid, kDrawThreads, 0, st, a);
-    else if (c.dtype == NCF_BF16) launch(k_draw<__bf16>, grid, kDrawThreads, 0, st, a);
-    else launch(k_draw<_Float16>, grid, kDrawThreads, 0, st, a);
+    a.unit = std::ldexp(1.0, 62 - bits < 51 ? 62 - bits : 51);
+    if (c.dtype == NCF_F32) draw_t<float>(a, st);
+    else if (c.dtype == NCF_BF16) draw_t<__bf16>(a, st);
+    else draw_t<_Float16>(a, st);
     return hipGetLastError();
 }
 

@@ -84,9 +84,8 @@ def quantize_blocks(x, tile=False):
     if cols < 1:
         raise ValueError("x has no columns")
     kb = (cols + BLOCK - 1) // BLOCK
-    with torch.cuda.device(x.device):
-        q = torch.empty(rows, (cols + 15) // 16 * 16, dtype=_FP8, device=x.device)
-        scale = torch.empty((rows + BLOCK - 1) // BLOCK if tile else rows, kb, dtype=torch.float32, device=x.device)
+    q = torch.empty(rows, (cols + 15) // 16 * 16, dtype=_FP8, device=x.device)
+    scale = torch.empty((rows + BLOCK - 1) // BLOCK if tile else rows, kb, dtype=torch.float32, device=x.device)
     if rows:
         _call(N.lib().ncf_quantize_blocks, x.device, x.data_ptr(), code, rows, cols, ld, 1 if tile else 0,
               q.data_ptr(), q.stride(0), scale.data_ptr())
@@ -113,8 +112,7 @@ def matmul_blocks(a, a_scale, b, b_scale, bias=None, out_dtype=torch.float32):
     if bias is not None:
         _dense("bias", bias, (n,), torch.float32, a.device)
     code = _dtype_code("out_dtype", out_dtype)
-    with torch.cuda.device(a.device):
-        y = torch.empty(m, n, dtype=out_dtype, device=a.device)
+    y = torch.empty(m, n, dtype=out_dtype, device=a.device)
     if m and n:
         _call(N.lib().ncf_matmul_blocks, a.device, a.data_ptr(), lda, a_scale.data_ptr(), b.data_ptr(), ldb,
               b_scale.data_ptr(), 1 if tile else 0, N.ptr(bias), m, n, k, code, y.data_ptr(), n)
@@ -164,14 +162,13 @@ def sample_items(logits, u, temperature=1.0, top_k=0, top_p=1.0, min_p=0.0, mask
         if not torch.is_tensor(mask) or mask.dtype not in (torch.bool, torch.uint8):
             raise ValueError("mask must be a bool or uint8 tensor")
         if tuple(mask.shape) == (n,):
-            mask = mask.view(1, n).expand(rows, n) if mask.is_contiguous() else mask.contiguous().expand(rows, n)
+            mask = mask.expand(rows, n)
         if tuple(mask.shape) != (rows, n):
             raise ValueError("mask must have shape (%d, %d) or (%d,), got %s" % (rows, n, n, tuple(mask.shape)))
         d.mask_ld = _matrix("mask", mask, dev)
         d.mask = mask.data_ptr()
-    with torch.cuda.device(dev):
-        items = torch.empty(u.shape, dtype=torch.int32, device=dev)
-        probs = torch.empty(u.shape, dtype=torch.float32, device=dev)
+    items = torch.empty(u.shape, dtype=torch.int32, device=dev)
+    probs = torch.empty(u.shape, dtype=torch.float32, device=dev)
     d.draws = 1 if u.dim() == 1 else u.shape[1]
     if rows and d.draws:
         d.logits, d.rows, d.n, d.ld = logits.data_ptr(), rows, n, ld
@@ -242,10 +239,9 @@ def distill_loss(logits, teacher_items, teacher_logits, temperature=1.0, teacher
     pass it in ``grad_loss``.)"""
     d = _distill(logits, teacher_items, teacher_logits, temperature, teacher_lse)
     dev = logits.device
-    with torch.cuda.device(dev):
-        loss = torch.empty(d.rows, dtype=torch.float32, device=dev)
-        state = torch.empty(d.rows, N.NCF_DISTILL_STATE, dtype=torch.float64, device=dev)
-        ws = _distill_workspace(d, dev)
+    loss = torch.empty(d.rows, dtype=torch.float32, device=dev)
+    state = torch.empty(d.rows, N.NCF_DISTILL_STATE, dtype=torch.float64, device=dev)
+    ws = _distill_workspace(d, dev)
     d.loss, d.state = loss.data_ptr(), state.data_ptr()
     if d.rows:
         _call(N.lib().ncf_distill_loss, dev, ctypes.byref(d), ws.data_ptr(), ws.numel())
@@ -258,8 +254,7 @@ def distill_grad(logits, teacher_items, teacher_logits, state, grad_loss=1.0, te
     d = _distill(logits, teacher_items, teacher_logits, temperature, teacher_lse)
     dev = logits.device
     _dense("state", state, (d.rows, N.NCF_DISTILL_STATE), torch.float64, dev)
-    with torch.cuda.device(dev):
-        grad = _distill_outputs(d, logits, grad_loss)
+    grad = _distill_outputs(d, logits, grad_loss)
     d.state = state.data_ptr()
     if d.rows:
         _call(N.lib().ncf_distill_grad, dev, ctypes.byref(d))
@@ -270,11 +265,10 @@ def distill_loss_grad(logits, teacher_items, teacher_logits, grad_loss=1.0, temp
     """:func:`distill_loss` and :func:`distill_grad` in one call: ``(loss, grad)``."""
     d = _distill(logits, teacher_items, teacher_logits, temperature, teacher_lse)
     dev = logits.device
-    with torch.cuda.device(dev):
-        loss = torch.empty(d.rows, dtype=torch.float32, device=dev)
-        state = torch.empty(d.rows, N.NCF_DISTILL_STATE, dtype=torch.float64, device=dev)
-        grad = _distill_outputs(d, logits, grad_loss)
-        ws = _distill_workspace(d, dev)
+    loss = torch.empty(d.rows, dtype=torch.float32, device=dev)
+    state = torch.empty(d.rows, N.NCF_DISTILL_STATE, dtype=torch.float64, device=dev)
+    grad = _distill_outputs(d, logits, grad_loss)
+    ws = _distill_workspace(d, dev)
     d.loss, d.state = loss.data_ptr(), state.data_ptr()
     if d.rows:
         _call(N.lib().ncf_distill_loss_grad, dev, ctypes.byref(d), ws.data_ptr(), ws.numel())
