@@ -562,7 +562,10 @@ typedef struct ncf_draw {
     int64_t top_k;
     int32_t* items;             /* [rows][draws] */
     float* probs;               /* [rows][draws] */
+    void* ws;                   /* ncf_draw_workspace_size bytes; may be NULL where that is 0 */
+    size_t ws_bytes;
 } ncf_draw_t;
+int ncf_draw_workspace_size(int64_t rows, int64_t n, size_t* bytes);
 int ncf_draw_items(const ncf_draw_t* draw, void* stream);
 
 /* Distillation from a teacher's best items (k <= NCF_DISTILL_MAX_K a row; item ids outside [0, v) are

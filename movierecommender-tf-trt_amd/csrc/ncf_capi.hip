@@ -1532,6 +1532,14 @@ int ncf_matmul_blocks(const void* a, int64_t a_ld, const float* a_scale, const v
                      "ncf_matmul_blocks");
 }
 
+int ncf_draw_workspace_size(int64_t rows, int64_t n, size_t* bytes) {
+    if (!bytes) return fail(NCF_EINVAL, "bytes is NULL");
+    if (rows < 0 || rows > INT32_MAX || n < 1 || n > INT32_MAX - 4096)   // (whole segments of items fit 32 bits)
+        return fail(NCF_EINVAL, "no workspace for %lld rows of %lld items", (long long)rows, (long long)n);
+    *bytes = ncf::draw_workspace(rows, n);
+    return 0;
+}
+
 int ncf_draw_items(const ncf_draw_t* d, void* stream) {
     if (!d) return fail(NCF_EINVAL, "draw is NULL");
     if (int r = check_dtype(d->dtype)) return r;
@@ -1542,8 +1550,12 @@ int ncf_draw_items(const ncf_draw_t* d, void* stream) {
     if (d->mask)
         if (int r = check_matrix("mask", d->mask, d->rows, d->n, d->mask_ld)) return r;
     if (!d->u || !d->items || !d->probs) return fail(NCF_EINVAL, "NULL device pointer");
-    if (d->rows > INT32_MAX || d->draws > INT32_MAX / d->rows)
+    if (ncf::draw_blocks(*d) > INT32_MAX || d->draws > INT32_MAX)
         return fail(NCF_EINVAL, "%lld rows of %lld draws are too many", (long long)d->rows, (long long)d->draws);
+    size_t need = 0;
+    if (int r = ncf_draw_workspace_size(d->rows, d->n, &need)) return r;
+    if (need && (!d->ws || d->ws_bytes < need))
+        return fail(NCF_EINVAL, "workspace of %zu bytes, need %zu", d->ws ? d->ws_bytes : (size_t)0, need);
     return hip_check(ncf::launch_draw(*d, (hipStream_t)stream), "ncf_draw_items");
 }
 

@@ -49,20 +49,13 @@ struct DrawArgs {
 
 // ----------------------------------------------------------------------------- keys and weights
 
-// unsigned keys in the order of the floats; 0 stands for an item that is not allowed
+// unsigned keys in the order of the floats
 __device__ __forceinline__ uint32_t ukey(float x) {
     const uint32_t b = __float_as_uint(x);
     return (b & 0x80000000u) ? ~b : b | 0x80000000u;
 }
 __device__ __forceinline__ float unukey(uint32_t k) {
     return __uint_as_float((k & 0x80000000u) ? k & 0x7fffffffu : ~k);
-}
-
-// -0 and 0 are equal logits: one key
-template <typename T>
-__device__ __forceinline__ uint32_t item_key(T x, bool allowed) {
-    const float f = (float)x + 0.0f;
-    return (allowed && f > -INFINITY) ? ukey(f) : 0u;   // (a NaN compares false)
 }
 
 // 2^(j / 64), filled by the compiler's exp2
@@ -98,260 +91,13 @@ struct Weigher {
     }
 };
 
-// ----------------------------------------------------------------------------- one workgroup per row
-
-constexpr int kDrawThreads = 1024;
-constexpr int kDrawBins = 2048;
-
-struct DrawShared {
-    union {
-        uint32_t count[kDrawBins];
-        unsigned long long weight[kDrawBins];
-    };
-    unsigned long long wave64[kDrawThreads / 64];
-    uint32_t wave32[kDrawThreads / 64];
-    unsigned long long pick64;
-    uint32_t pick_bin;
-    double power[kPowers];
-};
-
 __device__ __forceinline__ void fill_powers(double* power, int threads) {
     for (int j = threadIdx.x; j < kPowers; j += threads) power[j] = exp2(j * (1.0 / kPowers));
-}
-
-__device__ __forceinline__ unsigned long long shfl_up64(unsigned long long v, int d) {
-    return (unsigned long long)__shfl_up((long long)v, d, 64);
-}
-
-// exclusive prefix over the workgroup, total to *sum
-__device__ __forceinline__ unsigned long long block_before64(unsigned long long v, DrawShared& s,
-                                                             unsigned long long* sum) {
-    const int lane = threadIdx.x & 63, w = threadIdx.x >> 6;
-    unsigned long long inc = v;
-#pragma unroll
-    for (int d = 1; d < 64; d <<= 1) {
-        const unsigned long long o = shfl_up64(inc, d);
-        if (lane >= d) inc += o;
-    }
-    __syncthreads();
-    if (lane == 63) s.wave64[w] = inc;
-    __syncthreads();
-    unsigned long long before = 0, all = 0;
-    for (int j = 0; j < kDrawThreads / 64; ++j) {
-        if (j < w) before += s.wave64[j];
-        all += s.wave64[j];
-    }
-    *sum = all;
-    return before + inc - v;
-}
-
-__device__ __forceinline__ uint32_t block_before32(uint32_t v, DrawShared& s, uint32_t* sum) {
-    const int lane = threadIdx.x & 63, w = threadIdx.x >> 6;
-    uint32_t inc = v;
-#pragma unroll
-    for (int d = 1; d < 64; d <<= 1) {
-        const uint32_t o = (uint32_t)__shfl_up((int)inc, d, 64);
-        if (lane >= d) inc += o;
-    }
-    __syncthreads();
-    if (lane == 63) s.wave32[w] = inc;
-    __syncthreads();
-    uint32_t before = 0, all = 0;
-    for (int j = 0; j < kDrawThreads / 64; ++j) {
-        if (j < w) before += s.wave32[j];
-        all += s.wave32[j];
-    }
-    *sum = all;
-    return before + inc - v;
 }
 
 // (double)c >= p total, for a positive c: the one comparison that top-p makes
 __device__ __forceinline__ bool reaches(unsigned long long c, double p, double total) {
     return c > 0 && (double)c >= p * total;
-}
-
-template <typename T>
-struct RowView {
-    const T* x;
-    const uint8_t* mask;
-    int n;
-    __device__ __forceinline__ uint32_t key(int i) const {
-        return item_key(x[i], mask == nullptr || mask[i] != 0);
-    }
-};
-
-// key digits, most significant first: 11, 11 and 10 bits
-__device__ __forceinline__ int digit_shift(int level) { return level == 0 ? 21 : level == 1 ? 10 : 0; }
-__device__ __forceinline__ uint32_t digit_mask(int level) { return level == 2 ? 1023u : 2047u; }
-__device__ __forceinline__ bool same_prefix(uint32_t a, uint32_t b, int level) {
-    return level == 0 || (a >> digit_shift(level - 1)) == (b >> digit_shift(level - 1));
-}
-
-template <typename T>
-__global__ __launch_bounds__(kDrawThreads) void k_draw(DrawArgs a) {
-    __shared__ DrawShared s;
-    const int tid = threadIdx.x;
-    const int64_t row = blockIdx.x;
-    const RowView<T> r{static_cast<const T*>(a.logits) + row * a.ld, a.mask ? a.mask + row * a.mask_ld : nullptr,
-                       a.n};
-    const double t = a.temperature ? (double)a.temperature[row] : a.temperature_v;
-    const double p = a.top_p ? (double)a.top_p[row] : a.top_p_v;
-    double min_p = a.min_p ? (double)a.min_p[row] : a.min_p_v;
-    min_p = min_p > 1.0 ? 1.0 : min_p;   // the best item always stays
-    int k = a.top_k ? a.top_k[row] : a.top_k_v;
-    if (!(t > 0.0) || p <= 0.0) k = 1;
-
-    // the best item and how many are allowed
-    uint32_t top = 0, allowed = 0;
-    for (int i = tid; i < a.n; i += kDrawThreads) {
-        const uint32_t key = r.key(i);
-        top = max(top, key);
-        allowed += key != 0;
-    }
-    block_before32(allowed, s, &allowed);
-#pragma unroll
-    for (int d = 32; d >= 1; d >>= 1) top = max(top, (uint32_t)__shfl_xor((int)top, d, 64));
-    __syncthreads();
-    if ((tid & 63) == 0) s.wave32[tid >> 6] = top;
-    __syncthreads();
-    for (int j = 0; j < kDrawThreads / 64; ++j) top = max(top, s.wave32[j]);
-    __syncthreads();
-    if (allowed == 0) {
-        for (int d = tid; d < a.draws; d += kDrawThreads) {
-            a.items[row * a.draws + d] = -1;
-            a.probs[row * a.draws + d] = 0.0f;
-        }
-        return;
-    }
-    fill_powers(s.power, kDrawThreads);
-    __syncthreads();
-    const Weigher wt{(double)unukey(top), 1.4426950408889634074 / (t > 0.0 ? t : 1.0), a.unit, unukey(top), s.power};
-    const double min_w = min_p * a.unit;
-
-    // top-k: the k-th largest key, digit by digit
-    uint32_t bound = 1, ties = 0xffffffffu;   // all allowed items
-    if (k > 0 && (uint32_t)k < allowed) {
-        uint32_t left = (uint32_t)k, prefix = 0;
-        for (int level = 0; level < 3; ++level) {
-            for (int b = tid; b < kDrawBins; b += kDrawThreads) s.count[b] = 0;
-            __syncthreads();
-            for (int i = tid; i < a.n; i += kDrawThreads) {
-                const uint32_t key = r.key(i);
-                if (key != 0 && same_prefix(key, prefix, level))
-                    atomicAdd(&s.count[(key >> digit_shift(level)) & digit_mask(level)], 1u);
-            }
-            __syncthreads();
-            // from the best digit down, two bins a thread
-            const uint32_t c0 = s.count[kDrawBins - 1 - 2 * tid], c1 = s.count[kDrawBins - 2 - 2 * tid];
-            uint32_t all;
-            const uint32_t before = block_before32(c0 + c1, s, &all);
-            if (before < left && before + c0 + c1 >= left) {
-                const bool first = before + c0 >= left;
-                s.pick_bin = kDrawBins - 1 - 2 * tid - (first ? 0 : 1);
-                s.pick64 = before + (first ? 0 : c0);
-            }
-            __syncthreads();
-            prefix |= s.pick_bin << digit_shift(level);
-            left -= (uint32_t)s.pick64;
-            __syncthreads();
-        }
-        bound = prefix;
-        ties = left;
-    }
-
-    // top-p: the same over weights; of the bound's equals only `ties` count
-    if (p > 0.0 && p < 1.0) {
-        uint32_t equal = 0;
-        if (ties != 0xffffffffu) {
-            for (int i = tid; i < a.n; i += kDrawThreads) equal += r.key(i) == bound;
-            block_before32(equal, s, &equal);
-        }
-        const unsigned long long over =
-            ties != 0xffffffffu ? (unsigned long long)(equal - ties) * wt.fixed(unukey(bound)) : 0;
-        uint32_t prefix = 0;
-        unsigned long long above = 0;
-        double total = 0.0;
-        for (int level = 0; level < 3; ++level) {
-            for (int b = tid; b < kDrawBins; b += kDrawThreads) s.weight[b] = 0;
-            __syncthreads();
-            for (int i = tid; i < a.n; i += kDrawThreads) {
-                const uint32_t key = r.key(i);
-                if (key >= bound && same_prefix(key, prefix, level))
-                    atomicAdd(&s.weight[(key >> digit_shift(level)) & digit_mask(level)],
-                              wt.fixed(unukey(key)));
-            }
-            __syncthreads();
-            if (tid == 0 && over && same_prefix(bound, prefix, level))
-                s.weight[(bound >> digit_shift(level)) & digit_mask(level)] -= over;
-            __syncthreads();
-            const unsigned long long c0 = s.weight[kDrawBins - 1 - 2 * tid], c1 = s.weight[kDrawBins - 2 - 2 * tid];
-            unsigned long long all;
-            const unsigned long long before = above + block_before64(c0 + c1, s, &all);
-            if (level == 0) total = (double)all;
-            if (!reaches(before, p, total) && reaches(before + c0 + c1, p, total)) {
-                const bool first = reaches(before + c0, p, total);
-                s.pick_bin = kDrawBins - 1 - 2 * tid - (first ? 0 : 1);
-                s.pick64 = before + (first ? 0 : c0);
-            }
-            __syncthreads();
-            prefix |= s.pick_bin << digit_shift(level);
-            above = s.pick64;
-            __syncthreads();
-        }
-        // of the equals of this key, as many as it takes
-        const unsigned long long w = wt.fixed(unukey(prefix));
-        double want = ceil((p * total - (double)above) / (double)w);
-        uint32_t j = want < 1.0 ? 1u : want > (double)a.n ? (uint32_t)a.n : (uint32_t)want;
-        while (j > 1 && reaches(above + (unsigned long long)(j - 1) * w, p, total)) --j;
-        while (j < (uint32_t)a.n && !reaches(above + (unsigned long long)j * w, p, total)) ++j;
-        if (prefix > bound) {
-            bound = prefix;
-            ties = j;
-        } else {
-            ties = min(ties, j);
-        }
-    }
-
-    // segments of the row: their weight and their equals of the bound
-    const int per = (a.n + kDrawThreads - 1) / kDrawThreads;   // items of a thread, neighbours
-    const int i0 = min(tid * per, a.n), i1 = min(i0 + per, a.n);
-    uint32_t equal = 0, all32;
-    for (int i = i0; i < i1; ++i) equal += r.key(i) == bound;
-    const uint32_t ties_before = block_before32(equal, s, &all32);
-    auto weigh = [&](int i, uint32_t& seen) -> unsigned long long {
-        const uint32_t key = r.key(i);
-        if (key < bound || key == 0) return 0;
-        if (key == bound && seen++ >= ties) return 0;
-        const double w = wt.real(unukey(key));
-        return w >= min_w || !(min_w > 0.0) ? Weigher::round(w) : 0ull;
-    };
-    unsigned long long mine = 0, total;
-    {
-        uint32_t seen = ties_before;
-        for (int i = i0; i < i1; ++i) mine += weigh(i, seen);
-    }
-    const unsigned long long before = block_before64(mine, s, &total);
-    for (int d = 0; d < a.draws; ++d) {
-        const int64_t o = row * a.draws + d;
-        const double u = a.u ? a.u[o] : (double)a.u32[o];
-        const double at = u * (double)total;
-        // the first running sum above u total; a u outside [0, 1) takes the nearest end
-        unsigned long long target = at > 0.0 ? (at >= 9.2e18 ? ~0ull >> 1 : (unsigned long long)at) : 0ull;
-        if (target >= total) target = total - 1;
-        if (target >= before && target < before + mine) {
-            unsigned long long c = before;
-            uint32_t seen = ties_before;
-            for (int i = i0; i < i1; ++i) {
-                const unsigned long long w = weigh(i, seen);
-                c += w;
-                if (c > target) {
-                    a.items[o] = i;
-                    a.probs[o] = (float)((double)w / (double)total);
-                    break;
-                }
-            }
-        }
-    }
 }
 
 // ----------------------------------------------------------------------------- rows held in registers
@@ -498,9 +244,10 @@ struct Cut {
     float bound;
     uint32_t ties;
     bool partial;   // more items equal the bound than `ties`
+    uint32_t equal; // how many do (0: not known)
 };
 constexpr uint32_t kAllTies = 0xffffffffu;
-__device__ __forceinline__ Cut keep_all() { return Cut{-3.402823466e38f, kAllTies, false}; }
+__device__ __forceinline__ Cut keep_all() { return Cut{-3.402823466e38f, kAllTies, false, 0}; }
 
 // Threads' sums of two neighbouring bins, from bin 0 (the best) up, in c0 and c1: the bin at which
 // `found(before, before + bin)` holds goes to s.pick_bin, what lies before it to s.pick.
@@ -559,6 +306,77 @@ __device__ __forceinline__ bool count_bin(uint32_t k, const Bins& bins, RowShare
     return true;
 }
 
+// The k-th best of the items that each() gives, digit by digit of the key.
+template <int NT, typename Each>
+__device__ __forceinline__ Cut digits_count(uint32_t left, RowShared<NT>& s, Each each) {
+    const int tid = threadIdx.x;
+    uint32_t prefix = 0, equal = 0;
+    for (int level = 0; level < Digits<NT>::kLevels; ++level) {
+        __syncthreads();
+        s.count[2 * tid] = s.count[2 * tid + 1] = 0;
+        __syncthreads();
+        const uint32_t mask = Digits<NT>::mask(level);
+        each([&](float x, uint32_t) {
+            const uint32_t key = ukey(x + 0.0f);   // (-0 equals 0)
+            if (x > -INFINITY && Digits<NT>::same(key, prefix, level))
+                atomicAdd(&s.count[mask - ((key >> Digits<NT>::shift(level)) & mask)], 1u);
+        });
+        __syncthreads();
+        const uint32_t c0 = s.count[2 * tid], c1 = s.count[2 * tid + 1];
+        uint32_t all;
+        const uint32_t before = before32(c0 + c1, s, &all);
+        find_bin(before, c0, c1, s, [&](unsigned long long x, unsigned long long e) { return x < left && e >= left; });
+        prefix |= (mask - s.pick_bin) << Digits<NT>::shift(level);
+        left -= (uint32_t)s.pick;
+        equal = s.count[s.pick_bin];
+    }
+    return Cut{unukey(prefix), left, equal > left, equal};
+}
+
+// The item of those that each() gives at which the weight, from `ahead` on, reaches p of `all`; `over` is
+// what those equals of was.bound weigh that are beyond its ties and among these items.
+template <int NT, typename Each>
+__device__ __forceinline__ Cut digits_weight(double p, double all, unsigned long long ahead, Cut was,
+                                             unsigned long long over, const Weigher& wt, RowShared<NT>& s, Each each) {
+    const int tid = threadIdx.x;
+    uint32_t prefix = 0;
+    const uint32_t bound_key = ukey(was.bound + 0.0f);
+    for (int level = 0; level < Digits<NT>::kLevels; ++level) {
+        __syncthreads();
+        s.weight[2 * tid] = s.weight[2 * tid + 1] = 0;
+        __syncthreads();
+        const uint32_t mask = Digits<NT>::mask(level);
+        each([&](float x, uint32_t) {
+            const uint32_t key = ukey(x + 0.0f);
+            if (x >= was.bound && Digits<NT>::same(key, prefix, level))
+                atomicAdd(&s.weight[mask - ((key >> Digits<NT>::shift(level)) & mask)], wt.fixed(x));
+        });
+        __syncthreads();
+        if (tid == 0 && over && Digits<NT>::same(bound_key, prefix, level))
+            s.weight[mask - ((bound_key >> Digits<NT>::shift(level)) & mask)] -= over;
+        __syncthreads();
+        const unsigned long long c0 = s.weight[2 * tid], c1 = s.weight[2 * tid + 1];
+        unsigned long long level_sum;
+        const unsigned long long before = ahead + before64(c0 + c1, s, &level_sum);
+        find_bin(before, c0, c1, s,
+                 [&](unsigned long long x, unsigned long long e) { return !reaches(x, p, all) && reaches(e, p, all); });
+        prefix |= (mask - s.pick_bin) << Digits<NT>::shift(level);
+        ahead = s.pick;
+    }
+    const float bound = unukey(prefix);
+    uint32_t equal = 0;
+    each([&](float x, uint32_t) { equal += x == bound; });
+    before32(equal, s, &equal);
+    // of the equals of this logit, as many as it takes
+    const uint32_t most = bound == was.bound && was.partial ? was.ties : equal;
+    const unsigned long long w = wt.fixed(bound);
+    const double want = ceil((p * all - (double)ahead) / (double)w);
+    uint32_t j = want < 1.0 ? 1u : want > (double)most ? most : (uint32_t)want;
+    while (j > 1 && reaches(ahead + (unsigned long long)(j - 1) * w, p, all)) --j;
+    while (j < most && !reaches(ahead + (unsigned long long)j * w, p, all)) ++j;
+    return Cut{bound, j, equal > j, equal};
+}
+
 // Its bound.
 template <int NT, typename Each>
 __device__ __forceinline__ Cut cut_count(uint32_t k, const CountBin& in, const Bins& bins, RowShared<NT>& s,
@@ -591,29 +409,9 @@ __device__ __forceinline__ Cut cut_count(uint32_t k, const CountBin& in, const B
             }
         }
         __syncthreads();
-        return Cut{s.bound, s.ties, s.equal > s.ties};
+        return Cut{s.bound, s.ties, s.equal > s.ties, s.equal};
     }
-    uint32_t prefix = 0, equal = 0, left = k;
-    for (int level = 0; level < Digits<NT>::kLevels; ++level) {
-        __syncthreads();
-        s.count[2 * tid] = s.count[2 * tid + 1] = 0;
-        __syncthreads();
-        const uint32_t mask = Digits<NT>::mask(level);
-        each([&](float x, uint32_t) {
-            const uint32_t key = ukey(x + 0.0f);   // (-0 equals 0)
-            if (x > -INFINITY && Digits<NT>::same(key, prefix, level))
-                atomicAdd(&s.count[mask - ((key >> Digits<NT>::shift(level)) & mask)], 1u);
-        });
-        __syncthreads();
-        const uint32_t c0 = s.count[2 * tid], c1 = s.count[2 * tid + 1];
-        uint32_t all;
-        const uint32_t before = before32(c0 + c1, s, &all);
-        find_bin(before, c0, c1, s, [&](unsigned long long x, unsigned long long e) { return x < left && e >= left; });
-        prefix |= (mask - s.pick_bin) << Digits<NT>::shift(level);
-        left -= (uint32_t)s.pick;
-        equal = s.count[s.pick_bin];
-    }
-    return Cut{unukey(prefix), left, equal > left};
+    return digits_count(k, s, each);
 }
 
 // The shortest leading list with at least p of the weight, inside what `was` keeps.
@@ -681,45 +479,9 @@ __device__ __forceinline__ Cut cut_weight(double p, Cut was, const Bins& bins, c
             }
         }
         __syncthreads();
-        return Cut{s.bound, s.ties, s.equal > s.ties};
+        return Cut{s.bound, s.ties, s.equal > s.ties, s.equal};
     }
-    uint32_t prefix = 0;
-    unsigned long long ahead = 0;
-    const uint32_t bound_key = ukey(was.bound + 0.0f);
-    for (int level = 0; level < Digits<NT>::kLevels; ++level) {
-        __syncthreads();
-        s.weight[2 * tid] = s.weight[2 * tid + 1] = 0;
-        __syncthreads();
-        const uint32_t mask = Digits<NT>::mask(level);
-        each([&](float x, uint32_t) {
-            const uint32_t key = ukey(x + 0.0f);   // (-0 equals 0)
-            if (x >= was.bound && Digits<NT>::same(key, prefix, level))
-                atomicAdd(&s.weight[mask - ((key >> Digits<NT>::shift(level)) & mask)], wt.fixed(x));
-        });
-        __syncthreads();
-        if (tid == 0 && over && Digits<NT>::same(bound_key, prefix, level))
-            s.weight[mask - ((bound_key >> Digits<NT>::shift(level)) & mask)] -= over;
-        __syncthreads();
-        c0 = s.weight[2 * tid];
-        c1 = s.weight[2 * tid + 1];
-        unsigned long long level_sum;
-        const unsigned long long before = ahead + before64(c0 + c1, s, &level_sum);
-        find_bin(before, c0, c1, s, found);
-        prefix |= (mask - s.pick_bin) << Digits<NT>::shift(level);
-        ahead = s.pick;
-    }
-    const float bound = unukey(prefix);
-    uint32_t equal = 0;
-    each([&](float x, uint32_t) { equal += x == bound; });
-    before32(equal, s, &equal);
-    // of the equals of this logit, as many as it takes
-    const uint32_t most = bound == was.bound && was.partial ? was.ties : equal;
-    const unsigned long long w = wt.fixed(bound);
-    const double want = ceil((p * all - (double)ahead) / (double)w);
-    uint32_t j = want < 1.0 ? 1u : want > (double)most ? most : (uint32_t)want;
-    while (j > 1 && reaches(ahead + (unsigned long long)(j - 1) * w, p, all)) --j;
-    while (j < most && !reaches(ahead + (unsigned long long)j * w, p, all)) ++j;
-    return Cut{bound, j, equal > j};
+    return digits_weight(p, all, 0ull, was, over, wt, s, each);
 }
 
 struct RowSettings {
@@ -1076,14 +838,556 @@ __global__ __launch_bounds__(NT) void k_draw_row(DrawArgs a) {
     }
 }
 
+// ----------------------------------------------------------------------------- long rows
+//
+// A row longer than the registers of a workgroup is cut into parts, a workgroup each, and passed over by
+// a few launches that hand on what they find in a workspace: the best item; per cut (top-k by counts,
+// top-p by weights) the histogram over kLongBins steps of the logit, the items of the bin that holds the
+// cut, and the bound among them (one workgroup a row; where the items outgrow their list it reads the row
+// again instead); the weight of every segment of 64 vectors; the draws.  The row comes from memory once
+// and from the caches after that (1,000,000 items are 2 or 4 MB).
+
+constexpr int kLongThreads = 256;
+constexpr int kLongWaves = kLongThreads / 64;
+constexpr int kLongBins = 2048;
+constexpr int kResolveThreads = 512;
+
+struct LongRow {
+    float bound;
+    uint32_t ties, partial, equal;            // the cut so far
+    uint32_t members;                         // items of the bin, as far as they are gathered
+    int bin;                                  // -1: no cut to make
+    uint32_t above_n;
+    unsigned long long above_w, total_w;
+};
+
+struct LongArgs {
+    DrawArgs a;
+    int parts, part;          // parts of a row, items of a part (whole segments)
+    int segs;                 // segments of a row
+    uint32_t cap;             // of a row's list
+    float* tops;              // [rows][parts] best, sum and number of usual logits
+    float* sums;
+    float* nums;
+    uint32_t* count;          // [rows][kLongBins]
+    unsigned long long* weight;
+    LongRow* row;
+    uint2* list;              // [rows][cap] logit bits, id
+    unsigned long long* seg;  // [rows][segs]
+    uint32_t* seg_ties;
+};
+
 template <typename T>
-static void draw_t(const DrawArgs& a, hipStream_t st) {
+__host__ __device__ constexpr int seg_items() { return 64 * Elem<T>::kVec; }
+
+// the part's logits, a vector at a time: f(logits, first id), `part` of row `r`
+template <typename T, typename F>
+__device__ __forceinline__ void each_vector(const LongArgs& l, int64_t r, int part, F f) {
+    constexpr int V = Elem<T>::kVec, U = 4;
+    const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, step = (int)(blockDim.x >> 6);
+    const int s0 = part * (l.part / seg_items<T>()), s1 = min(l.segs, s0 + l.part / seg_items<T>());
+    for (int sg = s0 + wave; sg < s1; sg += U * step) {
+        float y[U][V];
+#pragma unroll
+        for (int u = 0; u < U; ++u)   // (segments past the part: past the row's end, or not used)
+            load_logits<T>(l.a, r, sg + u * step < s1 ? (sg + u * step) * seg_items<T>() + lane * V : l.a.n, y[u]);
+#pragma unroll
+        for (int u = 0; u < U; ++u)
+            if (sg + u * step < s1) f(y[u], (sg + u * step) * seg_items<T>() + lane * V);
+    }
+}
+
+struct LongShared {
+    union {
+        uint32_t count[kLongBins];
+        unsigned long long weight[kLongBins];
+    };
+    double power[kPowers];
+    unsigned long long wave64[kLongWaves], pick;
+    uint32_t wave32[kLongWaves];
+    float wavef[3][kLongWaves];
+    int pick_bin;
+};
+
+template <typename T>
+__global__ __launch_bounds__(kLongThreads) void k_long_top(LongArgs l) {
+    __shared__ LongShared s;
+    const int64_t r = blockIdx.x / l.parts;
+    const int part = (int)(blockIdx.x - r * l.parts), tid = threadIdx.x;
+    for (int b = part * kLongThreads + tid; b < kLongBins; b += l.parts * kLongThreads) {
+        l.count[r * kLongBins + b] = 0;
+        l.weight[r * kLongBins + b] = 0;
+    }
+    float top = -INFINITY, sum = 0.0f, num = 0.0f;
+    each_vector<T>(l, r, part, [&](const float* y, int) {
+#pragma unroll
+        for (int e = 0; e < Elem<T>::kVec; ++e) {
+            top = fmaxf(top, y[e]);
+            const bool usual = fabsf(y[e]) < 1e30f;
+            sum += usual ? y[e] : 0.0f;
+            num += usual ? 1.0f : 0.0f;
+        }
+    });
+#pragma unroll
+    for (int d = 32; d >= 1; d >>= 1) {
+        top = fmaxf(top, __shfl_xor(top, d, 64));
+        sum += __shfl_xor(sum, d, 64);
+        num += __shfl_xor(num, d, 64);
+    }
+    if ((tid & 63) == 0) {
+        s.wavef[0][tid >> 6] = top;
+        s.wavef[1][tid >> 6] = sum;
+        s.wavef[2][tid >> 6] = num;
+    }
+    __syncthreads();
+    if (tid == 0) {
+        for (int w = 1; w < kLongWaves; ++w) {
+            top = fmaxf(top, s.wavef[0][w]);
+            sum += s.wavef[1][w];
+            num += s.wavef[2][w];
+        }
+        l.tops[blockIdx.x] = top;
+        l.sums[blockIdx.x] = sum;
+        l.nums[blockIdx.x] = num;
+        if (part == 0) {
+            LongRow z{};
+            const Cut all = keep_all();
+            z.bound = all.bound;
+            z.ties = all.ties;
+            z.bin = -1;
+            l.row[r] = z;
+        }
+    }
+}
+
+// the row's best logit and its bins, from the parts' (every workgroup in the same order)
+__device__ __forceinline__ Bins long_bins(const LongArgs& l, int64_t r) {
+    const int lane = threadIdx.x & 63;
+    float top = -INFINITY, sum = 0.0f, num = 0.0f;
+    for (int p = lane; p < l.parts; p += 64) {
+        top = fmaxf(top, l.tops[r * l.parts + p]);
+        sum += l.sums[r * l.parts + p];
+        num += l.nums[r * l.parts + p];
+    }
+#pragma unroll
+    for (int d = 32; d >= 1; d >>= 1) {
+        top = fmaxf(top, __shfl_xor(top, d, 64));
+        sum += __shfl_xor(sum, d, 64);
+        num += __shfl_xor(num, d, 64);
+    }
+    return make_bins(top, 2.0f * (top - sum / num), kLongBins);
+}
+__device__ __forceinline__ Weigher long_weigher(const LongArgs& l, const Bins& bins, const RowSettings& set,
+                                                const double* power) {
+    return Weigher{(double)bins.top, 1.4426950408889634074 / set.t, l.a.unit, bins.top, power};
+}
+__device__ __forceinline__ Cut row_cut(const LongRow& w) { return Cut{w.bound, w.ties, w.partial != 0, w.equal}; }
+__device__ __forceinline__ bool wants_cut(const LongArgs& l, const RowSettings& set, bool weights) {
+    return weights ? !set.all_p : set.k > 0 && set.k < (uint32_t)l.a.n;
+}
+
+template <typename T, bool WEIGHTS>
+__global__ __launch_bounds__(kLongThreads) void k_long_histogram(LongArgs l) {
+    __shared__ LongShared s;
+    const int64_t r = blockIdx.x / l.parts;
+    const int part = (int)(blockIdx.x - r * l.parts), tid = threadIdx.x;
+    const RowSettings set = row_settings(l.a, r);
+    if (!wants_cut(l, set, WEIGHTS)) return;
+    const Bins bins = long_bins(l, r);
+    if (!(bins.top > -INFINITY)) return;
+    for (int b = tid; b < kLongBins; b += kLongThreads) {
+        if constexpr (WEIGHTS) s.weight[b] = 0;
+        else s.count[b] = 0;
+    }
+    fill_powers(s.power, kLongThreads);
+    __syncthreads();
+    const Weigher wt = long_weigher(l, bins, set, s.power);
+    const float bound = l.row[r].bound;
+    each_vector<T>(l, r, part, [&](const float* y, int) {
+#pragma unroll
+        for (int e = 0; e < Elem<T>::kVec; ++e) {
+            if (!(y[e] >= bound)) continue;   // (-inf too)
+            if constexpr (WEIGHTS) atomicAdd(&s.weight[bins.of(y[e])], wt.fixed(y[e]));
+            else atomicAdd(&s.count[bins.of(y[e])], 1u);
+        }
+    });
+    __syncthreads();
+    for (int b = tid; b < kLongBins; b += kLongThreads) {
+        if constexpr (WEIGHTS) {
+            if (s.weight[b]) atomicAdd(&l.weight[r * kLongBins + b], s.weight[b]);
+        } else {
+            if (s.count[b]) atomicAdd(&l.count[r * kLongBins + b], s.count[b]);
+        }
+    }
+}
+
+// exclusive sums over the workgroup
+__device__ __forceinline__ unsigned long long long_before(unsigned long long v, LongShared& s,
+                                                          unsigned long long* sum) {
+    const int lane = threadIdx.x & 63, w = threadIdx.x >> 6;
+    const unsigned long long inc = lane_sums64(v);
+    __syncthreads();
+    if (lane == 63) s.wave64[w] = inc;
+    __syncthreads();
+    unsigned long long before = 0, all = 0;
+#pragma unroll
+    for (int j = 0; j < kLongWaves; ++j) {
+        before += j < w ? s.wave64[j] : 0ull;
+        all += s.wave64[j];
+    }
+    *sum = all;
+    return before + inc - v;
+}
+
+// The bin of the cut (every workgroup of a row finds the same), and its items to the row's list.
+template <typename T, bool WEIGHTS>
+__global__ __launch_bounds__(kLongThreads) void k_long_gather(LongArgs l) {
+    __shared__ LongShared s;
+    constexpr int kPer = kLongBins / kLongThreads;
+    const int64_t r = blockIdx.x / l.parts;
+    const int part = (int)(blockIdx.x - r * l.parts), tid = threadIdx.x;
+    const RowSettings set = row_settings(l.a, r);
+    if (!wants_cut(l, set, WEIGHTS)) return;
+    const Bins bins = long_bins(l, r);
+    if (!(bins.top > -INFINITY)) return;
+    fill_powers(s.power, kLongThreads);
+    if (tid == 0) s.pick_bin = -1;
+    __syncthreads();
+    const Cut was = row_cut(l.row[r]);
+    unsigned long long c[kPer], mine = 0, total;
+#pragma unroll
+    for (int b = 0; b < kPer; ++b) {
+        const int64_t at = r * kLongBins + kPer * tid + b;
+        c[b] = WEIGHTS ? l.weight[at] : (unsigned long long)l.count[at];
+    }
+    if (WEIGHTS && was.partial) {   // equals of top-k's bound beyond its ties
+        const Weigher wt = long_weigher(l, bins, set, s.power);
+        const int at = bins.of(was.bound);
+#pragma unroll
+        for (int b = 0; b < kPer; ++b)
+            if (kPer * tid + b == at) c[b] -= (unsigned long long)(was.equal - was.ties) * wt.fixed(was.bound);
+    }
+#pragma unroll
+    for (int b = 0; b < kPer; ++b) mine += c[b];
+    unsigned long long ahead = long_before(mine, s, &total);
+    const double all = (double)total;
+    if (WEIGHTS || total > set.k) {
+#pragma unroll
+        for (int b = 0; b < kPer; ++b) {
+            const unsigned long long e = ahead + c[b];
+            const bool found = WEIGHTS ? !reaches(ahead, set.p, all) && reaches(e, set.p, all)
+                                       : ahead < set.k && e >= set.k;
+            if (found) {
+                s.pick_bin = kPer * tid + b;
+                s.pick = ahead;
+            }
+            ahead = e;
+        }
+    }
+    __syncthreads();
+    const int bin = s.pick_bin;
+    if (part == 0 && tid == 0) {
+        l.row[r].bin = bin;
+        l.row[r].above_n = (uint32_t)s.pick;
+        l.row[r].above_w = s.pick;
+        l.row[r].total_w = total;
+    }
+    if (bin < 0) return;
+    each_vector<T>(l, r, part, [&](const float* y, int id) {
+#pragma unroll
+        for (int e = 0; e < Elem<T>::kVec; ++e) {
+            const bool in = y[e] >= was.bound && bins.of(y[e]) == bin;
+            const uint64_t m = __ballot(in);
+            if (m == 0) continue;
+            // one reservation a wave
+            uint32_t base = 0;
+            if ((tid & 63) == __builtin_ctzll(m)) base = atomicAdd(&l.row[r].members, (uint32_t)lane_count(m));
+            base = (uint32_t)__builtin_amdgcn_readlane((int)base, __builtin_ctzll(m));
+            const uint32_t at = lanes_before(m, base);
+            if (in && at < l.cap) l.list[r * l.cap + at] = make_uint2(__float_as_uint(y[e]), (uint32_t)(id + e));
+        }
+    });
+}
+
+// The bound among the items of the bin; a workgroup a row.
+template <typename T, bool WEIGHTS>
+__global__ __launch_bounds__(kResolveThreads) void k_long_resolve(LongArgs l) {
+    __shared__ RowShared<kResolveThreads> s;
+    const int64_t r = blockIdx.x;
+    const int tid = threadIdx.x;
+    const RowSettings set = row_settings(l.a, r);
+    if (!wants_cut(l, set, WEIGHTS)) return;
+    const LongRow w = l.row[r];
+    const Bins bins = long_bins(l, r);
+    if (!(bins.top > -INFINITY) || w.bin < 0) return;
+    fill_powers(s.power, kResolveThreads);
+    __syncthreads();
+    const Cut was = row_cut(w);
+    const Weigher wt = long_weigher(l, bins, set, s.power);
+    const unsigned long long over =
+        WEIGHTS && was.partial && bins.of(was.bound) == w.bin
+            ? (unsigned long long)(was.equal - was.ties) * wt.fixed(was.bound) : 0ull;
+    auto bound_of = [&](auto each) {
+        if constexpr (WEIGHTS)
+            return digits_weight(set.p, (double)w.total_w, w.above_w, was, over, wt, s, each);
+        else
+            return digits_count(set.k - w.above_n, s, each);
+    };
+    Cut cut;
+    if (w.members <= l.cap) {
+        cut = bound_of([&](auto f) {
+            for (uint32_t i = tid; i < w.members; i += kResolveThreads) {
+                const uint2 m = l.list[r * l.cap + i];
+                f(__uint_as_float(m.x), m.y);
+            }
+        });
+    } else {
+        LongArgs whole = l;   // (the row as one part)
+        whole.part = l.segs * seg_items<T>();
+        cut = bound_of([&](auto f) {
+            each_vector<T>(whole, r, 0, [&](const float* y, int id) {
+#pragma unroll
+                for (int e = 0; e < Elem<T>::kVec; ++e)
+                    if (y[e] >= was.bound && bins.of(y[e]) == w.bin) f(y[e], (uint32_t)(id + e));
+            });
+        });
+    }
+    __syncthreads();
+    if (tid == 0) {
+        LongRow n = w;
+        n.bound = cut.bound;
+        n.ties = cut.ties;
+        n.partial = cut.partial;
+        n.equal = cut.equal;
+        n.members = 0;
+        n.bin = -1;
+        l.row[r] = n;
+    }
+}
+
+// weights of V neighbours, of which `seen` equals of the bound lie ahead
+template <int V>
+__device__ __forceinline__ unsigned long long weigh_vector(const float* y, uint32_t seen, const Cut& cut,
+                                                           const Weigher& wt, double min_w, unsigned long long* w) {
+    unsigned long long sum = 0;
+#pragma unroll
+    for (int e = 0; e < V; ++e) {
+        w[e] = 0;
+        if (y[e] >= cut.bound && !(cut.partial && y[e] == cut.bound && seen++ >= cut.ties)) {
+            const double real = wt.real(y[e]);
+            if (real >= min_w || !(min_w > 0.0)) w[e] = Weigher::round(real);
+        }
+        sum += w[e];
+    }
+    return sum;
+}
+
+// Equals of a partial bound in every segment.
+template <typename T>
+__global__ __launch_bounds__(kLongThreads) void k_long_ties(LongArgs l) {
+    const int64_t r = blockIdx.x / l.parts;
+    const int part = (int)(blockIdx.x - r * l.parts);
+    const Cut cut = row_cut(l.row[r]);
+    if (!cut.partial) return;
+    each_vector<T>(l, r, part, [&](const float* y, int id) {
+        int n = 0;
+#pragma unroll
+        for (int e = 0; e < Elem<T>::kVec; ++e) n += lane_count(__ballot(y[e] == cut.bound));
+        if ((threadIdx.x & 63) == 0) l.seg_ties[r * l.segs + id / seg_items<T>()] = (uint32_t)n;
+    });
+}
+
+// equals of the bound ahead of a segment; each lane a share of the segments before it
+__device__ __forceinline__ uint32_t ties_ahead(const LongArgs& l, int64_t r, int from, int to) {
+    uint32_t n = 0;
+    for (int g = from + (int)(threadIdx.x & 63); g < to; g += 64) n += l.seg_ties[r * l.segs + g];
+    return lane63(lane_sums32(n));
+}
+
+// The weight of every segment.
+template <typename T>
+__global__ __launch_bounds__(kLongThreads) void k_long_weigh(LongArgs l) {
+    __shared__ double power[kPowers];
+    constexpr int V = Elem<T>::kVec;
+    const int64_t r = blockIdx.x / l.parts;
+    const int part = (int)(blockIdx.x - r * l.parts), lane = threadIdx.x & 63;
+    const RowSettings set = row_settings(l.a, r);
+    const Bins bins = long_bins(l, r);
+    if (!(bins.top > -INFINITY)) return;
+    fill_powers(power, kLongThreads);
+    __syncthreads();
+    const Weigher wt = long_weigher(l, bins, set, power);
+    const double min_w = set.min_p * l.a.unit;
+    const Cut cut = row_cut(l.row[r]);
+    int done = 0;             // segments whose equals are counted in `ahead`
+    uint32_t ahead = 0;
+    each_vector<T>(l, r, part, [&](const float* y, int id) {
+        const int g = id / seg_items<T>();
+        uint32_t seen = 0;
+        if (cut.partial) {
+            ahead += ties_ahead(l, r, done, g);
+            done = g;
+            seen = ahead;
+#pragma unroll
+            for (int e = 0; e < V; ++e) seen = lanes_before(__ballot(y[e] == cut.bound), seen);
+        }
+        unsigned long long w[V];
+        const unsigned long long sum = lane_sums64(weigh_vector<V>(y, seen, cut, wt, min_w, w));
+        if (lane == 63) l.seg[r * l.segs + g] = sum;
+    });
+}
+
+// A draw of a row: the segment in which the running sum passes the target, then the item in it.
+template <typename T>
+__global__ __launch_bounds__(kLongThreads) void k_long_draw(LongArgs l) {
+    __shared__ LongShared s;
+    constexpr int V = Elem<T>::kVec;
+    const int64_t o = blockIdx.x, r = o / l.a.draws;
+    const int tid = threadIdx.x, lane = tid & 63;
+    const RowSettings set = row_settings(l.a, r);
+    const Bins bins = long_bins(l, r);
+    if (!(bins.top > -INFINITY)) {
+        if (tid == 0) {
+            l.a.items[o] = -1;
+            l.a.probs[o] = 0.0f;
+        }
+        return;
+    }
+    fill_powers(s.power, kLongThreads);
+    // a thread's share of the segments
+    const int per = (l.segs + kLongThreads - 1) / kLongThreads;
+    const int g0 = min(tid * per, l.segs), g1 = min(g0 + per, l.segs);
+    const unsigned long long* seg = l.seg + r * l.segs;
+    unsigned long long mine = 0, total;
+    for (int g = g0; g < g1; ++g) mine += seg[g];
+    unsigned long long c = long_before(mine, s, &total);
+    const unsigned long long target = draw_target(l.a, o, total);
+    if (c <= target && target < c + mine) {
+        for (int g = g0; g < g1; ++g) {
+            if (target < c + seg[g]) {
+                s.pick_bin = g;
+                s.pick = c;
+                break;
+            }
+            c += seg[g];
+        }
+    }
+    __syncthreads();
+    if (tid >= 64) return;
+    const int g = s.pick_bin, at = g * seg_items<T>() + lane * V;
+    const Weigher wt = long_weigher(l, bins, set, s.power);
+    const Cut cut = row_cut(l.row[r]);
+    float y[V];
+    load_logits<T>(l.a, r, at, y);
+    uint32_t seen = 0;
+    if (cut.partial) {
+        seen = ties_ahead(l, r, 0, g);
+#pragma unroll
+        for (int e = 0; e < V; ++e) seen = lanes_before(__ballot(y[e] == cut.bound), seen);
+    }
+    unsigned long long w[V];
+    const unsigned long long sum = weigh_vector<V>(y, seen, cut, wt, set.min_p * l.a.unit, w);
+    c = s.pick + lane_sums64(sum) - sum;
+    if (c <= target && target < c + sum) {
+        bool open = true;
+#pragma unroll
+        for (int e = 0; e < V; ++e) {
+            if (open && target < c + w[e]) {
+                open = false;
+                l.a.items[o] = at + e;
+                l.a.probs[o] = (float)((double)w[e] / (double)total);
+            }
+            c += w[e];
+        }
+    }
+}
+
+// workspace of the long path (sizes by the narrower vector, so it serves every element type)
+struct LongLayout {
+    int64_t parts, segs, cap;
+    size_t tops, count, weight, row, list, seg, seg_ties, total;
+};
+static LongLayout long_layout(int64_t rows, int64_t n, int vec) {
+    LongLayout l{};
+    const int64_t seg = 64 * vec;
+    l.segs = (n + seg - 1) / seg;
+    // about 1024 workgroups, four a CU, of at least four segments for each of their waves
+    l.parts = 1024 / rows;
+    const int64_t most = (l.segs + 4 * kLongWaves - 1) / (4 * kLongWaves);
+    l.parts = l.parts < 1 ? 1 : l.parts > most ? most : l.parts;
+    // lists of 64 MB together: 2,048 items at least, 65,536 at most
+    l.cap = ((int64_t)8 << 20) / rows;
+    l.cap = l.cap < 2048 ? 2048 : l.cap > 65536 ? 65536 : l.cap;
+    size_t off = 0;
+    auto take = [&](size_t bytes) {
+        const size_t at = off;
+        off = (off + bytes + 255) / 256 * 256;
+        return at;
+    };
+    l.tops = take((size_t)rows * l.parts * 3 * sizeof(float));
+    l.count = take((size_t)rows * kLongBins * sizeof(uint32_t));
+    l.weight = take((size_t)rows * kLongBins * sizeof(unsigned long long));
+    l.row = take((size_t)rows * sizeof(LongRow));
+    l.list = take((size_t)rows * l.cap * sizeof(uint2));
+    l.seg = take((size_t)rows * l.segs * sizeof(unsigned long long));
+    l.seg_ties = take((size_t)rows * l.segs * sizeof(uint32_t));
+    l.total = off;
+    return l;
+}
+
+constexpr int kRowMost = 512 * 56;   // the longest row that two workgroups a CU hold in registers
+
+size_t draw_workspace(int64_t rows, int64_t n) {
+    return rows > 0 && n > kRowMost ? long_layout(rows, n, Elem<float>::kVec).total : 0;
+}
+int64_t draw_blocks(const ncf_draw_t& d) {
+    const int64_t draws = d.rows > INT64_MAX / (d.draws > 0 ? d.draws : 1) ? INT64_MAX : d.rows * d.draws;
+    return draws > d.rows ? draws : d.rows;   // (parts only where rows are few)
+}
+
+template <typename T>
+static void draw_long(const DrawArgs& a, void* ws, bool may_k, bool may_p, hipStream_t st) {
+    const LongLayout y = long_layout(a.rows, a.n, Elem<T>::kVec);
+    LongArgs l{};
+    l.a = a;
+    l.parts = (int)y.parts;
+    l.segs = (int)y.segs;
+    l.part = (int)((y.segs + y.parts - 1) / y.parts) * seg_items<T>();
+    l.cap = (uint32_t)y.cap;
+    l.tops = at<float>(ws, y.tops);
+    l.sums = l.tops + a.rows * y.parts;
+    l.nums = l.sums + a.rows * y.parts;
+    l.count = at<uint32_t>(ws, y.count);
+    l.weight = at<unsigned long long>(ws, y.weight);
+    l.row = at<LongRow>(ws, y.row);
+    l.list = at<uint2>(ws, y.list);
+    l.seg = at<unsigned long long>(ws, y.seg);
+    l.seg_ties = at<uint32_t>(ws, y.seg_ties);
+    const dim3 grid((unsigned)(a.rows * y.parts)), rows((unsigned)a.rows);
+    launch(k_long_top<T>, grid, kLongThreads, 0, st, l);
+    if (may_k) {
+        launch(k_long_histogram<T, false>, grid, kLongThreads, 0, st, l);
+        launch(k_long_gather<T, false>, grid, kLongThreads, 0, st, l);
+        launch(k_long_resolve<T, false>, rows, kResolveThreads, 0, st, l);
+    }
+    if (may_p) {
+        launch(k_long_histogram<T, true>, grid, kLongThreads, 0, st, l);
+        launch(k_long_gather<T, true>, grid, kLongThreads, 0, st, l);
+        launch(k_long_resolve<T, true>, rows, kResolveThreads, 0, st, l);
+    }
+    if (may_k || may_p) launch(k_long_ties<T>, grid, kLongThreads, 0, st, l);
+    launch(k_long_weigh<T>, grid, kLongThreads, 0, st, l);
+    launch(k_long_draw<T>, dim3((unsigned)(a.rows * a.draws)), kLongThreads, 0, st, l);
+}
+
+template <typename T>
+static void draw_t(const DrawArgs& a, void* ws, bool may_k, bool may_p, hipStream_t st) {
     const dim3 grid((unsigned)a.rows);
     if (a.n <= 64 * 8) launch(k_draw_row<T, 64, 8>, grid, 64, 0, st, a);
     else if (a.n <= 64 * 32) launch(k_draw_row<T, 64, 32>, grid, 64, 0, st, a);
     else if (a.n <= 256 * 32) launch(k_draw_row<T, 256, 32>, grid, 256, 0, st, a);
-    else if (a.n <= 512 * 56) launch(k_draw_row<T, 512, 56>, grid, 512, 0, st, a);
-    else launch(k_draw<T>, grid, kDrawThreads, 0, st, a);
+    else if (a.n <= kRowMost) launch(k_draw_row<T, 512, 56>, grid, 512, 0, st, a);
+    else draw_long<T>(a, ws, may_k, may_p, st);
 }
 
 hipError_t launch_draw(const ncf_draw_t& c, hipStream_t st) {
@@ -1111,9 +1415,12 @@ hipError_t launch_draw(const ncf_draw_t& c, hipStream_t st) {
     int bits = 0;
     while ((int64_t)1 << bits < c.n) ++bits;
     a.unit = std::ldexp(1.0, 62 - bits < 51 ? 62 - bits : 51);
-    if (c.dtype == NCF_F32) draw_t<float>(a, st);
-    else if (c.dtype == NCF_BF16) draw_t<__bf16>(a, st);
-    else draw_t<_Float16>(a, st);
+    // which cuts some row may ask for
+    const bool greedy = c.temperature_rows || !(c.temperature > 0.0) || c.top_p_rows || !(c.top_p > 0.0);
+    const bool may_k = c.top_k_rows || c.top_k > 0 || greedy, may_p = c.top_p_rows || c.top_p < 1.0;
+    if (c.dtype == NCF_F32) draw_t<float>(a, c.ws, may_k, may_p, st);
+    else if (c.dtype == NCF_BF16) draw_t<__bf16>(a, c.ws, may_k, may_p, st);
+    else draw_t<_Float16>(a, c.ws, may_k, may_p, st);
     return hipGetLastError();
 }
 

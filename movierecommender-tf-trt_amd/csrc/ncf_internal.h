@@ -1001,8 +1001,11 @@ hipError_t launch_matmul_blocks(const uint8_t* a, int64_t lda, const float* sa, 
                                 const float* sb, int b_tile, const float* bias, int64_t m, int64_t n, int k,
                                 int out_dtype, void* y, int64_t ldy, hipStream_t st);
 
-hipError_t launch_draw(const ncf_draw_t& d, hipStream_t st);                                   // ncf_draw.hip
-size_t distill_workspace(int64_t rows, int v);                                                // ncf_distill.hip
+// drawing items (ncf_draw.hip), distillation (ncf_distill.hip)
+hipError_t launch_draw(const ncf_draw_t& d, hipStream_t st);
+size_t draw_workspace(int64_t rows, int64_t n);
+int64_t draw_blocks(const ncf_draw_t& d);  // workgroups of the largest launch
+size_t distill_workspace(int64_t rows, int v);
 int64_t distill_blocks(int64_t rows, int v);  // workgroups of the largest launch
 hipError_t launch_distill(const ncf_distill_t& d, void* ws, bool forward, bool backward, hipStream_t st);
 

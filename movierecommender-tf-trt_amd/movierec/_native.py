@@ -72,7 +72,7 @@ class NcfDraw(ctypes.Structure):
                 ("mask", _vp), ("mask_ld", _i64), ("u", _vp), ("draws", _i64), ("temperature_rows", _vp),
                 ("top_k_rows", _vp), ("top_p_rows", _vp), ("min_p_rows", _vp), ("temperature", ctypes.c_double),
                 ("top_p", ctypes.c_double), ("min_p", ctypes.c_double), ("top_k", _i64), ("items", _vp),
-                ("probs", _vp)]
+                ("probs", _vp), ("ws", _vp), ("ws_bytes", ctypes.c_size_t)]
 
 
 class NcfDistill(ctypes.Structure):
@@ -155,6 +155,7 @@ _SIGNATURES = {
     "ncf_quantize_blocks": (ctypes.c_int, [_vp, _i32, _i64, _i64, _i64, _i32, _vp, _i64, _vp, _vp]),
     "ncf_matmul_blocks": (ctypes.c_int, [_vp, _i64, _vp, _vp, _i64, _vp, _i32, _vp, _i64, _i64, _i64, _i32, _vp,
                                          _i64, _vp]),
+    "ncf_draw_workspace_size": (ctypes.c_int, [_i64, _i64, _P(ctypes.c_size_t)]),
     "ncf_draw_items": (ctypes.c_int, [_P(NcfDraw), _vp]),
     "ncf_distill_workspace_size": (ctypes.c_int, [_i64, _i64, _P(ctypes.c_size_t)]),
     "ncf_distill_loss": (ctypes.c_int, [_P(NcfDistill), _vp, ctypes.c_size_t, _vp]),

@@ -72,6 +72,13 @@ def _call(fn, device, *args):
             N.check(fn(*args, N.stream_handle(idx)))
 
 
+def _workspace(size_fn, rows, cols, device):
+    """Scratch for a call over rows x cols (None where it needs none)."""
+    nbytes = ctypes.c_size_t()
+    N.check(size_fn(rows, cols, ctypes.byref(nbytes)))
+    return torch.empty(nbytes.value, dtype=torch.uint8, device=device) if nbytes.value else None
+
+
 def quantize_blocks(x, tile=False):
     """``x`` (rows, cols; float32, bfloat16 or float16) as 8-bit values with block scales: ``(q, scale)``
     with ``q`` float8_e4m3fn (rows, cols) and ``scale`` float32, one per 128 consecutive values of a
@@ -174,6 +181,9 @@ def sample_items(logits, u, temperature=1.0, top_k=0, top_p=1.0, min_p=0.0, mask
         d.logits, d.rows, d.n, d.ld = logits.data_ptr(), rows, n, ld
         d.u, d.u64 = u.data_ptr(), 1 if u.dtype == torch.float64 else 0
         d.items, d.probs = items.data_ptr(), probs.data_ptr()
+        ws = _workspace(N.lib().ncf_draw_workspace_size, rows, n, dev)
+        if ws is not None:
+            d.ws, d.ws_bytes = ws.data_ptr(), ws.numel()
         _call(N.lib().ncf_draw_items, dev, ctypes.byref(d))
     return items, probs
 
@@ -218,12 +228,6 @@ def _distill_outputs(d, logits, grad_loss):
     return grad
 
 
-def _distill_workspace(d, device):
-    nbytes = ctypes.c_size_t()
-    N.check(N.lib().ncf_distill_workspace_size(d.rows, d.v, ctypes.byref(nbytes)))
-    return torch.empty(nbytes.value, dtype=torch.uint8, device=device)
-
-
 def distill_loss(logits, teacher_items, teacher_logits, temperature=1.0, teacher_lse=None):
     """Per row, the divergence of a student's softmax over the catalogue from a teacher's list of its
     best items: ``(loss, state)``, loss float32 (rows,), state for :func:`distill_grad`.
@@ -241,10 +245,10 @@ def distill_loss(logits, teacher_items, teacher_logits, temperature=1.0, teacher
     dev = logits.device
     loss = torch.empty(d.rows, dtype=torch.float32, device=dev)
     state = torch.empty(d.rows, N.NCF_DISTILL_STATE, dtype=torch.float64, device=dev)
-    ws = _distill_workspace(d, dev)
+    ws = _workspace(N.lib().ncf_distill_workspace_size, d.rows, d.v, dev)
     d.loss, d.state = loss.data_ptr(), state.data_ptr()
     if d.rows:
-        _call(N.lib().ncf_distill_loss, dev, ctypes.byref(d), ws.data_ptr(), ws.numel())
+        _call(N.lib().ncf_distill_loss, dev, ctypes.byref(d), N.ptr(ws), ws.numel() if ws is not None else 0)
     return loss, state
 
 
@@ -268,8 +272,8 @@ def distill_loss_grad(logits, teacher_items, teacher_logits, grad_loss=1.0, temp
     loss = torch.empty(d.rows, dtype=torch.float32, device=dev)
     state = torch.empty(d.rows, N.NCF_DISTILL_STATE, dtype=torch.float64, device=dev)
     grad = _distill_outputs(d, logits, grad_loss)
-    ws = _distill_workspace(d, dev)
+    ws = _workspace(N.lib().ncf_distill_workspace_size, d.rows, d.v, dev)
     d.loss, d.state = loss.data_ptr(), state.data_ptr()
     if d.rows:
-        _call(N.lib().ncf_distill_loss_grad, dev, ctypes.byref(d), ws.data_ptr(), ws.numel())
+        _call(N.lib().ncf_distill_loss_grad, dev, ctypes.byref(d), N.ptr(ws), ws.numel() if ws is not None else 0)
     return loss, grad

@@ -116,6 +116,16 @@ def test_equal_logits_rank_by_the_lower_id(n):
         check(x, u, *call(x, u, **s), **s)
 
 
+def test_more_equal_logits_than_a_long_row_lists():
+    n = 150001
+    x = torch.zeros(3, n)
+    x[1, ::3] = 2.0
+    x[2] = torch.randint(0, 3, (n,), generator=gen(2)).float()
+    u = torch.rand(3, 5, generator=gen(3))
+    for s in (dict(), dict(k=70000), dict(k=n - 1), dict(p=0.5), dict(p=0.9, k=120000), dict(p=0.3, min_p=0.5)):
+        check(x, u, *call(x, u, **s), **s)
+
+
 @pytest.mark.parametrize("n", [5, 300, 9000, 50000])
 def test_masks_infinities_and_nan(n):
     x = logits(8, n, "float32", 5)
