@@ -58,32 +58,32 @@ __device__ __forceinline__ float unukey(uint32_t k) {
     return __uint_as_float((k & 0x80000000u) ? k & 0x7fffffffu : ~k);
 }
 
-// 2^(j / 64), filled by the compiler's exp2
-constexpr int kPowers = 64;
+// 2^(j / 256) in units of the weights
+constexpr int kPowerBits = 8, kPowers = 1 << kPowerBits;
 
-// w = exp((x - m) / t) as an integer in units of 2^-S.  With y = (x - m) log2(e) / t = j / 64 + f,
-// w = 2^(j / 64) e^(f ln 2): the powers of two from a table in LDS, the rest, |f ln 2| <= ln 2 / 128, by
-// its Taylor polynomial to the fifth power (the next term is below 2^-54).  Adding 2^52 rounds to an
-// integer.  About 14 instructions of 64 bits against about 40 of exp().
+// w = exp(z), z = (x - m) / t, as an integer in units of 2^-S.  With z = j ln 2 / 256 + r,
+// w = 2^(j / 256) e^r: the powers of two from a table in LDS (their whole part into the exponent), the
+// rest, |r| <= ln 2 / 512, by its Taylor polynomial to the fourth power (the next term is below 2^-54).
+// Adding 2^52 rounds to an integer.  13 instructions of 64 bits; exp() takes about 40.
 struct Weigher {
-    double m, c, unit;
+    double m, inv_t, unit;
     float top;
-    const double* power;   // [kPowers]
+    const double* power;   // [kPowers], times unit
 
     // w 2^S, not rounded
     __device__ __forceinline__ double real(float x) const {
         if (x == top) return unit;
-        double y = ((double)x - m) * c;
-        y = fmax(y, -200.0);   // (below every unit; also where infinities in both made a NaN)
-        const double j = rint(y * 64.0);
-        const double r = (y - j * 0x1p-6) * 0.69314718055994530942;
-        double e = fma(r, 1.0 / 120.0, 1.0 / 24.0);
-        e = fma(r, e, 1.0 / 6.0);
+        // (below -60 less than half a unit; fmax also where infinities in both made a NaN)
+        const double z = fmax(((double)x - m) * inv_t, -60.0);
+        const double j = rint(z * (kPowers * 1.4426950408889634074));
+        const double r = fma(j, -0.69314718055994530942 / kPowers, z);
+        double e = fma(r, 1.0 / 24.0, 1.0 / 6.0);
         e = fma(r, e, 0.5);
         e = fma(r, e, 1.0);
         e = fma(r, e, 1.0);
         const int n = (int)j;
-        return ldexp(power[n & (kPowers - 1)] * e, n >> 6) * unit;
+        const uint64_t p = (uint64_t)__double_as_longlong(power[n & (kPowers - 1)]);
+        return __longlong_as_double((long long)(p + ((uint64_t)(int64_t)(n >> kPowerBits) << 52))) * e;
     }
     __device__ __forceinline__ unsigned long long fixed(float x) const { return round(real(x)); }
     __device__ __forceinline__ static unsigned long long round(double w) {
@@ -91,8 +91,8 @@ struct Weigher {
     }
 };
 
-__device__ __forceinline__ void fill_powers(double* power, int threads) {
-    for (int j = threadIdx.x; j < kPowers; j += threads) power[j] = exp2(j * (1.0 / kPowers));
+__device__ __forceinline__ void fill_powers(double* power, double unit, int threads) {
+    for (int j = threadIdx.x; j < kPowers; j += threads) power[j] = exp2(j * (1.0 / kPowers)) * unit;
 }
 
 // (double)c >= p total, for a positive c: the one comparison that top-p makes
@@ -561,7 +561,7 @@ __global__ __launch_bounds__(NT) void k_draw_row(DrawArgs a) {
             for (int e = 0; e < V; ++e) x[V * j + e] = -INFINITY;
         }
     }
-    fill_powers(s.power, NT);
+    fill_powers(s.power, a.unit, NT);
 
     // the best item, and the mean of the first logits of every thread for the bins' range
     float top = -INFINITY, sum = 0.0f, num = 0.0f;
@@ -602,7 +602,7 @@ __global__ __launch_bounds__(NT) void k_draw_row(DrawArgs a) {
         }
         return;
     }
-    const Weigher wt{(double)top, 1.4426950408889634074 / set.t, a.unit, top, s.power};
+    const Weigher wt{(double)top, 1.0 / set.t, a.unit, top, s.power};
     const double min_w = set.min_p * a.unit;
     // twice the way from the best to the mean holds what top-k and top-p cut between
     const float range = 2.0f * (top - sum / num);
@@ -880,20 +880,30 @@ struct LongArgs {
 template <typename T>
 __host__ __device__ constexpr int seg_items() { return 64 * Elem<T>::kVec; }
 
-// the part's logits, a vector at a time: f(logits, first id), `part` of row `r`
+// the segments of this wave in a part
+template <typename T>
+__device__ __forceinline__ void wave_segments(const LongArgs& l, int part, int* s0, int* s1) {
+    const int wave = __builtin_amdgcn_readfirstlane((int)(threadIdx.x >> 6)), waves = (int)(blockDim.x >> 6);
+    const int n = l.part / seg_items<T>(), per = (n + waves - 1) / waves, end = min(l.segs, (part + 1) * n);
+    *s0 = min(part * n + wave * per, end);
+    *s1 = min(*s0 + per, end);
+}
+
+// the part's logits, a vector at a time: f(logits, first id); a wave takes a contiguous part of it
 template <typename T, typename F>
 __device__ __forceinline__ void each_vector(const LongArgs& l, int64_t r, int part, F f) {
     constexpr int V = Elem<T>::kVec, U = 4;
-    const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, step = (int)(blockDim.x >> 6);
-    const int s0 = part * (l.part / seg_items<T>()), s1 = min(l.segs, s0 + l.part / seg_items<T>());
-    for (int sg = s0 + wave; sg < s1; sg += U * step) {
+    const int lane = threadIdx.x & 63;
+    int s0, s1;
+    wave_segments<T>(l, part, &s0, &s1);
+    for (int sg = s0; sg < s1; sg += U) {
         float y[U][V];
 #pragma unroll
-        for (int u = 0; u < U; ++u)   // (segments past the part: past the row's end, or not used)
-            load_logits<T>(l.a, r, sg + u * step < s1 ? (sg + u * step) * seg_items<T>() + lane * V : l.a.n, y[u]);
+        for (int u = 0; u < U; ++u)   // (past the part: as past the row's end)
+            load_logits<T>(l.a, r, sg + u < s1 ? (sg + u) * seg_items<T>() + lane * V : l.a.n, y[u]);
 #pragma unroll
         for (int u = 0; u < U; ++u)
-            if (sg + u * step < s1) f(y[u], (sg + u * step) * seg_items<T>() + lane * V);
+            if (sg + u < s1) f(y[u], (sg + u) * seg_items<T>() + lane * V);
     }
 }
 
@@ -979,7 +989,7 @@ __device__ __forceinline__ Bins long_bins(const LongArgs& l, int64_t r) {
 }
 __device__ __forceinline__ Weigher long_weigher(const LongArgs& l, const Bins& bins, const RowSettings& set,
                                                 const double* power) {
-    return Weigher{(double)bins.top, 1.4426950408889634074 / set.t, l.a.unit, bins.top, power};
+    return Weigher{(double)bins.top, 1.0 / set.t, l.a.unit, bins.top, power};
 }
 __device__ __forceinline__ Cut row_cut(const LongRow& w) { return Cut{w.bound, w.ties, w.partial != 0, w.equal}; }
 __device__ __forceinline__ bool wants_cut(const LongArgs& l, const RowSettings& set, bool weights) {
@@ -999,7 +1009,7 @@ __global__ __launch_bounds__(kLongThreads) void k_long_histogram(LongArgs l) {
         if constexpr (WEIGHTS) s.weight[b] = 0;
         else s.count[b] = 0;
     }
-    fill_powers(s.power, kLongThreads);
+    fill_powers(s.power, l.a.unit, kLongThreads);
     __syncthreads();
     const Weigher wt = long_weigher(l, bins, set, s.power);
     const float bound = l.row[r].bound;
@@ -1050,7 +1060,7 @@ __global__ __launch_bounds__(kLongThreads) void k_long_gather(LongArgs l) {
     if (!wants_cut(l, set, WEIGHTS)) return;
     const Bins bins = long_bins(l, r);
     if (!(bins.top > -INFINITY)) return;
-    fill_powers(s.power, kLongThreads);
+    fill_powers(s.power, l.a.unit, kLongThreads);
     if (tid == 0) s.pick_bin = -1;
     __syncthreads();
     const Cut was = row_cut(l.row[r]);
@@ -1093,19 +1103,28 @@ __global__ __launch_bounds__(kLongThreads) void k_long_gather(LongArgs l) {
         l.row[r].total_w = total;
     }
     if (bin < 0) return;
+    // counted, a place in the row's list reserved for all of them at once, then stored (with an atomic for
+    // each wave's items this kernel took 57 us, so 20: they all meet at one address; 16 rows of 1,000,000)
+        uint32_t items = 0;
+    each_vector<T>(l, r, part, [&](const float* y, int) {
+#pragma unroll
+        for (int e = 0; e < Elem<T>::kVec; ++e) items += y[e] >= was.bound && bins.of(y[e]) == bin;
+    });
+    unsigned long long part_items;
+    const uint32_t ahead_items = (uint32_t)long_before(items, s, &part_items);
+    if (part_items == 0) return;
+    __syncthreads();
+    if (tid == 0) s.wave32[0] = atomicAdd(&l.row[r].members, (uint32_t)part_items);
+    __syncthreads();
+    uint32_t at = s.wave32[0] + ahead_items;
+    if (items == 0) return;
     each_vector<T>(l, r, part, [&](const float* y, int id) {
 #pragma unroll
-        for (int e = 0; e < Elem<T>::kVec; ++e) {
-            const bool in = y[e] >= was.bound && bins.of(y[e]) == bin;
-            const uint64_t m = __ballot(in);
-            if (m == 0) continue;
-            // one reservation a wave
-            uint32_t base = 0;
-            if ((tid & 63) == __builtin_ctzll(m)) base = atomicAdd(&l.row[r].members, (uint32_t)lane_count(m));
-            base = (uint32_t)__builtin_amdgcn_readlane((int)base, __builtin_ctzll(m));
-            const uint32_t at = lanes_before(m, base);
-            if (in && at < l.cap) l.list[r * l.cap + at] = make_uint2(__float_as_uint(y[e]), (uint32_t)(id + e));
-        }
+        for (int e = 0; e < Elem<T>::kVec; ++e)
+            if (y[e] >= was.bound && bins.of(y[e]) == bin) {
+                if (at < l.cap) l.list[r * l.cap + at] = make_uint2(__float_as_uint(y[e]), (uint32_t)(id + e));
+                ++at;
+            }
     });
 }
 
@@ -1120,7 +1139,7 @@ __global__ __launch_bounds__(kResolveThreads) void k_long_resolve(LongArgs l) {
     const LongRow w = l.row[r];
     const Bins bins = long_bins(l, r);
     if (!(bins.top > -INFINITY) || w.bin < 0) return;
-    fill_powers(s.power, kResolveThreads);
+    fill_powers(s.power, l.a.unit, kResolveThreads);
     __syncthreads();
     const Cut was = row_cut(w);
     const Weigher wt = long_weigher(l, bins, set, s.power);
@@ -1197,11 +1216,12 @@ __global__ __launch_bounds__(kLongThreads) void k_long_ties(LongArgs l) {
     });
 }
 
-// equals of the bound ahead of a segment; each lane a share of the segments before it
-__device__ __forceinline__ uint32_t ties_ahead(const LongArgs& l, int64_t r, int from, int to) {
-    uint32_t n = 0;
-    for (int g = from + (int)(threadIdx.x & 63); g < to; g += 64) n += l.seg_ties[r * l.segs + g];
-    return lane63(lane_sums32(n));
+// equals of the bound in the segments before `to`, for threads i, i + n, .. of those who ask
+__device__ __forceinline__ uint32_t ties_ahead(const LongArgs& l, int64_t r, int to, int i, int n) {
+    uint32_t sum = 0;
+#pragma unroll 8
+    for (int g = i; g < to; g += n) sum += l.seg_ties[r * l.segs + g];
+    return lane63(lane_sums32(sum));   // of this wave
 }
 
 // The weight of every segment.
@@ -1214,22 +1234,27 @@ __global__ __launch_bounds__(kLongThreads) void k_long_weigh(LongArgs l) {
     const RowSettings set = row_settings(l.a, r);
     const Bins bins = long_bins(l, r);
     if (!(bins.top > -INFINITY)) return;
-    fill_powers(power, kLongThreads);
+    fill_powers(power, l.a.unit, kLongThreads);
     __syncthreads();
     const Weigher wt = long_weigher(l, bins, set, power);
     const double min_w = set.min_p * l.a.unit;
     const Cut cut = row_cut(l.row[r]);
-    int done = 0;             // segments whose equals are counted in `ahead`
-    uint32_t ahead = 0;
+    uint32_t ahead = 0;   // equals of the bound before this wave's next segment
+    if (cut.partial) {
+        int s0, s1;
+        wave_segments<T>(l, part, &s0, &s1);
+        ahead = ties_ahead(l, r, s0, lane, 64);
+    }
     each_vector<T>(l, r, part, [&](const float* y, int id) {
         const int g = id / seg_items<T>();
-        uint32_t seen = 0;
+        uint32_t seen = ahead;
         if (cut.partial) {
-            ahead += ties_ahead(l, r, done, g);
-            done = g;
-            seen = ahead;
 #pragma unroll
-            for (int e = 0; e < V; ++e) seen = lanes_before(__ballot(y[e] == cut.bound), seen);
+            for (int e = 0; e < V; ++e) {
+                const uint64_t m = __ballot(y[e] == cut.bound);
+                seen = lanes_before(m, seen);
+                ahead += (uint32_t)lane_count(m);
+            }
         }
         unsigned long long w[V];
         const unsigned long long sum = lane_sums64(weigh_vector<V>(y, seen, cut, wt, min_w, w));
@@ -1253,7 +1278,7 @@ __global__ __launch_bounds__(kLongThreads) void k_long_draw(LongArgs l) {
         }
         return;
     }
-    fill_powers(s.power, kLongThreads);
+    fill_powers(s.power, l.a.unit, kLongThreads);
     // a thread's share of the segments
     const int per = (l.segs + kLongThreads - 1) / kLongThreads;
     const int g0 = min(tid * per, l.segs), g1 = min(g0 + per, l.segs);
@@ -1273,15 +1298,21 @@ __global__ __launch_bounds__(kLongThreads) void k_long_draw(LongArgs l) {
         }
     }
     __syncthreads();
-    if (tid >= 64) return;
     const int g = s.pick_bin, at = g * seg_items<T>() + lane * V;
     const Weigher wt = long_weigher(l, bins, set, s.power);
     const Cut cut = row_cut(l.row[r]);
+    if (cut.partial) {
+        const uint32_t n = ties_ahead(l, r, g, tid, kLongThreads);
+        if (lane == 0) s.wave32[tid >> 6] = n;
+        __syncthreads();
+    }
+    if (tid >= 64) return;
     float y[V];
     load_logits<T>(l.a, r, at, y);
     uint32_t seen = 0;
     if (cut.partial) {
-        seen = ties_ahead(l, r, 0, g);
+#pragma unroll
+        for (int w = 0; w < kLongWaves; ++w) seen += s.wave32[w];
 #pragma unroll
         for (int e = 0; e < V; ++e) seen = lanes_before(__ballot(y[e] == cut.bound), seen);
     }
