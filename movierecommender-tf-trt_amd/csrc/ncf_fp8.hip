@@ -173,19 +173,8 @@ __device__ __forceinline__ mf16x8 widen(mi32x8 f, int e) {
     return r;
 }
 
-// One block of 128: both operands hold lane l's row l & 15 and its 32 values from 32 (l >> 4) on (which
-// of them share an instruction is the same in both, so the order of k does not matter).
-template <bool WIDE>
-__device__ __forceinline__ vf32x4 mfma_block(mi32x8 a, mi32x8 b) {
-    vf32x4 d = {0.0f, 0.0f, 0.0f, 0.0f};
-    if constexpr (WIDE) {
-#pragma unroll
-        for (int e = 0; e < 4; ++e) d = __builtin_amdgcn_mfma_f32_16x16x32_f16(widen(a, e), widen(b, e), d, 0, 0, 0);
-    } else {
-        d = __builtin_amdgcn_mfma_scale_f32_16x16x128_f8f6f4(a, b, d, 0, 0, 0, 0, 0, 0);
-    }
-    return d;
-}
+// One block of 128: both operands hold lane l's row l & 15 and 32 of its values, the same columns in both
+// for the same l >> 4 (which of them share an instruction does not matter: a sum over k has no order).
 
 // 16 values from column c on of a row of k values, zero past its end
 __device__ __forceinline__ vu32x4 load_q16(const uint8_t* row, int c, int k) {
@@ -199,6 +188,33 @@ __device__ __forceinline__ mi32x8 load_frag(const uint8_t* row, int c, int k) {
     const vu32x4 lo = load_q16(row, c, k), hi = load_q16(row, c + 16, k);
     return mi32x8{(int)lo[0], (int)lo[1], (int)lo[2], (int)lo[3], (int)hi[0], (int)hi[1], (int)hi[2], (int)hi[3]};
 }
+
+// a fragment as the MFMA takes it: widened once, for all the products it enters
+template <bool WIDE>
+struct Operand;
+template <>
+struct Operand<false> {
+    mi32x8 v;
+    __device__ __forceinline__ void set(mi32x8 f) { v = f; }
+    __device__ __forceinline__ static vf32x4 product(const Operand& a, const Operand& b) {
+        const vf32x4 zero = {0.0f, 0.0f, 0.0f, 0.0f};
+        return __builtin_amdgcn_mfma_scale_f32_16x16x128_f8f6f4(a.v, b.v, zero, 0, 0, 0, 0, 0, 0);
+    }
+};
+template <>
+struct Operand<true> {
+    mf16x8 v[4];
+    __device__ __forceinline__ void set(mi32x8 f) {
+#pragma unroll
+        for (int e = 0; e < 4; ++e) v[e] = widen(f, e);
+    }
+    __device__ __forceinline__ static vf32x4 product(const Operand& a, const Operand& b) {
+        vf32x4 d = {0.0f, 0.0f, 0.0f, 0.0f};
+#pragma unroll
+        for (int e = 0; e < 4; ++e) d = __builtin_amdgcn_mfma_f32_16x16x32_f16(a.v[e], b.v[e], d, 0, 0, 0);
+        return d;
+    }
+};
 
 struct MmArgs {
     const uint8_t* a;
@@ -233,6 +249,7 @@ __device__ __forceinline__ void store_y4(TO* p, vf32x4 v, int valid) {
 // rows of b are the MFMA's A operand, so a lane ends with four neighbouring columns of one row of y.
 template <int MI, int NI, typename TO>
 __global__ __launch_bounds__(kBlock) void k_mm_direct(MmArgs p) {
+    constexpr bool WIDE = std::is_same<TO, float>::value;
     const int lane = threadIdx.x & 63, g = lane >> 4, i = lane & 15;
     const int64_t wave = (int64_t)blockIdx.x * (kBlock / 64) + (threadIdx.x >> 6);
     if (wave >= p.mt * p.nt) return;
@@ -251,11 +268,11 @@ __global__ __launch_bounds__(kBlock) void k_mm_direct(MmArgs p) {
     for (int j = 0; j < NI; ++j) br[j] = p.b + min(n0 + 16 * j + i, p.n - 1) * p.ldb;
     for (int kb = 0; kb < p.kb; ++kb) {
         const int c = kb * kScaleBlock + 32 * g;
-        mi32x8 fb[NI];
+        Operand<WIDE> fb[NI];
         vf32x4 sb[NI];
 #pragma unroll
         for (int j = 0; j < NI; ++j) {
-            fb[j] = load_frag(br[j], c, p.k);
+            fb[j].set(load_frag(br[j], c, p.k));
 #pragma unroll
             for (int r = 0; r < 4; ++r) {
                 const int64_t n = min(n0 + 16 * j + 4 * g + r, p.n - 1);
@@ -264,11 +281,12 @@ __global__ __launch_bounds__(kBlock) void k_mm_direct(MmArgs p) {
         }
 #pragma unroll
         for (int x = 0; x < MI; ++x) {
-            const mi32x8 fa = load_frag(ar[x], c, p.k);
+            Operand<WIDE> fa;
+            fa.set(load_frag(ar[x], c, p.k));
             const float sa = p.sa[min(m0 + 16 * x + i, p.m - 1) * p.kb + kb];
 #pragma unroll
             for (int j = 0; j < NI; ++j) {
-                const vf32x4 d = mfma_block<std::is_same<TO, float>::value>(fb[j], fa);
+                const vf32x4 d = Operand<WIDE>::product(fb[j], fa);
 #pragma unroll
                 for (int r = 0; r < 4; ++r) acc[x][j][r] = fmaf(sa * sb[j][r], d[r], acc[x][j][r]);
             }
@@ -292,17 +310,184 @@ __global__ __launch_bounds__(kBlock) void k_mm_direct(MmArgs p) {
     }
 }
 
-template <typename TO>
-static hipError_t mm_t(MmArgs p, hipStream_t st) {
-    if (p.m <= 16) {
-        p.mt = 1;
-        p.nt = (p.n + 15) / 16;
-        launch(k_mm_direct<1, 1, TO>, dim3((unsigned)((p.nt + 3) / 4)), kBlock, 0, st, p);
-    } else {
-        p.mt = (p.m + 63) / 64;
-        p.nt = (p.n + 63) / 64;
-        launch(k_mm_direct<4, 4, TO>, dim3((unsigned)((p.mt * p.nt + 3) / 4)), kBlock, 0, st, p);
+// ----------------------------------------------------------------------------- large products
+//
+// 256 x 256 of y a workgroup of eight waves (64 rows by 128 columns each), 128 of k a step.  Both
+// operands' steps go straight from memory to LDS (16 bytes a lane), the next while this one is multiplied.
+// In LDS the 16-byte pieces of a row are permuted by the row (piece c at c ^ (row / 2 % 8)), so the 16
+// lanes that read a fragment touch all 64 banks; a lane's fragment is pieces g and g + 4 of its row, in
+// both operands alike.
+
+constexpr int kTile = 256, kTileThreads = 512, kTileWaves = kTileThreads / 64;
+constexpr int kTileMI = 4, kTileNI = 8;   // 16-row, 16-column tiles of a wave
+
+struct TileStage {
+    uint8_t a[kTile * kScaleBlock];
+    uint8_t b[kTile * kScaleBlock];
+    float sa[kTile];
+    float sb[kTile];
+};
+
+// Rows [r0, r0 + 256) of an operand, step j, into LDS; rows past the end repeat the last one.  A thread
+// stages piece tid % 8 of rows tid / 8 + 64 i, in LDS order.
+__device__ __forceinline__ void stage_rows(const uint8_t* q, int64_t ld, int64_t rows, int64_t r0, int j,
+                                           uint8_t* lds) {
+    const int wave = __builtin_amdgcn_readfirstlane((int)(threadIdx.x >> 6));
+    const uint32_t t = threadIdx.x >> 3, c = 16 * ((threadIdx.x & 7) ^ (t >> 1 & 7));
+#pragma unroll
+    for (int i = 0; i < kTile / 64; ++i) {
+        const int64_t rb = min(r0 + 64 * i, rows - 1);               // (uniform: a scalar base, 32-bit offsets)
+        const uint32_t off = min(t, (uint32_t)min(rows - 1 - rb, (int64_t)63)) * (uint32_t)ld + c;
+        const uint8_t* src = q + rb * ld + (int64_t)j * kScaleBlock;
+        uint8_t* dst = lds + 1024 * (8 * i + wave);                  // the wave's; a lane's 16 bytes follow
+        __builtin_amdgcn_global_load_lds((const __attribute__((address_space(1))) void*)(src + off),
+                                         (__attribute__((address_space(3))) void*)dst, 16, 0, 0);
     }
+}
+// the same for a last step that ends inside the block: zeros past column k
+__device__ __forceinline__ void stage_tail(const uint8_t* q, int64_t ld, int64_t rows, int64_t r0, int j, int k,
+                                           uint8_t* lds) {
+    const int t = threadIdx.x >> 3, c = j * kScaleBlock + 16 * ((threadIdx.x & 7) ^ (t >> 1 & 7));
+#pragma unroll 1
+    for (int i = 0; i < kTile / 64; ++i)
+        *reinterpret_cast<vu32x4*>(lds + 16 * (512 * i + (int)threadIdx.x)) =
+            load_q16(q + min(r0 + 64 * i + t, rows - 1) * ld, c, k);
+}
+
+// a fragment from its lane's two pieces, `rows` rows below the first
+__device__ __forceinline__ mi32x8 tile_frag(const uint8_t* lo_piece, const uint8_t* hi_piece, int rows) {
+    const vu32x4 lo = *reinterpret_cast<const vu32x4*>(lo_piece + rows * kScaleBlock);
+    const vu32x4 hi = *reinterpret_cast<const vu32x4*>(hi_piece + rows * kScaleBlock);
+    return mi32x8{(int)lo[0], (int)lo[1], (int)lo[2], (int)lo[3], (int)hi[0], (int)hi[1], (int)hi[2], (int)hi[3]};
+}
+
+template <typename TO, bool B_TILE>
+__global__ __launch_bounds__(kTileThreads, 2) void k_mm_tile(MmArgs p) {
+    constexpr bool WIDE = std::is_same<TO, float>::value;
+    extern __shared__ __attribute__((aligned(16))) uint8_t tile_lds[];
+    TileStage* st = reinterpret_cast<TileStage*>(tile_lds);   // [2]
+    const int tid = threadIdx.x, lane = tid & 63, g = lane >> 4, i = lane & 15;
+    const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
+    // neighbouring tiles to one XCD (workgroups go round the eight); within it bands of four tile rows,
+    // column by column
+    const uint32_t mt = (uint32_t)p.mt, nt = (uint32_t)p.nt, total = mt * nt, per = (total + 7) / 8;
+    const uint32_t tile = (blockIdx.x & 7) * per + (blockIdx.x >> 3);
+    if (tile >= total) return;
+    const uint32_t band = tile / (4 * nt), in_band = tile - band * 4 * nt, rows_in = min(4u, mt - 4 * band);
+    const uint32_t col = in_band / rows_in, row = 4 * band + in_band - col * rows_in;
+    const int64_t m0 = (int64_t)__builtin_amdgcn_readfirstlane((int)row) * kTile;
+    const int64_t n0 = (int64_t)__builtin_amdgcn_readfirstlane((int)col) * kTile;
+    const int wm = (wave & 3) * 16 * kTileMI, wn = (wave >> 2) * 16 * kTileNI;
+    const int full = p.k / kScaleBlock;   // whole blocks
+    // a lane's pieces g and g + 4 of row i of its wave (16 rows further the permutation is the same)
+    const int piece = 16 * (g ^ (i >> 1)), at_a = (wm + i) * kScaleBlock, at_b = (wn + i) * kScaleBlock;
+
+    vf32x4 acc[kTileMI][kTileNI];
+#pragma unroll
+    for (int x = 0; x < kTileMI; ++x)
+#pragma unroll
+        for (int j = 0; j < kTileNI; ++j) acc[x][j] = vf32x4{0.0f, 0.0f, 0.0f, 0.0f};
+    // a thread's scale of a step: rows of a, then rows (or tiles) of b
+    const bool of_b = tid >= kTile;
+    const int64_t srow = of_b ? min(n0 + tid - kTile, p.n - 1) : min(m0 + tid, p.m - 1);
+    const float* sp = of_b ? p.sb + (B_TILE ? srow / kScaleBlock : srow) * p.kb : p.sa + srow * p.kb;
+    // a block that k ends inside comes first, so every step of the loop stages a whole one
+    const int tail = p.kb - full;
+    if (tail) {
+        stage_tail(p.a, p.lda, p.m, m0, full, p.k, st[0].a);
+        stage_tail(p.b, p.ldb, p.n, n0, full, p.k, st[0].b);
+    } else {
+        stage_rows(p.a, p.lda, p.m, m0, 0, st[0].a);
+        stage_rows(p.b, p.ldb, p.n, n0, 0, st[0].b);
+    }
+    (of_b ? st[0].sb : st[0].sa)[tid & (kTile - 1)] = sp[tail ? full : 0];
+    __syncthreads();
+    for (int step = 0; step < p.kb; ++step) {
+        const TileStage& s = st[step & 1];
+        TileStage& next = st[step & 1 ^ 1];
+        const int kb = step + 1 - tail;   // the next block
+        const float scale = sp[min(kb, p.kb - 1)];
+        if (step + 1 < p.kb) {
+            stage_rows(p.a, p.lda, p.m, m0, kb, next.a);
+            stage_rows(p.b, p.ldb, p.n, n0, kb, next.b);
+        }
+        Operand<WIDE> fa[kTileMI];
+        float sa[kTileMI];
+#pragma unroll
+        for (int x = 0; x < kTileMI; ++x) {
+            fa[x].set(tile_frag(s.a + at_a + piece, s.a + at_a + (piece ^ 64), 16 * x));
+            sa[x] = s.sa[wm + 16 * x + i];
+            if constexpr (B_TILE) sa[x] *= s.sb[wn];   // (the wave's 128 columns are one tile of b)
+        }
+#pragma unroll
+        for (int j = 0; j < kTileNI; ++j) {
+            Operand<WIDE> fb;
+            fb.set(tile_frag(s.b + at_b + piece, s.b + at_b + (piece ^ 64), 16 * j));
+            vf32x4 sb;
+            if constexpr (!B_TILE) sb = *reinterpret_cast<const vf32x4*>(&s.sb[wn + 16 * j + 4 * g]);
+#pragma unroll
+            for (int x = 0; x < kTileMI; ++x) {
+                const vf32x4 d = Operand<WIDE>::product(fb, fa[x]);
+#pragma unroll
+                for (int r = 0; r < 4; ++r)
+                    acc[x][j][r] = fmaf(B_TILE ? sa[x] : sa[x] * sb[r], d[r], acc[x][j][r]);
+            }
+            __builtin_amdgcn_sched_barrier(0);
+        }
+        // (also after the last step, where nobody reads it: a branch here would draw the sums behind it and
+        // hold all 32 products in registers)
+        (of_b ? next.sb : next.sa)[tid & (kTile - 1)] = scale;
+        __syncthreads();
+    }
+#pragma unroll
+    for (int j = 0; j < kTileNI; ++j) {
+        const int64_t n = n0 + wn + 16 * j + 4 * g;
+        const int valid = (int)min((int64_t)4, p.n - n);
+        if (valid <= 0) continue;
+        vf32x4 bias = {0.0f, 0.0f, 0.0f, 0.0f};
+        if (p.bias)
+#pragma unroll
+            for (int r = 0; r < 4; ++r)
+                if (r < valid) bias[r] = p.bias[n + r];
+#pragma unroll
+        for (int x = 0; x < kTileMI; ++x) {
+            const int64_t m = m0 + wm + 16 * x + i;
+            if (m < p.m) store_y4(static_cast<TO*>(p.y) + m * p.ldy + n, acc[x][j] + bias, valid);
+        }
+    }
+}
+
+template <int MI, int NI, typename TO>
+static void mm_direct(MmArgs p, hipStream_t st) {
+    p.mt = (p.m + 16 * MI - 1) / (16 * MI);
+    p.nt = (p.n + 16 * NI - 1) / (16 * NI);
+    launch(k_mm_direct<MI, NI, TO>, dim3((unsigned)((p.mt * p.nt + 3) / 4)), kBlock, 0, st, p);
+}
+
+template <typename TO, bool B_TILE>
+static hipError_t mm_tile(MmArgs p, hipStream_t st) {
+    constexpr size_t lds = 2 * sizeof(TileStage);
+    static const hipError_t attr = hipFuncSetAttribute(reinterpret_cast<const void*>(k_mm_tile<TO, B_TILE>),
+                                                       hipFuncAttributeMaxDynamicSharedMemorySize, (int)lds);
+    if (attr != hipSuccess) return attr;
+    p.mt = (p.m + kTile - 1) / kTile;
+    p.nt = (p.n + kTile - 1) / kTile;
+    const int64_t per = (p.mt * p.nt + 7) / 8;
+    launch(k_mm_tile<TO, B_TILE>, dim3((unsigned)(8 * per)), kTileThreads, lds, st, p);
+    return hipGetLastError();
+}
+
+template <typename TO>
+static hipError_t mm_t(const MmArgs& p, hipStream_t st) {
+    const bool aligned = ((uintptr_t)p.a | (uintptr_t)p.b | (uint64_t)p.lda | (uint64_t)p.ldb) % 16 == 0;
+    // (rows up to 16 MB apart: a thread's offsets in 32 bits)
+    const bool near = p.lda <= 1 << 24 && p.ldb <= 1 << 24;
+    if (aligned && near && p.k > kScaleBlock && ((p.m + kTile - 1) / kTile) * ((p.n + kTile - 1) / kTile) >= 128)
+        return p.b_tile ? mm_tile<TO, true>(p, st) : mm_tile<TO, false>(p, st);
+    const int64_t waves = ((p.m + 63) / 64) * ((p.n + 63) / 64);   // of 64 x 64
+    if (p.m <= 16) mm_direct<1, 1, TO>(p, st);
+    else if (waves >= 1024) mm_direct<4, 4, TO>(p, st);
+    else mm_direct<2, 2, TO>(p, st);
     return hipGetLastError();
 }
 

@@ -129,6 +129,26 @@ def test_product_half_outputs(shape, dtype):
     check_product(*operands(*shape, True, seed=6), dtype, True)
 
 
+LARGE = [(2819, 2999, 259), (33000, 130, 384), (200, 33000, 144), (3000, 2900, 129)]
+
+
+@pytest.mark.parametrize("tile", [False, True])
+@pytest.mark.parametrize("shape", LARGE, ids=str)
+def test_large_products(shape, tile):
+    ops = operands(*shape, tile, seed=9)
+    check_product(*ops, F, tile)
+    check_product(*ops, BF, tile)
+    check_product(*ops, HF, tile)
+
+
+@pytest.mark.parametrize("shape", [(5000, 3000, 64), (4100, 4099, 128), (3000, 5000, 100), (20000, 700, 8),
+                                   (17, 70000, 31)], ids=str)
+def test_many_outputs_of_short_rows(shape):
+    for tile in (False, True):
+        check_product(*operands(*shape, tile, seed=10), F, tile)
+    check_product(*operands(*shape, False, seed=11, bias=False), BF, False)
+
+
 @pytest.mark.parametrize("at", [0, 1, 4, 13])
 @pytest.mark.parametrize("shape", [(1, 65, 70), (3, 65, 300), (130, 257, 300), (260, 300, 1024)], ids=str)
 def test_product_any_alignment_and_row_distance(shape, at):
