@@ -16,6 +16,7 @@
 //
 // The reference scores one user against a list of items (movierec/trt_client.py:43-57).
 
+#include <algorithm>
 #include <cmath>
 #include <type_traits>
 
@@ -457,6 +458,167 @@ __global__ __launch_bounds__(kTileThreads, 2) void k_mm_tile(MmArgs p) {
     }
 }
 
+// ----------------------------------------------------------------------------- rows of one block
+//
+// k <= 128, as the factors of the models here: the output's write is the work.  A wave keeps 64 rows of a in
+// registers and goes along the columns, 64 at a time, the next columns' operand loaded meanwhile; their
+// products pass through LDS, so that a store instruction writes 256 bytes of each of four rows of y (from
+// the MFMA's layout it would be 64 bytes of sixteen).
+
+constexpr int kShortRows = 64, kShortCols = 64;
+constexpr int kShortWaves = kBlock / 64;
+
+// 8 values from column c on, zero past column k
+__device__ __forceinline__ uint2 load_q8(const uint8_t* row, int c, int k) {
+    typedef uint32_t u __attribute__((ext_vector_type(2), aligned(1)));
+    if (c + 8 <= k) {
+        const u v = *reinterpret_cast<const u*>(row + c);
+        return make_uint2(v[0], v[1]);
+    }
+    uint32_t w[2] = {0, 0};
+    for (int e = 0; c + e < k; ++e) w[e >> 2] |= (uint32_t)row[c + e] << (8 * (e & 3));
+    return make_uint2(w[0], w[1]);
+}
+
+// A lane's part of a row, as the MFMA takes it.  fp32 outputs: E instructions of 32 columns, 8 a lane;
+// 16-bit outputs: one of 128, 32 a lane.
+template <bool WIDE, int E>
+struct ShortRaw;
+template <int E>
+struct ShortRaw<true, E> {
+    uint2 v[E];
+    __device__ __forceinline__ void load(const uint8_t* row, int g, int k) {
+#pragma unroll
+        for (int e = 0; e < E; ++e) v[e] = load_q8(row, 32 * e + 8 * g, k);
+    }
+};
+template <int E>
+struct ShortRaw<false, E> {
+    mi32x8 v;
+    __device__ __forceinline__ void load(const uint8_t* row, int g, int k) { v = load_frag(row, 32 * g, k); }
+};
+template <bool WIDE, int E>
+struct ShortOperand;
+template <int E>
+struct ShortOperand<true, E> {
+    mf16x8 v[E];
+    __device__ __forceinline__ void set(const ShortRaw<true, E>& r) {
+#pragma unroll
+        for (int e = 0; e < E; ++e) {
+            const mi32x8 f = {(int)r.v[e].x, (int)r.v[e].y, 0, 0, 0, 0, 0, 0};
+            v[e] = widen(f, 0);
+        }
+    }
+    __device__ __forceinline__ static vf32x4 product(const ShortOperand& a, const ShortOperand& b) {
+        vf32x4 d = {0.0f, 0.0f, 0.0f, 0.0f};
+#pragma unroll
+        for (int e = 0; e < E; ++e) d = __builtin_amdgcn_mfma_f32_16x16x32_f16(a.v[e], b.v[e], d, 0, 0, 0);
+        return d;
+    }
+};
+template <int E>
+struct ShortOperand<false, E> {
+    mi32x8 v;
+    __device__ __forceinline__ void set(const ShortRaw<false, E>& r) { v = r.v; }
+    __device__ __forceinline__ static vf32x4 product(const ShortOperand& a, const ShortOperand& b) {
+        const vf32x4 zero = {0.0f, 0.0f, 0.0f, 0.0f};
+        return __builtin_amdgcn_mfma_scale_f32_16x16x128_f8f6f4(a.v, b.v, zero, 0, 0, 0, 0, 0, 0);
+    }
+};
+
+__device__ __forceinline__ vf32x4 load_f4(const float* p, int valid) {
+    vf32x4 r = {0.0f, 0.0f, 0.0f, 0.0f};
+    if (valid >= 4) {
+        typedef float f4 __attribute__((ext_vector_type(4), aligned(4)));
+        return *reinterpret_cast<const f4*>(p);
+    }
+#pragma unroll
+    for (int e = 0; e < 3; ++e)
+        if (e < valid) r[e] = p[e];
+    return r;
+}
+
+template <int E, typename TO>
+__global__ __launch_bounds__(kBlock) void k_mm_short(MmArgs p, int64_t cols) {
+    constexpr bool WIDE = std::is_same<TO, float>::value;
+    constexpr int kPad = 4;   // (a row's 16-byte pieces one bank group further than the row above's)
+    __shared__ __attribute__((aligned(16))) float out[kShortWaves][kShortRows][kShortCols + kPad];
+    const int lane = threadIdx.x & 63, g = lane >> 4, i = lane & 15;
+    const int wave = __builtin_amdgcn_readfirstlane((int)(threadIdx.x >> 6));
+    const int64_t m0 = blockIdx.x % p.mt * kShortRows;
+    // this wave's column blocks: every kShortWaves-th of the workgroup's
+    const int64_t c0 = blockIdx.x / p.mt * cols, c1 = min(c0 + cols, p.n);
+    ShortOperand<WIDE, E> fa[kShortRows / 16];
+    float sa[kShortRows / 16];
+#pragma unroll
+    for (int x = 0; x < kShortRows / 16; ++x) {
+        const int64_t m = min(m0 + 16 * x + i, p.m - 1);
+        ShortRaw<WIDE, E> raw;
+        raw.load(p.a + m * p.lda, g, p.k);
+        fa[x].set(raw);
+        sa[x] = p.sa[m];
+    }
+    constexpr int NJ = kShortCols / 16;
+    ShortRaw<WIDE, E> raw[NJ];
+    int64_t n0 = c0 + wave * kShortCols;
+    if (n0 >= c1) return;
+    auto load_b = [&](int64_t n) {
+#pragma unroll
+        for (int j = 0; j < NJ; ++j) raw[j].load(p.b + min(n + 16 * j + i, p.n - 1) * p.ldb, g, p.k);
+    };
+    load_b(n0);
+    for (; n0 < c1; n0 += kShortWaves * kShortCols) {
+        ShortOperand<WIDE, E> fb[NJ];
+        vf32x4 sb[NJ], bias[NJ];
+#pragma unroll
+        for (int j = 0; j < NJ; ++j) {
+            fb[j].set(raw[j]);
+            const int64_t n = n0 + 16 * j + 4 * g;
+            const int valid = (int)min((int64_t)4, p.n - n);
+            if (p.b_tile) {   // (16 columns from a multiple of 16 on share a tile)
+                const float t = p.sb[min(n, p.n - 1) / kScaleBlock];
+                sb[j] = vf32x4{t, t, t, t};
+            } else {
+                sb[j] = load_f4(p.sb + n, valid);
+            }
+            bias[j] = p.bias ? load_f4(p.bias + n, valid) : vf32x4{0.0f, 0.0f, 0.0f, 0.0f};
+        }
+        if (n0 + kShortWaves * kShortCols < c1) load_b(n0 + kShortWaves * kShortCols);
+#pragma unroll
+        for (int j = 0; j < NJ; ++j) {
+#pragma unroll
+            for (int x = 0; x < kShortRows / 16; ++x) {
+                const vf32x4 d = ShortOperand<WIDE, E>::product(fb[j], fa[x]);
+                vf32x4 y;
+#pragma unroll
+                for (int r = 0; r < 4; ++r) y[r] = fmaf(sa[x] * sb[j][r], d[r], bias[j][r]);
+                *reinterpret_cast<vf32x4*>(&out[wave][16 * x + i][16 * j + 4 * g]) = y;
+            }
+        }
+        asm volatile("" ::: "memory");   // (the wave's own LDS, written and read in order)
+        const int64_t n = n0 + 4 * i;
+        const int valid = (int)min((int64_t)4, p.n - n);
+#pragma unroll
+        for (int q = 0; q < kShortRows / 4; ++q) {
+            const vf32x4 y = *reinterpret_cast<const vf32x4*>(&out[wave][4 * q + g][4 * i]);
+            const int64_t m = m0 + 4 * q + g;
+            if (m < p.m && valid > 0) store_y4(static_cast<TO*>(p.y) + m * p.ldy + n, y, valid);
+        }
+        asm volatile("" ::: "memory");
+    }
+}
+
+template <int E, typename TO>
+static void mm_short(MmArgs p, hipStream_t st) {
+    p.mt = (p.m + kShortRows - 1) / kShortRows;
+    // columns of a workgroup: whole turns of its waves, about 2048 workgroups together
+    const int64_t turn = kShortWaves * kShortCols, turns = (p.n + turn - 1) / turn;
+    const int64_t split = std::max<int64_t>(1, std::min<int64_t>(turns, 2048 / p.mt));
+    const int64_t cols = (turns + split - 1) / split * turn;
+    const int64_t grid = p.mt * ((p.n + cols - 1) / cols);
+    launch(k_mm_short<E, TO>, dim3((unsigned)grid), kBlock, 0, st, p, cols);
+}
+
 template <int MI, int NI, typename TO>
 static void mm_direct(MmArgs p, hipStream_t st) {
     p.mt = (p.m + 16 * MI - 1) / (16 * MI);
@@ -485,7 +647,11 @@ static hipError_t mm_t(const MmArgs& p, hipStream_t st) {
     if (aligned && near && p.k > kScaleBlock && ((p.m + kTile - 1) / kTile) * ((p.n + kTile - 1) / kTile) >= 128)
         return p.b_tile ? mm_tile<TO, true>(p, st) : mm_tile<TO, false>(p, st);
     const int64_t waves = ((p.m + 63) / 64) * ((p.n + 63) / 64);   // of 64 x 64
-    if (p.m <= 16) mm_direct<1, 1, TO>(p, st);
+    if (p.k <= kScaleBlock && waves >= 1024) {
+        if (p.k <= 32) mm_short<1, TO>(p, st);
+        else if (p.k <= 64) mm_short<2, TO>(p, st);
+        else mm_short<4, TO>(p, st);
+    } else if (p.m <= 16) mm_direct<1, 1, TO>(p, st);
     else if (waves >= 1024) mm_direct<4, 4, TO>(p, st);
     else mm_direct<2, 2, TO>(p, st);
     return hipGetLastError();
