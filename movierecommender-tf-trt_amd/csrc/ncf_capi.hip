@@ -1523,6 +1523,8 @@ int ncf_matmul_blocks(const void* a, int64_t a_ld, const float* a_scale, const v
     if (int r = check_matrix("b", b, n, k, b_ld)) return r;
     if (int r = check_output("y", y, m, n, y_ld)) return r;
     if (!a_scale || !b_scale) return fail(NCF_EINVAL, "a scale is NULL");
+    if (reinterpret_cast<uintptr_t>(y) % (out_dtype == NCF_F32 ? 4 : 2))
+        return fail(NCF_EINVAL, "y is not aligned to its elements");
     // one workgroup for 16 rows x 64 columns is the finest grid of any variant
     if ((m + 15) / 16 > INT32_MAX / ((n + 15) / 16))
         return fail(NCF_EINVAL, "%lld x %lld is too large a product", (long long)m, (long long)n);

@@ -460,52 +460,76 @@ __global__ __launch_bounds__(kTileThreads, 2) void k_mm_tile(MmArgs p) {
 
 // ----------------------------------------------------------------------------- rows of one block
 //
-// k <= 128, as the factors of the models here: the output's write is the work.  A wave keeps 64 rows of a in
-// registers and goes along the columns, 64 at a time, the next columns' operand loaded meanwhile; their
-// products pass through LDS, so that a store instruction writes 256 bytes of each of four rows of y (from
-// the MFMA's layout it would be 64 bytes of sixteen).
+// k <= 128, as the factors of the models here: the output's write is the work.  A wave keeps 32 rows of a in
+// registers and goes along the columns, 128 bytes of each row of y at a time, the next columns' operand
+// loaded meanwhile; the workgroup's four waves go along the same columns.  Products pass through a ring of
+// two such pieces in LDS, placed by their address in y, so that every store writes whole, aligned lines of
+// 128 bytes whatever the distance of the rows (8,192 x 27,278 fp32, rows 8 bytes off: 16-byte stores at
+// their own addresses took 100 us of 303).
 
-constexpr int kShortRows = 64, kShortCols = 64;
+constexpr int kShortRows = 32;
 constexpr int kShortWaves = kBlock / 64;
+constexpr int kLine = 128;
 
-// 8 values from column c on, zero past column k
-__device__ __forceinline__ uint2 load_q8(const uint8_t* row, int c, int k) {
-    typedef uint32_t u __attribute__((ext_vector_type(2), aligned(1)));
-    if (c + 8 <= k) {
-        const u v = *reinterpret_cast<const u*>(row + c);
-        return make_uint2(v[0], v[1]);
-    }
-    uint32_t w[2] = {0, 0};
-    for (int e = 0; c + e < k; ++e) w[e >> 2] |= (uint32_t)row[c + e] << (8 * (e & 3));
-    return make_uint2(w[0], w[1]);
-}
-
-// A lane's part of a row, as the MFMA takes it.  fp32 outputs: E instructions of 32 columns, 8 a lane;
-// 16-bit outputs: one of 128, 32 a lane.
-template <bool WIDE, int E>
-struct ShortRaw;
+// A lane's part of a row of k <= 32 E values, 8 E of them: for E = 1 the 8 from column 8 g on, else 16 from
+// column 16 g on of each 64.  Loads have no branch: a part that passes column k is read where the row's
+// last values stand and shifted down when it is used (`past`: how many of its values the row has not).
 template <int E>
-struct ShortRaw<true, E> {
+struct ShortRaw {
     uint2 v[E];
-    __device__ __forceinline__ void load(const uint8_t* row, int g, int k) {
-#pragma unroll
-        for (int e = 0; e < E; ++e) v[e] = load_q8(row, 32 * e + 8 * g, k);
+    __device__ __forceinline__ static int past(int e, int g, int k) {
+        return E == 1 ? 8 * g + 8 - max(k, 8) : 64 * (e / 2) + 16 * g + 16 - k;
     }
-};
-template <int E>
-struct ShortRaw<false, E> {
-    mi32x8 v;
-    __device__ __forceinline__ void load(const uint8_t* row, int g, int k) { v = load_frag(row, 32 * g, k); }
+    __device__ __forceinline__ void load(const uint8_t* row, int g, int k) {
+        if constexpr (E == 1) {
+            typedef uint32_t u __attribute__((ext_vector_type(2), aligned(1)));
+            if (k >= 8) {
+                const u w = *reinterpret_cast<const u*>(row + min(8 * g, k - 8));
+                v[0] = make_uint2(w[0], w[1]);
+            } else {
+                v[0] = make_uint2(0, 0);
+                for (int c = 0; c < k; ++c) {
+                    const uint32_t byte = (uint32_t)row[c] << (8 * (c & 3));
+                    if (c < 4) v[0].x |= byte;
+                    else v[0].y |= byte;
+                }
+            }
+        } else {   // (k > 32)
+#pragma unroll
+            for (int e = 0; e < E; e += 2) {
+                const vu32x4 w = load16(row + min(64 * (e / 2) + 16 * g, k - 16));
+                v[e] = make_uint2(w[0], w[1]);
+                v[e + 1] = make_uint2(w[2], w[3]);
+            }
+        }
+    }
+    // the part with zeros past column k
+    __device__ __forceinline__ void settle(int g, int k) {
+        if (k == 32 * E) return;
+#pragma unroll
+        for (int e = 0; e < E; e += 2) {
+            const int n = max(past(e, g, k), 0);
+            const uint64_t lo = (uint64_t)v[e].y << 32 | v[e].x;
+            const uint64_t hi = E == 1 ? 0 : (uint64_t)v[E == 1 ? 0 : e + 1].y << 32 | v[E == 1 ? 0 : e + 1].x;
+            const int bits = 8 * (n & 7);
+            // whole halves first, then bytes
+            const uint64_t l = n >= 16 ? 0 : n >= 8 ? hi : lo, h = n >= 8 ? 0 : hi;
+            const uint64_t rl = bits ? l >> bits | h << (64 - bits) : l, rh = h >> bits;
+            v[e] = make_uint2((uint32_t)rl, (uint32_t)(rl >> 32));
+            if constexpr (E > 1) v[e + 1] = make_uint2((uint32_t)rh, (uint32_t)(rh >> 32));
+        }
+    }
 };
 template <bool WIDE, int E>
 struct ShortOperand;
 template <int E>
 struct ShortOperand<true, E> {
     mf16x8 v[E];
-    __device__ __forceinline__ void set(const ShortRaw<true, E>& r) {
+    __device__ __forceinline__ void set(ShortRaw<E> raw, int g, int k) {
+        raw.settle(g, k);
 #pragma unroll
         for (int e = 0; e < E; ++e) {
-            const mi32x8 f = {(int)r.v[e].x, (int)r.v[e].y, 0, 0, 0, 0, 0, 0};
+            const mi32x8 f = {(int)raw.v[e].x, (int)raw.v[e].y, 0, 0, 0, 0, 0, 0};
             v[e] = widen(f, 0);
         }
     }
@@ -519,90 +543,142 @@ struct ShortOperand<true, E> {
 template <int E>
 struct ShortOperand<false, E> {
     mi32x8 v;
-    __device__ __forceinline__ void set(const ShortRaw<false, E>& r) { v = r.v; }
+    __device__ __forceinline__ void set(ShortRaw<E> raw, int g, int k) {
+        raw.settle(g, k);
+        v = mi32x8{0, 0, 0, 0, 0, 0, 0, 0};
+#pragma unroll
+        for (int e = 0; e < E; ++e) {
+            v[2 * e] = (int)raw.v[e].x;
+            v[2 * e + 1] = (int)raw.v[e].y;
+        }
+    }
     __device__ __forceinline__ static vf32x4 product(const ShortOperand& a, const ShortOperand& b) {
         const vf32x4 zero = {0.0f, 0.0f, 0.0f, 0.0f};
         return __builtin_amdgcn_mfma_scale_f32_16x16x128_f8f6f4(a.v, b.v, zero, 0, 0, 0, 0, 0, 0);
     }
 };
 
-__device__ __forceinline__ vf32x4 load_f4(const float* p, int valid) {
-    vf32x4 r = {0.0f, 0.0f, 0.0f, 0.0f};
-    if (valid >= 4) {
-        typedef float f4 __attribute__((ext_vector_type(4), aligned(4)));
-        return *reinterpret_cast<const f4*>(p);
-    }
+// four neighbouring outputs to their places in a row's ring, G of them at a time
+template <typename TO, int G>
+__device__ __forceinline__ void ring_put(uint8_t* ring, int col, vf32x4 y) {
+    constexpr int S = (int)sizeof(TO), M = 2 * kLine - 1;
+    typedef TO og __attribute__((ext_vector_type(G)));
 #pragma unroll
-    for (int e = 0; e < 3; ++e)
-        if (e < valid) r[e] = p[e];
-    return r;
+    for (int e = 0; e < 4; e += G) {
+        og v;
+#pragma unroll
+        for (int f = 0; f < G; ++f) v[f] = (TO)y[e + f];
+        *reinterpret_cast<og*>(ring + ((col + e) * S & M)) = v;
+    }
 }
 
+constexpr int kShortCols = 512;   // most columns of a workgroup (four workgroups a CU in LDS)
+
 template <int E, typename TO>
-__global__ __launch_bounds__(kBlock) void k_mm_short(MmArgs p, int64_t cols) {
+__global__ __launch_bounds__(kBlock, 4) void k_mm_short(MmArgs p, int cols, int unit) {
     constexpr bool WIDE = std::is_same<TO, float>::value;
-    constexpr int kPad = 4;   // (a row's 16-byte pieces one bank group further than the row above's)
-    __shared__ __attribute__((aligned(16))) float out[kShortWaves][kShortRows][kShortCols + kPad];
+    constexpr int S = (int)sizeof(TO), C = kLine / S;      // columns of a line
+    constexpr int NX = kShortRows / 16, NJ = 2, Step = 16 * NJ;   // columns of a step: a line takes C / Step
+    constexpr int kPitch = 2 * kLine + 16;
+    __shared__ __attribute__((aligned(16))) uint8_t rings[kShortWaves][kShortRows * kPitch];
+    __shared__ __attribute__((aligned(16))) float col_scale[kShortCols], col_bias[kShortCols];
     const int lane = threadIdx.x & 63, g = lane >> 4, i = lane & 15;
     const int wave = __builtin_amdgcn_readfirstlane((int)(threadIdx.x >> 6));
-    const int64_t m0 = blockIdx.x % p.mt * kShortRows;
-    // this wave's column blocks: every kShortWaves-th of the workgroup's
-    const int64_t c0 = blockIdx.x / p.mt * cols, c1 = min(c0 + cols, p.n);
-    ShortOperand<WIDE, E> fa[kShortRows / 16];
-    float sa[kShortRows / 16];
-#pragma unroll
-    for (int x = 0; x < kShortRows / 16; ++x) {
-        const int64_t m = min(m0 + 16 * x + i, p.m - 1);
-        ShortRaw<WIDE, E> raw;
-        raw.load(p.a + m * p.lda, g, p.k);
-        fa[x].set(raw);
-        sa[x] = p.sa[m];
+    const uint32_t mt = (uint32_t)p.mt;
+    const int64_t m0 = ((int64_t)(blockIdx.x % mt) * kShortWaves + wave) * kShortRows;
+    const int64_t c0 = (int64_t)(blockIdx.x / mt) * cols;
+    const int width = (int)min((int64_t)cols, p.n - c0);   // columns of this workgroup, from c0 on
+    for (int c = threadIdx.x; c < cols; c += kBlock) {
+        const int64_t n = c0 + min(c, width - 1);
+        col_scale[c] = p.sb[p.b_tile ? n / kScaleBlock : n];
+        col_bias[c] = p.bias ? p.bias[n] : 0.0f;
     }
-    constexpr int NJ = kShortCols / 16;
-    ShortRaw<WIDE, E> raw[NJ];
-    int64_t n0 = c0 + wave * kShortCols;
-    if (n0 >= c1) return;
-    auto load_b = [&](int64_t n) {
-#pragma unroll
-        for (int j = 0; j < NJ; ++j) raw[j].load(p.b + min(n + 16 * j + i, p.n - 1) * p.ldb, g, p.k);
+    __syncthreads();
+    if (m0 >= p.m) return;
+    uint8_t* ring = rings[wave];
+    // columns (of C) that y[m][c0] lies behind the start of its line
+    auto off_of = [&](int64_t m) {
+        return (int)(((uint64_t)(uintptr_t)p.y / S + (uint64_t)(m * p.ldy + c0)) & (C - 1));
     };
-    load_b(n0);
-    for (; n0 < c1; n0 += kShortWaves * kShortCols) {
-        ShortOperand<WIDE, E> fb[NJ];
-        vf32x4 sb[NJ], bias[NJ];
+    ShortOperand<WIDE, E> fa[NX];
+    float sa[NX];
+    int put[NX];        // the lane's place in a ring for its row and its columns
 #pragma unroll
-        for (int j = 0; j < NJ; ++j) {
-            fb[j].set(raw[j]);
-            const int64_t n = n0 + 16 * j + 4 * g;
-            const int valid = (int)min((int64_t)4, p.n - n);
-            if (p.b_tile) {   // (16 columns from a multiple of 16 on share a tile)
-                const float t = p.sb[min(n, p.n - 1) / kScaleBlock];
-                sb[j] = vf32x4{t, t, t, t};
-            } else {
-                sb[j] = load_f4(p.sb + n, valid);
+    for (int x = 0; x < NX; ++x) {
+        const int64_t m = min(m0 + 16 * x + i, p.m - 1);
+        ShortRaw<E> raw;
+        raw.load(p.a + m * p.lda, g, p.k);
+        fa[x].set(raw, g, p.k);
+        sa[x] = p.sa[m];
+        put[x] = off_of(m) + 4 * g;
+    }
+    // the lane's stores: 16 bytes l % 8 of lines of rows l / 8 + 8 q
+    constexpr int NQ = kShortRows / 8, P = 16 / S;
+    const int piece = lane & 7;
+    TO* to[NQ];         // where the lane's piece of the first line lies
+    int first[NQ];      // its first column, from c0
+#pragma unroll
+    for (int q = 0; q < NQ; ++q) {
+        const int64_t m = min(m0 + 8 * q + (lane >> 3), p.m - 1);
+        first[q] = P * piece - off_of(m);
+        to[q] = static_cast<TO*>(p.y) + m * p.ldy + c0 + first[q];
+    }
+    const uint8_t* b = p.b + c0 * p.ldb;
+    ShortRaw<E> raw[NJ];
+    auto load_b = [&](int n) {   // columns n .. n + Step
+#pragma unroll
+        for (int j = 0; j < NJ; ++j) raw[j].load(b + (int64_t)min(n + 16 * j + i, width - 1) * p.ldb, g, p.k);
+    };
+    load_b(0);
+    // after the columns from n on are in the ring the line that starts n - off is whole; a last turn
+    // without columns writes what is left
+    for (int n = 0; n < width + C; n += C) {
+#pragma unroll
+        for (int h = n; h < n + C; h += Step) {
+            if (h >= width) continue;
+            ShortOperand<WIDE, E> fb[NJ];
+            vf32x4 y[NJ][NX];
+#pragma unroll
+            for (int j = 0; j < NJ; ++j) fb[j].set(raw[j], g, p.k);
+            load_b(min(h + Step, width - 1));
+#pragma unroll
+            for (int j = 0; j < NJ; ++j) {
+                const vf32x4 sb = *reinterpret_cast<const vf32x4*>(&col_scale[h + 16 * j + 4 * g]);
+                const vf32x4 bias = *reinterpret_cast<const vf32x4*>(&col_bias[h + 16 * j + 4 * g]);
+#pragma unroll
+                for (int x = 0; x < NX; ++x) {
+                    const vf32x4 d = ShortOperand<WIDE, E>::product(fb[j], fa[x]);
+#pragma unroll
+                    for (int r = 0; r < 4; ++r) y[j][x][r] = fmaf(sa[x] * sb[r], d[r], bias[r]);
+                }
             }
-            bias[j] = p.bias ? load_f4(p.bias + n, valid) : vf32x4{0.0f, 0.0f, 0.0f, 0.0f};
-        }
-        if (n0 + kShortWaves * kShortCols < c1) load_b(n0 + kShortWaves * kShortCols);
+            auto put_all = [&](auto group) {
 #pragma unroll
-        for (int j = 0; j < NJ; ++j) {
+                for (int j = 0; j < NJ; ++j)
 #pragma unroll
-            for (int x = 0; x < kShortRows / 16; ++x) {
-                const vf32x4 d = ShortOperand<WIDE, E>::product(fb[j], fa[x]);
-                vf32x4 y;
-#pragma unroll
-                for (int r = 0; r < 4; ++r) y[r] = fmaf(sa[x] * sb[j][r], d[r], bias[j][r]);
-                *reinterpret_cast<vf32x4*>(&out[wave][16 * x + i][16 * j + 4 * g]) = y;
-            }
+                    for (int x = 0; x < NX; ++x)
+                        ring_put<TO, decltype(group)::value>(ring + (16 * x + i) * kPitch, h + 16 * j + put[x],
+                                                             y[j][x]);
+            };
+            if (unit >= 4 * S) put_all(std::integral_constant<int, 4>());
+            else if (unit >= 2 * S) put_all(std::integral_constant<int, 2>());
+            else put_all(std::integral_constant<int, 1>());
         }
         asm volatile("" ::: "memory");   // (the wave's own LDS, written and read in order)
-        const int64_t n = n0 + 4 * i;
-        const int valid = (int)min((int64_t)4, p.n - n);
+        if (n >= C && n <= width - C && m0 + kShortRows <= p.m) {
 #pragma unroll
-        for (int q = 0; q < kShortRows / 4; ++q) {
-            const vf32x4 y = *reinterpret_cast<const vf32x4*>(&out[wave][4 * q + g][4 * i]);
-            const int64_t m = m0 + 4 * q + g;
-            if (m < p.m && valid > 0) store_y4(static_cast<TO*>(p.y) + m * p.ldy + n, y, valid);
+            for (int q = 0; q < NQ; ++q)
+                *reinterpret_cast<vu32x4*>(to[q] + n) = *reinterpret_cast<const vu32x4*>(
+                    ring + (8 * q + (lane >> 3)) * kPitch + ((n * S + 16 * piece) & (2 * kLine - 1)));
+        } else {
+#pragma unroll 1
+            for (int q = 0; q < NQ; ++q) {
+                const int row = 8 * q + (lane >> 3), c = n + first[q];
+                const TO* from = reinterpret_cast<const TO*>(ring + row * kPitch +
+                                                             ((n * S + 16 * piece) & (2 * kLine - 1)));
+                for (int e = 0; e < P; ++e)
+                    if (m0 + row < p.m && c + e >= 0 && c + e < width) to[q][n + e] = from[e];
+            }
         }
         asm volatile("" ::: "memory");
     }
@@ -610,13 +686,19 @@ __global__ __launch_bounds__(kBlock) void k_mm_short(MmArgs p, int64_t cols) {
 
 template <int E, typename TO>
 static void mm_short(MmArgs p, hipStream_t st) {
-    p.mt = (p.m + kShortRows - 1) / kShortRows;
-    // columns of a workgroup: whole turns of its waves, about 2048 workgroups together
-    const int64_t turn = kShortWaves * kShortCols, turns = (p.n + turn - 1) / turn;
-    const int64_t split = std::max<int64_t>(1, std::min<int64_t>(turns, 2048 / p.mt));
-    const int64_t cols = (turns + split - 1) / split * turn;
+    constexpr int C = kLine / (int)sizeof(TO);
+    constexpr int64_t rows = kShortWaves * kShortRows;
+    p.mt = (p.m + rows - 1) / rows;
+    // columns of a workgroup: whole lines, at least eight of them where there are, and no more than LDS
+    // holds scales for; about 2048 workgroups together
+    const int64_t lines = (p.n + C - 1) / C;
+    const int64_t split = std::max<int64_t>(1, std::min<int64_t>((lines + 7) / 8, 2048 / p.mt));
+    const int64_t cols = std::min<int64_t>((lines + split - 1) / split * C, kShortCols);
     const int64_t grid = p.mt * ((p.n + cols - 1) / cols);
-    launch(k_mm_short<E, TO>, dim3((unsigned)grid), kBlock, 0, st, p, cols);
+    // the largest power of two, up to four outputs, that divides every row's distance from a line's start
+    const uint64_t bytes = (uint64_t)(uintptr_t)p.y | (p.m > 1 ? (uint64_t)p.ldy * sizeof(TO) : 0);
+    const int unit = (int)std::min<uint64_t>(bytes & (0 - bytes), 16);
+    launch(k_mm_short<E, TO>, dim3((unsigned)grid), kBlock, 0, st, p, (int)cols, unit);
 }
 
 template <int MI, int NI, typename TO>
@@ -648,9 +730,9 @@ static hipError_t mm_t(const MmArgs& p, hipStream_t st) {
         return p.b_tile ? mm_tile<TO, true>(p, st) : mm_tile<TO, false>(p, st);
     const int64_t waves = ((p.m + 63) / 64) * ((p.n + 63) / 64);   // of 64 x 64
     if (p.k <= kScaleBlock && waves >= 1024) {
-        if (p.k <= 32) mm_short<1, TO>(p, st);
-        else if (p.k <= 64) mm_short<2, TO>(p, st);
-        else mm_short<4, TO>(p, st);
+        if (p.k > 64) mm_short<4, TO>(p, st);
+        else if (p.k > 32) mm_short<2, TO>(p, st);
+        else mm_short<1, TO>(p, st);
     } else if (p.m <= 16) mm_direct<1, 1, TO>(p, st);
     else if (waves >= 1024) mm_direct<4, 4, TO>(p, st);
     else mm_direct<2, 2, TO>(p, st);
