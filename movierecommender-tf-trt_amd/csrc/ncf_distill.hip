@@ -74,44 +74,80 @@ __device__ __forceinline__ float wave_max32(float x) {
     return x;
 }
 
+// over a workgroup of NT threads, in the same order for every thread
+template <int NT>
 struct BlockRed {
-    double d[kDistThreads / 64];
-    float f[kDistThreads / 64];
+    double d[2][NT / 64];
+    float f[NT / 64];
 };
-__device__ __forceinline__ double block_sum64(double x, BlockRed& r) {
+template <int NT>
+__device__ __forceinline__ double block_sum64(double x, BlockRed<NT>& r) {
     x = wave_sum64(x);
+    if constexpr (NT == 64) return x;
     __syncthreads();
-    if ((threadIdx.x & 63) == 0) r.d[threadIdx.x >> 6] = x;
+    if ((threadIdx.x & 63) == 0) r.d[0][threadIdx.x >> 6] = x;
     __syncthreads();
-    return (r.d[0] + r.d[1]) + (r.d[2] + r.d[3]);
+    x = 0.0;
+#pragma unroll
+    for (int w = 0; w < NT / 64; ++w) x += r.d[0][w];
+    return x;
 }
-__device__ __forceinline__ double block_max64(double x, BlockRed& r) {
+template <int NT>
+__device__ __forceinline__ void block_sum64(double& x, double& y, BlockRed<NT>& r) {
+    x = wave_sum64(x);
+    y = wave_sum64(y);
+    if constexpr (NT == 64) return;
+    __syncthreads();
+    if ((threadIdx.x & 63) == 0) {
+        r.d[0][threadIdx.x >> 6] = x;
+        r.d[1][threadIdx.x >> 6] = y;
+    }
+    __syncthreads();
+    x = y = 0.0;
+#pragma unroll
+    for (int w = 0; w < NT / 64; ++w) {
+        x += r.d[0][w];
+        y += r.d[1][w];
+    }
+}
+template <int NT>
+__device__ __forceinline__ double block_max64(double x, BlockRed<NT>& r) {
     x = wave_max64(x);
+    if constexpr (NT == 64) return x;
     __syncthreads();
-    if ((threadIdx.x & 63) == 0) r.d[threadIdx.x >> 6] = x;
+    if ((threadIdx.x & 63) == 0) r.d[0][threadIdx.x >> 6] = x;
     __syncthreads();
-    return fmax(fmax(r.d[0], r.d[1]), fmax(r.d[2], r.d[3]));
+#pragma unroll
+    for (int w = 0; w < NT / 64; ++w) x = fmax(x, r.d[0][w]);
+    return x;
 }
-__device__ __forceinline__ float block_max32(float x, BlockRed& r) {
+template <int NT>
+__device__ __forceinline__ float block_max32(float x, BlockRed<NT>& r) {
     x = wave_max32(x);
+    if constexpr (NT == 64) return x;
     __syncthreads();
     if ((threadIdx.x & 63) == 0) r.f[threadIdx.x >> 6] = x;
     __syncthreads();
-    return fmaxf(fmaxf(r.f[0], r.f[1]), fmaxf(r.f[2], r.f[3]));
+#pragma unroll
+    for (int w = 0; w < NT / 64; ++w) x = fmaxf(x, r.f[w]);
+    return x;
 }
+
+// one instruction, right to a unit in the last place; below 2^-126 it may give 0
+__device__ __forceinline__ float pow2(float x) { return __builtin_amdgcn_exp2f(x); }
 
 // a thread's vectors of kVec neighbours: vector j starts at kVec (j kDistThreads + thread)
-template <typename T>
+template <typename T, int NT = kDistThreads>
 __device__ __forceinline__ int vec_at(int j) {
-    return Elem<T>::kVec * (j * kDistThreads + (int)threadIdx.x);
+    return Elem<T>::kVec * (j * NT + (int)threadIdx.x);
 }
 
-template <typename T>
-__device__ __forceinline__ void load_chunk(const T* x, int left, float (&r)[kDistItems]) {
+template <int NT, int EPT, typename T>
+__device__ __forceinline__ void load_chunk(const T* x, int left, float (&r)[EPT]) {
     constexpr int V = Elem<T>::kVec;
 #pragma unroll
-    for (int j = 0; j < kDistItems / V; ++j) {
-        const int o = vec_at<T>(j);
+    for (int j = 0; j < EPT / V; ++j) {
+        const int o = vec_at<T, NT>(j);
         if (o + V <= left) {
             const typename Elem<T>::vec w = *reinterpret_cast<const typename Elem<T>::vec*>(x + o);
 #pragma unroll
@@ -123,13 +159,14 @@ __device__ __forceinline__ void load_chunk(const T* x, int left, float (&r)[kDis
     }
 }
 
-// the chunk's bits of the list
+// the list's bits of the items [first, first + 32 WORDS)
+template <int NT, int WORDS>
 __device__ __forceinline__ void mark_list(const DistArgs& a, int64_t row, int first, uint32_t* bits) {
-    for (int w = threadIdx.x; w < kDistWords; w += kDistThreads) bits[w] = 0;
+    for (int w = threadIdx.x; w < WORDS; w += NT) bits[w] = 0;
     __syncthreads();
-    for (int k = threadIdx.x; k < a.k; k += kDistThreads) {
+    for (int k = threadIdx.x; k < a.k; k += NT) {
         const int64_t i = list_item(a, row, k) - first;
-        if (i >= 0 && i < kDistChunk) atomicOr(&bits[i >> 5], 1u << (i & 31));
+        if (i >= 0 && i < 32 * WORDS) atomicOr(&bits[i >> 5], 1u << (i & 31));
     }
     __syncthreads();
 }
@@ -137,14 +174,14 @@ __device__ __forceinline__ void mark_list(const DistArgs& a, int64_t row, int fi
 // Max and masses of one chunk of a row.
 template <typename T>
 __global__ __launch_bounds__(kDistThreads) void k_distill_sums(DistArgs a) {
-    __shared__ BlockRed red;
+    __shared__ BlockRed<kDistThreads> red;
     __shared__ uint32_t bits[kDistWords];
     constexpr int V = Elem<T>::kVec;
     const int64_t row = blockIdx.x / a.chunks;
     const int chunk = (int)(blockIdx.x - row * a.chunks), first = chunk * kDistChunk;
     float x[kDistItems];
-    load_chunk(static_cast<const T*>(a.x) + row * a.ld + first, a.v - first, x);
-    if (a.ref) mark_list(a, row, first, bits);
+    load_chunk<kDistThreads, kDistItems>(static_cast<const T*>(a.x) + row * a.ld + first, a.v - first, x);
+    if (a.ref) mark_list<kDistThreads, kDistWords>(a, row, first, bits);
     float m = -INFINITY;
 #pragma unroll
     for (int e = 0; e < kDistItems; ++e) m = fmaxf(m, x[e]);
@@ -157,23 +194,87 @@ __global__ __launch_bounds__(kDistThreads) void k_distill_sums(DistArgs a) {
         const uint32_t b = a.ref ? bits[o >> 5] >> (o & 31) : 0u;
 #pragma unroll
         for (int e = 0; e < V; ++e) {
-            const double w = (double)exp2f((x[V * j + e] - base) * a.c2);
+            const double w = (double)pow2((x[V * j + e] - base) * a.c2);
             if (b >> e & 1u) in += w;
             else out += w;
         }
     }
-    out = block_sum64(out, red);
-    in = block_sum64(in, red);
+    block_sum64(out, in, red);
     if (threadIdx.x == 0) {
         a.tops[blockIdx.x] = m;
         a.sums[blockIdx.x] = make_double2(out, in);
     }
 }
 
+// What the gradient of a row needs.
+struct RowState {
+    float base;             // the largest logit
+    double inv_sum, c_in, c_out, ref;
+};
+
+// The row's loss and state from its max m and its masses outside and inside the list; NT threads.
+template <int NT, typename T>
+__device__ __forceinline__ RowState finish_row(const DistArgs& a, int64_t row, const T* x, float m, double out,
+                                               double in, BlockRed<NT>& red) {
+    const float base = m > -INFINITY ? m : 0.0f;
+    const double sum = out + in;
+    // the teacher's reference: given, or the list's own
+    double ref;
+    if (a.ref) {
+        ref = (double)a.ref[row];
+    } else {
+        double top = -INFINITY;
+        for (int k = threadIdx.x; k < a.k; k += NT) {
+            const int64_t i = list_item(a, row, k);
+            if (i >= 0 && i < a.v) top = fmax(top, (double)a.y[row * a.y_ld + k] * a.inv_t);
+        }
+        top = block_max64(top, red);
+        double s = 0.0;
+        for (int k = threadIdx.x; k < a.k; k += NT) {
+            const int64_t i = list_item(a, row, k);
+            if (i >= 0 && i < a.v && top > -INFINITY) s += exp((double)a.y[row * a.y_ld + k] * a.inv_t - top);
+        }
+        s = block_sum64(s, red);
+        ref = s != 0.0 ? top + log(s) : INFINITY;   // no entry: q = 0
+    }
+    const double log_sum = log(sum);
+    double loss = 0.0, q_sum = 0.0;
+    for (int k = threadIdx.x; k < a.k; k += NT) {
+        const int64_t i = list_item(a, row, k);
+        if (i < 0 || i >= a.v) continue;
+        const double lq = (double)a.y[row * a.y_ld + k] * a.inv_t - ref, q = exp(lq);
+        q_sum += q;
+        if (q != 0.0) loss += q * (lq - (((double)(float)x[i] - (double)base) * a.inv_t - log_sum));
+    }
+    block_sum64(loss, q_sum, red);
+    double inside = q_sum, outside = q_sum;
+    if (a.ref) {
+        const double q0 = 1.0 - q_sum;
+        if (q0 > 0.0 && !(out <= 0.0)) {
+            loss += q0 * (log1p(-q_sum) + log1p(in / out));
+            inside = q_sum + q0;
+            outside = inside - q0 * (sum / out);
+        }
+    }
+    const bool none = !(m > -INFINITY) && sum == 0.0;   // (a NaN logit leaves a NaN sum)
+    const RowState st = none ? RowState{base, 0.0, 0.0, 0.0, INFINITY}
+                             : RowState{base, 1.0 / sum, inside, outside, ref};
+    if (threadIdx.x == 0) {
+        double* to = a.state + row * kState;
+        to[0] = st.base;
+        to[1] = st.inv_sum;
+        to[2] = st.c_in;
+        to[3] = st.c_out;
+        to[4] = st.ref;
+        a.loss[row] = none ? 0.0f : (float)loss;
+    }
+    return st;
+}
+
 // The row's loss and what its gradient needs.
 template <typename T>
 __global__ __launch_bounds__(kDistThreads) void k_distill_loss(DistArgs a) {
-    __shared__ BlockRed red;
+    __shared__ BlockRed<kDistThreads> red;
     const int64_t row = blockIdx.x;
     const T* x = static_cast<const T*>(a.x) + row * a.ld;
     float m = -INFINITY;
@@ -188,118 +289,164 @@ __global__ __launch_bounds__(kDistThreads) void k_distill_loss(DistArgs a) {
         out += s.x * f;
         in += s.y * f;
     }
-    out = block_sum64(out, red);
-    in = block_sum64(in, red);
-    const double sum = out + in;
-    // the teacher's reference: given, or the list's own
-    double ref;
-    if (a.ref) {
-        ref = (double)a.ref[row];
-    } else {
-        double top = -INFINITY;
-        for (int k = threadIdx.x; k < a.k; k += kDistThreads) {
-            const int64_t i = list_item(a, row, k);
-            if (i >= 0 && i < a.v) top = fmax(top, (double)a.y[row * a.y_ld + k] * a.inv_t);
-        }
-        top = block_max64(top, red);
-        double s = 0.0;
-        for (int k = threadIdx.x; k < a.k; k += kDistThreads) {
-            const int64_t i = list_item(a, row, k);
-            if (i >= 0 && i < a.v && top > -INFINITY) s += exp((double)a.y[row * a.y_ld + k] * a.inv_t - top);
-        }
-        s = block_sum64(s, red);
-        ref = s != 0.0 ? top + log(s) : INFINITY;   // no entry: q = 0
-    }
-    const double log_sum = log(sum);
-    double loss = 0.0, q_sum = 0.0;
-    for (int k = threadIdx.x; k < a.k; k += kDistThreads) {
-        const int64_t i = list_item(a, row, k);
-        if (i < 0 || i >= a.v) continue;
-        const double lq = (double)a.y[row * a.y_ld + k] * a.inv_t - ref, q = exp(lq);
-        q_sum += q;
-        if (q != 0.0) loss += q * (lq - (((double)(float)x[i] - (double)base) * a.inv_t - log_sum));
-    }
-    loss = block_sum64(loss, red);
-    q_sum = block_sum64(q_sum, red);
-    if (threadIdx.x != 0) return;
-    double inside = q_sum, outside = q_sum;
-    if (a.ref) {
-        const double q0 = 1.0 - q_sum;
-        if (q0 > 0.0 && !(out <= 0.0)) {
-            loss += q0 * (log1p(-q_sum) + log1p(in / out));
-            inside = q_sum + q0;
-            outside = inside - q0 * (sum / out);
-        }
-    }
-    double* st = a.state + row * kState;
-    const bool none = !(m > -INFINITY) && sum == 0.0;   // (a NaN logit leaves a NaN sum)
-    st[0] = base;
-    st[1] = none ? 0.0 : 1.0 / sum;
-    st[2] = none ? 0.0 : inside;
-    st[3] = none ? 0.0 : outside;
-    st[4] = none ? INFINITY : ref;
-    a.loss[row] = none ? 0.0f : (float)loss;
+    block_sum64(out, in, red);
+    finish_row<kDistThreads>(a, row, x, m, out, in, red);
 }
 
-struct ChunkList {
-    uint32_t bits[kDistWords];
-    uint32_t before[kDistWords];               // marked items ahead of each word
-    unsigned long long q[NCF_DISTILL_MAX_K];   // q of the chunk's marked items in 2^-51
-    int scan[4];
+// The list's q by item: a bit map, the marked items ahead of each of its words, and the q of each marked
+// item in units of 2^-51 (integers: the sum of an item's entries does not depend on their order).
+template <int NT, int WORDS>
+struct ItemQ {
+    uint32_t bits[WORDS];
+    uint32_t before[WORDS];
+    unsigned long long q[NCF_DISTILL_MAX_K];
+    uint32_t wave[NT / 64];
+
+    __device__ __forceinline__ uint32_t slot(int o) const {
+        return before[o >> 5] + __popc(bits[o >> 5] & ((1u << (o & 31)) - 1u));
+    }
+    __device__ __forceinline__ double at(int o) const { return (double)q[slot(o)] * 0x1p-51; }
+
+    // from the marked bits (mark_list)
+    __device__ __forceinline__ void fill(const DistArgs& a, int64_t row, int first, double ref) {
+        constexpr int W = (WORDS + NT - 1) / NT;
+        const int lane = threadIdx.x & 63, w0 = W * (int)threadIdx.x;
+        uint32_t n[W], mine = 0;
+#pragma unroll
+        for (int w = 0; w < W; ++w) {
+            n[w] = w0 + w < WORDS ? __popc(bits[w0 + w]) : 0;
+            mine += n[w];
+        }
+        uint32_t inc = mine;
+#pragma unroll
+        for (int d = 1; d < 64; d <<= 1) {
+            const uint32_t o = (uint32_t)__shfl_up((int)inc, d, 64);
+            if (lane >= d) inc += o;
+        }
+        if (lane == 63) wave[threadIdx.x >> 6] = inc;
+        __syncthreads();
+        uint32_t ahead = inc - mine, total = 0;
+#pragma unroll
+        for (int w = 0; w < NT / 64; ++w) {
+            ahead += w < (int)(threadIdx.x >> 6) ? wave[w] : 0;
+            total += wave[w];
+        }
+#pragma unroll
+        for (int w = 0; w < W; ++w) {
+            if (w0 + w < WORDS) before[w0 + w] = ahead;
+            ahead += n[w];
+        }
+        for (uint32_t s = threadIdx.x; s < total; s += NT) q[s] = 0;
+        __syncthreads();
+        for (int k = threadIdx.x; k < a.k; k += NT) {
+            const int64_t i = list_item(a, row, k) - first;
+            if (i < 0 || i >= 32 * WORDS || i + first >= a.v) continue;
+            // (no q of a log-sum-exp passes 1, up to its rounding; a NaN has made c inside and outside NaN)
+            const double e = exp((double)a.y[row * a.y_ld + k] * a.inv_t - ref);
+            atomicAdd(&q[slot((int)i)], (unsigned long long)rint(fmin(e, 2.0) * 0x1p51));
+        }
+        __syncthreads();
+    }
 };
+
+// V neighbours' gradients from their weights, o items behind `first`
+template <typename T, typename Q>
+__device__ __forceinline__ void store_grad(T* out, int o, int left, const float* w, uint32_t b, float p_in,
+                                           float p_out, double g, const Q& l) {
+    constexpr int V = Elem<T>::kVec;
+    float r[V];
+#pragma unroll
+    for (int e = 0; e < V; ++e) r[e] = w[e] * ((b >> e & 1u) ? p_in : p_out);
+    if (b & ((1u << V) - 1u)) {
+#pragma unroll
+        for (int e = 0; e < V; ++e)
+            if (b >> e & 1u) r[e] -= (float)(l.at(o + e) * g);
+    }
+    if (o + V <= left) {
+        typename Elem<T>::vec y;
+#pragma unroll
+        for (int e = 0; e < V; ++e) y[e] = (T)r[e];
+        *reinterpret_cast<typename Elem<T>::vec*>(out + o) = y;
+    } else {
+#pragma unroll
+        for (int e = 0; e < V; ++e)
+            if (o + e < left) out[o + e] = (T)r[e];
+    }
+}
 
 // Gradient of one chunk of a row.
 template <typename T>
 __global__ __launch_bounds__(kDistThreads) void k_distill_grad(DistArgs a) {
-    static_assert(kDistWords == kDistThreads, "one word of the bit map a thread");
-    __shared__ ChunkList l;
+    __shared__ ItemQ<kDistThreads, kDistWords> l;
     constexpr int V = Elem<T>::kVec;
     const int64_t row = blockIdx.x / a.chunks;
     const int chunk = (int)(blockIdx.x - row * a.chunks), first = chunk * kDistChunk;
     float x[kDistItems];
-    load_chunk(static_cast<const T*>(a.x) + row * a.ld + first, a.v - first, x);
+    load_chunk<kDistThreads, kDistItems>(static_cast<const T*>(a.x) + row * a.ld + first, a.v - first, x);
     const double* st = a.state + row * kState;
     const float base = (float)st[0];
-    const double ref = st[4];
     const double g = (double)(a.gl ? a.gl[row] : a.gl_v) * a.inv_t;
     const float p_in = (float)(st[1] * st[2] * g), p_out = (float)(st[1] * st[3] * g);
-    mark_list(a, row, first, l.bits);
-    int total;
-    l.before[threadIdx.x] = (uint32_t)block_exscan_256(__popc(l.bits[threadIdx.x]), l.scan, &total);
-    for (int s = threadIdx.x; s < total; s += kDistThreads) l.q[s] = 0;
-    __syncthreads();
-    auto slot = [&](int o) { return l.before[o >> 5] + __popc(l.bits[o >> 5] & ((1u << (o & 31)) - 1u)); };
-    for (int k = threadIdx.x; k < a.k; k += kDistThreads) {
-        const int64_t i = list_item(a, row, k) - first;
-        if (i < 0 || i >= kDistChunk || i + first >= a.v) continue;
-        const double q = exp((double)a.y[row * a.y_ld + k] * a.inv_t - ref);
-        // integers: the sum of an item's entries does not depend on their order.  (No q of a log-sum-exp
-        // passes 1, up to its rounding; a NaN has made the row's p_in and p_out NaN.)
-        atomicAdd(&l.q[slot((int)i)], (unsigned long long)rint(fmin(q, 2.0) * 0x1p51));
-    }
-    __syncthreads();
+    mark_list<kDistThreads, kDistWords>(a, row, first, l.bits);
+    l.fill(a, row, first, st[4]);
     T* out = static_cast<T*>(a.grad) + row * a.grad_ld + first;
-    const int left = a.v - first;
 #pragma unroll
     for (int j = 0; j < kDistItems / V; ++j) {
         const int o = vec_at<T>(j);
-        const uint32_t b = l.bits[o >> 5] >> (o & 31);
-        float r[V];
+        float w[V];
+#pragma unroll
+        for (int e = 0; e < V; ++e) w[e] = pow2((x[V * j + e] - base) * a.c2);
+        store_grad(out, o, a.v - first, w, l.bits[o >> 5] >> (o & 31), p_in, p_out, g, l);
+    }
+}
+
+// A whole row in a workgroup's registers: read once, its loss, and its gradient written.  NT EPT items at
+// most; 56 of a thread leave two workgroups of 512 a CU.
+template <typename T, int NT, int EPT, bool GRAD>
+__global__ __launch_bounds__(NT) void k_distill_row(DistArgs a) {
+    constexpr int V = Elem<T>::kVec, WORDS = NT * EPT / 32;
+    __shared__ BlockRed<NT> red;
+    __shared__ ItemQ<NT, WORDS> l;
+    const int64_t row = blockIdx.x;
+    const T* px = static_cast<const T*>(a.x) + row * a.ld;
+    float x[EPT];
+    load_chunk<NT, EPT>(px, a.v, x);
+    if (GRAD || a.ref) mark_list<NT, WORDS>(a, row, 0, l.bits);
+    float m = -INFINITY;
+#pragma unroll
+    for (int e = 0; e < EPT; ++e) m = fmaxf(m, x[e]);
+    m = block_max32(m, red);
+    const float base = m > -INFINITY ? m : 0.0f;
+    double out = 0.0, in = 0.0;
+#pragma unroll
+    for (int j = 0; j < EPT / V; ++j) {
+        const int o = vec_at<T, NT>(j);
+        const uint32_t b = a.ref ? l.bits[o >> 5] >> (o & 31) & ((1u << V) - 1u) : 0u;
 #pragma unroll
         for (int e = 0; e < V; ++e) {
-            const float w = exp2f((x[V * j + e] - base) * a.c2);
-            r[e] = w * ((b >> e & 1u) ? p_in : p_out);
-            if (b >> e & 1u) r[e] -= (float)((double)l.q[slot(o + e)] * 0x1p-51 * g);
+            const float w = pow2((x[V * j + e] - base) * a.c2);
+            x[V * j + e] = w;
+            if (b == 0) out += (double)w;
         }
-        if (o + V <= left) {
-            typename Elem<T>::vec w;
+        if (b != 0) {
 #pragma unroll
-            for (int e = 0; e < V; ++e) w[e] = (T)r[e];
-            *reinterpret_cast<typename Elem<T>::vec*>(out + o) = w;
-        } else {
+            for (int e = 0; e < V; ++e) {
+                if (b >> e & 1u) in += (double)x[V * j + e];
+                else out += (double)x[V * j + e];
+            }
+        }
+    }
+    block_sum64(out, in, red);
+    const RowState st = finish_row<NT>(a, row, px, m, out, in, red);
+    if constexpr (GRAD) {
+        const double g = (double)(a.gl ? a.gl[row] : a.gl_v) * a.inv_t;
+        const float p_in = (float)(st.inv_sum * st.c_in * g), p_out = (float)(st.inv_sum * st.c_out * g);
+        l.fill(a, row, 0, st.ref);
+        T* to = static_cast<T*>(a.grad) + row * a.grad_ld;
 #pragma unroll
-            for (int e = 0; e < V; ++e)
-                if (o + e < left) out[o + e] = (T)r[e];
+        for (int j = 0; j < EPT / V; ++j) {
+            const int o = vec_at<T, NT>(j);
+            store_grad(to, o, a.v, x + V * j, l.bits[o >> 5] >> (o & 31), p_in, p_out, g, l);
         }
     }
 }
@@ -340,9 +487,25 @@ int64_t distill_blocks(int64_t rows, int v) {
     return rows > INT64_MAX / c ? INT64_MAX : rows * c;
 }
 
+template <typename T, int NT, int EPT>
+static void distill_row(const DistArgs& a, bool backward, hipStream_t st) {
+    const dim3 grid((unsigned)a.rows);
+    if (backward) launch(k_distill_row<T, NT, EPT, true>, grid, NT, 0, st, a);
+    else launch(k_distill_row<T, NT, EPT, false>, grid, NT, 0, st, a);
+}
+
 template <typename T>
 static hipError_t distill_t(const DistArgs& a, bool forward, bool backward, hipStream_t st) {
     const unsigned grid = (unsigned)(a.rows * a.chunks);
+    // few rows of more than a chunk each would leave CUs idle: those go by chunks
+    const bool by_row = a.v <= kDistChunk || (a.v <= 512 * 56 && a.rows >= 128);
+    if (forward && by_row) {
+        if (a.v <= 64 * 8) distill_row<T, 64, 8>(a, backward, st);
+        else if (a.v <= 64 * 32) distill_row<T, 64, 32>(a, backward, st);
+        else if (a.v <= 256 * 32) distill_row<T, 256, 32>(a, backward, st);
+        else distill_row<T, 512, 56>(a, backward, st);
+        return hipGetLastError();
+    }
     if (forward) {
         launch(k_distill_sums<T>, dim3(grid), kDistThreads, 0, st, a);
         launch(k_distill_loss<T>, dim3((unsigned)a.rows), kDistThreads, 0, st, a);

@@ -92,7 +92,7 @@ def problem(rows, v, k, dtype="float32", seed=0, lse_t=None, index="int64"):
 
 
 def both(x, items, y, t=1.0, lse=None, gl=None):
-    """The three calls; the one-call and the two-call forms have to agree bit for bit."""
+    """The three calls, each against the reference; the one-call form's outputs."""
     dev = lambda a: None if a is None else a.cuda()   # noqa: E731
     g = 1.0 if gl is None else gl.cuda()
     loss, state = C.distill_loss(dev(x), dev(items), dev(y), temperature=t, teacher_lse=dev(lse))
@@ -114,6 +114,14 @@ def test_fp32(size, lse):
     x, items, y, ls = problem(*size, seed=sum(size), lse_t=t if lse else None)
     gl = torch.rand(size[0], generator=torch.Generator().manual_seed(1)) + 0.1
     both(x, items, y, t, ls, gl)
+
+
+@pytest.mark.parametrize("lse", [False, True])
+@pytest.mark.parametrize("size", [(300, 20000, 32, "float32"), (130, 28672, 9, "bfloat16"), (200, 8193, 700, "float16")],
+                         ids=str)
+def test_many_rows(size, lse):
+    x, items, y, ls = problem(*size, seed=2, lse_t=1.0 if lse else None)
+    both(x, items, y, 1.0, ls, torch.rand(size[0], generator=torch.Generator().manual_seed(1)))
 
 
 @pytest.mark.parametrize("dtype", ["bfloat16", "float16"])
