@@ -142,21 +142,34 @@ __device__ __forceinline__ int vec_at(int j) {
     return Elem<T>::kVec * (j * NT + (int)threadIdx.x);
 }
 
+// a thread's EPT logits as they are stored, and as floats; -inf past the end
+template <int EPT, typename T>
+struct Raw {
+    static constexpr int V = Elem<T>::kVec, J = EPT / V;
+    typedef T vec __attribute__((ext_vector_type(V)));
+    vec v[J];
+};
 template <int NT, int EPT, typename T>
-__device__ __forceinline__ void load_chunk(const T* x, int left, float (&r)[EPT]) {
+__device__ __forceinline__ void load_chunk(const T* x, int left, Raw<EPT, T>& r) {
     constexpr int V = Elem<T>::kVec;
 #pragma unroll
     for (int j = 0; j < EPT / V; ++j) {
         const int o = vec_at<T, NT>(j);
         if (o + V <= left) {
-            const typename Elem<T>::vec w = *reinterpret_cast<const typename Elem<T>::vec*>(x + o);
-#pragma unroll
-            for (int e = 0; e < V; ++e) r[V * j + e] = (float)w[e];
+            r.v[j] = *reinterpret_cast<const typename Elem<T>::vec*>(x + o);
         } else {
 #pragma unroll
-            for (int e = 0; e < V; ++e) r[V * j + e] = o + e < left ? (float)x[o + e] : -INFINITY;
+            for (int e = 0; e < V; ++e) r.v[j][e] = o + e < left ? x[o + e] : (T)(-INFINITY);
         }
     }
+}
+template <int EPT, typename T>
+__device__ __forceinline__ void to_floats(const Raw<EPT, T>& r, float (&x)[EPT]) {
+    constexpr int V = Elem<T>::kVec;
+#pragma unroll
+    for (int j = 0; j < EPT / V; ++j)
+#pragma unroll
+        for (int e = 0; e < V; ++e) x[V * j + e] = (float)r.v[j][e];
 }
 
 // the list's bits of the items [first, first + 32 WORDS)
@@ -179,9 +192,11 @@ __global__ __launch_bounds__(kDistThreads) void k_distill_sums(DistArgs a) {
     constexpr int V = Elem<T>::kVec;
     const int64_t row = blockIdx.x / a.chunks;
     const int chunk = (int)(blockIdx.x - row * a.chunks), first = chunk * kDistChunk;
-    float x[kDistItems];
-    load_chunk<kDistThreads, kDistItems>(static_cast<const T*>(a.x) + row * a.ld + first, a.v - first, x);
+    Raw<kDistItems, T> raw;
+    load_chunk<kDistThreads>(static_cast<const T*>(a.x) + row * a.ld + first, a.v - first, raw);
     if (a.ref) mark_list<kDistThreads, kDistWords>(a, row, first, bits);
+    float x[kDistItems];
+    to_floats(raw, x);
     float m = -INFINITY;
 #pragma unroll
     for (int e = 0; e < kDistItems; ++e) m = fmaxf(m, x[e]);
@@ -206,69 +221,101 @@ __global__ __launch_bounds__(kDistThreads) void k_distill_sums(DistArgs a) {
     }
 }
 
+// What depends on a row's list alone: the teacher's reference, sum q, sum q log q and sum q x / t.
+struct ListSums {
+    double ref, q, q_log_q, q_z;
+};
+
+// A thread's first entry of the list, loaded ahead of the row.
+struct ListEntry {
+    int64_t item;   // -1: none
+    double z;       // y / t
+    float x;
+};
+template <typename T>
+__device__ __forceinline__ ListEntry list_entry(const DistArgs& a, int64_t row, const T* x, int k) {
+    ListEntry e{-1, 0.0, 0.0f};
+    if (k < a.k) {
+        const int64_t i = list_item(a, row, k);
+        if (i >= 0 && i < a.v) {
+            e.item = i;
+            e.z = (double)a.y[row * a.y_ld + k] * a.inv_t;
+            e.x = (float)x[i];
+        }
+    }
+    return e;
+}
+// f(entry) for the thread's entries k = thread, thread + NT, ..
+template <int NT, typename T, typename F>
+__device__ __forceinline__ void each_entry(const DistArgs& a, int64_t row, const T* x, const ListEntry& first, F f) {
+    if (first.item >= 0) f(first);
+    for (int k = threadIdx.x + NT; k < a.k; k += NT) {
+        const ListEntry e = list_entry(a, row, x, k);
+        if (e.item >= 0) f(e);
+    }
+}
+
+template <int NT, typename T>
+__device__ __forceinline__ ListSums list_sums(const DistArgs& a, int64_t row, const T* x, const ListEntry& first,
+                                              BlockRed<NT>& red) {
+    ListSums l{};
+    if (a.ref) {   // the teacher's reference: given, or the list's own
+        l.ref = (double)a.ref[row];
+    } else {
+        double top = -INFINITY, s = 0.0;
+        each_entry<NT>(a, row, x, first, [&](const ListEntry& e) { top = fmax(top, e.z); });
+        top = block_max64(top, red);
+        each_entry<NT>(a, row, x, first, [&](const ListEntry& e) {
+            if (top > -INFINITY) s += exp(e.z - top);
+        });
+        s = block_sum64(s, red);
+        l.ref = s != 0.0 ? top + log(s) : INFINITY;   // no entry: q = 0
+    }
+    each_entry<NT>(a, row, x, first, [&](const ListEntry& e) {
+        const double lq = e.z - l.ref, q = exp(lq);
+        l.q += q;
+        if (q != 0.0) {
+            l.q_log_q += q * lq;
+            l.q_z += q * ((double)e.x * a.inv_t);
+        }
+    });
+    block_sum64(l.q, l.q_log_q, red);
+    l.q_z = block_sum64(l.q_z, red);
+    return l;
+}
+
 // What the gradient of a row needs.
 struct RowState {
     float base;             // the largest logit
     double inv_sum, c_in, c_out, ref;
 };
 
-// The row's loss and state from its max m and its masses outside and inside the list; NT threads.
-template <int NT, typename T>
-__device__ __forceinline__ RowState finish_row(const DistArgs& a, int64_t row, const T* x, float m, double out,
-                                               double in, BlockRed<NT>& red) {
-    const float base = m > -INFINITY ? m : 0.0f;
-    const double sum = out + in;
-    // the teacher's reference: given, or the list's own
-    double ref;
-    if (a.ref) {
-        ref = (double)a.ref[row];
-    } else {
-        double top = -INFINITY;
-        for (int k = threadIdx.x; k < a.k; k += NT) {
-            const int64_t i = list_item(a, row, k);
-            if (i >= 0 && i < a.v) top = fmax(top, (double)a.y[row * a.y_ld + k] * a.inv_t);
-        }
-        top = block_max64(top, red);
-        double s = 0.0;
-        for (int k = threadIdx.x; k < a.k; k += NT) {
-            const int64_t i = list_item(a, row, k);
-            if (i >= 0 && i < a.v && top > -INFINITY) s += exp((double)a.y[row * a.y_ld + k] * a.inv_t - top);
-        }
-        s = block_sum64(s, red);
-        ref = s != 0.0 ? top + log(s) : INFINITY;   // no entry: q = 0
+// The state of a row from its max m, its masses outside and inside the list, and the list's sums.
+__device__ __forceinline__ RowState row_state(const DistArgs& a, float m, double out, double in, const ListSums& l) {
+    const double sum = out + in, q0 = 1.0 - l.q;
+    RowState st{m > -INFINITY ? m : 0.0f, 1.0 / sum, l.q, l.q, l.ref};
+    if (a.ref && q0 > 0.0 && !(out <= 0.0)) {
+        st.c_in = l.q + q0;
+        st.c_out = st.c_in - q0 * (sum / out);
     }
-    const double log_sum = log(sum);
-    double loss = 0.0, q_sum = 0.0;
-    for (int k = threadIdx.x; k < a.k; k += NT) {
-        const int64_t i = list_item(a, row, k);
-        if (i < 0 || i >= a.v) continue;
-        const double lq = (double)a.y[row * a.y_ld + k] * a.inv_t - ref, q = exp(lq);
-        q_sum += q;
-        if (q != 0.0) loss += q * (lq - (((double)(float)x[i] - (double)base) * a.inv_t - log_sum));
-    }
-    block_sum64(loss, q_sum, red);
-    double inside = q_sum, outside = q_sum;
-    if (a.ref) {
-        const double q0 = 1.0 - q_sum;
-        if (q0 > 0.0 && !(out <= 0.0)) {
-            loss += q0 * (log1p(-q_sum) + log1p(in / out));
-            inside = q_sum + q0;
-            outside = inside - q0 * (sum / out);
-        }
-    }
-    const bool none = !(m > -INFINITY) && sum == 0.0;   // (a NaN logit leaves a NaN sum)
-    const RowState st = none ? RowState{base, 0.0, 0.0, 0.0, INFINITY}
-                             : RowState{base, 1.0 / sum, inside, outside, ref};
-    if (threadIdx.x == 0) {
-        double* to = a.state + row * kState;
-        to[0] = st.base;
-        to[1] = st.inv_sum;
-        to[2] = st.c_in;
-        to[3] = st.c_out;
-        to[4] = st.ref;
-        a.loss[row] = none ? 0.0f : (float)loss;
-    }
+    if (!(m > -INFINITY) && sum == 0.0) st = RowState{st.base, 0.0, 0.0, 0.0, INFINITY};   // (NaN logits: a NaN sum)
     return st;
+}
+
+// Its loss, by one thread; and the state, for a gradient later.
+__device__ __forceinline__ void write_row(const DistArgs& a, int64_t row, const RowState& st, double out, double in,
+                                          const ListSums& l) {
+    // sum q (log q - log p) with log p = (x - base) / t - log sum
+    double loss = l.q_log_q - (l.q_z - l.q * ((double)st.base * a.inv_t)) + l.q * log(out + in);
+    const double q0 = 1.0 - l.q;
+    if (a.ref && q0 > 0.0 && !(out <= 0.0)) loss += q0 * (log1p(-l.q) + log1p(in / out));
+    double* to = a.state + row * kState;
+    to[0] = st.base;
+    to[1] = st.inv_sum;
+    to[2] = st.c_in;
+    to[3] = st.c_out;
+    to[4] = st.ref;
+    a.loss[row] = st.inv_sum == 0.0 || (l.q == 0.0 && !a.ref) ? 0.0f : (float)loss;
 }
 
 // The row's loss and what its gradient needs.
@@ -277,6 +324,7 @@ __global__ __launch_bounds__(kDistThreads) void k_distill_loss(DistArgs a) {
     __shared__ BlockRed<kDistThreads> red;
     const int64_t row = blockIdx.x;
     const T* x = static_cast<const T*>(a.x) + row * a.ld;
+    const ListEntry entry = list_entry(a, row, x, threadIdx.x);
     float m = -INFINITY;
     for (int c = threadIdx.x; c < a.chunks; c += kDistThreads) m = fmaxf(m, a.tops[row * a.chunks + c]);
     m = block_max32(m, red);
@@ -290,7 +338,8 @@ __global__ __launch_bounds__(kDistThreads) void k_distill_loss(DistArgs a) {
         in += s.y * f;
     }
     block_sum64(out, in, red);
-    finish_row<kDistThreads>(a, row, x, m, out, in, red);
+    const ListSums sums = list_sums<kDistThreads>(a, row, x, entry, red);
+    if (threadIdx.x == 0) write_row(a, row, row_state(a, m, out, in, sums), out, in, sums);
 }
 
 // The list's q by item: a bit map, the marked items ahead of each of its words, and the q of each marked
@@ -374,25 +423,28 @@ __device__ __forceinline__ void store_grad(T* out, int o, int left, const float*
     }
 }
 
-// Gradient of one chunk of a row.
-template <typename T>
-__global__ __launch_bounds__(kDistThreads) void k_distill_grad(DistArgs a) {
-    __shared__ ItemQ<kDistThreads, kDistWords> l;
-    constexpr int V = Elem<T>::kVec;
-    const int64_t row = blockIdx.x / a.chunks;
-    const int chunk = (int)(blockIdx.x - row * a.chunks), first = chunk * kDistChunk;
-    float x[kDistItems];
-    load_chunk<kDistThreads, kDistItems>(static_cast<const T*>(a.x) + row * a.ld + first, a.v - first, x);
+// Gradient of NT EPT items of a row, `chunks` such a row.  From the last row to the first: what the pass over
+// the sums read last is still in the cache.
+template <typename T, int NT, int EPT>
+__global__ __launch_bounds__(NT) void k_distill_grad(DistArgs a, int chunks) {
+    constexpr int V = Elem<T>::kVec, WORDS = NT * EPT / 32;
+    __shared__ ItemQ<NT, WORDS> l;
+    const int64_t at = (int64_t)gridDim.x - 1 - blockIdx.x, row = at / chunks;
+    const int first = (int)(at - row * chunks) * NT * EPT;
+    Raw<EPT, T> raw;
+    load_chunk<NT>(static_cast<const T*>(a.x) + row * a.ld + first, a.v - first, raw);
     const double* st = a.state + row * kState;
     const float base = (float)st[0];
     const double g = (double)(a.gl ? a.gl[row] : a.gl_v) * a.inv_t;
     const float p_in = (float)(st[1] * st[2] * g), p_out = (float)(st[1] * st[3] * g);
-    mark_list<kDistThreads, kDistWords>(a, row, first, l.bits);
+    mark_list<NT, WORDS>(a, row, first, l.bits);
     l.fill(a, row, first, st[4]);
     T* out = static_cast<T*>(a.grad) + row * a.grad_ld + first;
+    float x[EPT];
+    to_floats(raw, x);
 #pragma unroll
-    for (int j = 0; j < kDistItems / V; ++j) {
-        const int o = vec_at<T>(j);
+    for (int j = 0; j < EPT / V; ++j) {
+        const int o = vec_at<T, NT>(j);
         float w[V];
 #pragma unroll
         for (int e = 0; e < V; ++e) w[e] = pow2((x[V * j + e] - base) * a.c2);
@@ -403,15 +455,22 @@ __global__ __launch_bounds__(kDistThreads) void k_distill_grad(DistArgs a) {
 // A whole row in a workgroup's registers: read once, its loss, and its gradient written.  NT EPT items at
 // most; 56 of a thread leave two workgroups of 512 a CU.
 template <typename T, int NT, int EPT, bool GRAD>
-__global__ __launch_bounds__(NT) void k_distill_row(DistArgs a) {
+__global__ __launch_bounds__(NT, 4) void k_distill_row(DistArgs a) {
     constexpr int V = Elem<T>::kVec, WORDS = NT * EPT / 32;
     __shared__ BlockRed<NT> red;
     __shared__ ItemQ<NT, WORDS> l;
     const int64_t row = blockIdx.x;
     const T* px = static_cast<const T*>(a.x) + row * a.ld;
-    float x[EPT];
-    load_chunk<NT, EPT>(px, a.v, x);
+    // the list first: its arithmetic and the row do not fit the registers together (the CU's other workgroup
+    // reads meanwhile)
+    const ListSums sums = list_sums<NT>(a, row, px, list_entry(a, row, px, threadIdx.x), red);
     if (GRAD || a.ref) mark_list<NT, WORDS>(a, row, 0, l.bits);
+    if constexpr (GRAD) l.fill(a, row, 0, sums.ref);
+    __builtin_amdgcn_sched_barrier(0);
+    Raw<EPT, T> raw;
+    load_chunk<NT>(px, a.v, raw);
+    float x[EPT];
+    to_floats(raw, x);
     float m = -INFINITY;
 #pragma unroll
     for (int e = 0; e < EPT; ++e) m = fmaxf(m, x[e]);
@@ -435,20 +494,24 @@ __global__ __launch_bounds__(NT) void k_distill_row(DistArgs a) {
                 else out += (double)x[V * j + e];
             }
         }
+        __builtin_amdgcn_sched_barrier(0);   // (a vector at a time: registers for one)
     }
     block_sum64(out, in, red);
-    const RowState st = finish_row<NT>(a, row, px, m, out, in, red);
+    const RowState st = row_state(a, m, out, in, sums);
     if constexpr (GRAD) {
         const double g = (double)(a.gl ? a.gl[row] : a.gl_v) * a.inv_t;
         const float p_in = (float)(st.inv_sum * st.c_in * g), p_out = (float)(st.inv_sum * st.c_out * g);
-        l.fill(a, row, 0, st.ref);
+        const double q_g = st.inv_sum != 0.0 ? g : 0.0;   // (a row with no logit left has no gradient)
         T* to = static_cast<T*>(a.grad) + row * a.grad_ld;
 #pragma unroll
         for (int j = 0; j < EPT / V; ++j) {
             const int o = vec_at<T, NT>(j);
-            store_grad(to, o, a.v, x + V * j, l.bits[o >> 5] >> (o & 31), p_in, p_out, g, l);
+            store_grad(to, o, a.v, x + V * j, l.bits[o >> 5] >> (o & 31), p_in, p_out, q_g, l);
+            __builtin_amdgcn_sched_barrier(0);
         }
     }
+    // (the logarithms last: they and the row do not fit the registers together)
+    if (threadIdx.x == 0) write_row(a, row, st, out, in, sums);
 }
 
 static DistArgs dist_args(const ncf_distill_t& c, void* ws) {
@@ -510,7 +573,11 @@ static hipError_t distill_t(const DistArgs& a, bool forward, bool backward, hipS
         launch(k_distill_sums<T>, dim3(grid), kDistThreads, 0, st, a);
         launch(k_distill_loss<T>, dim3((unsigned)a.rows), kDistThreads, 0, st, a);
     }
-    if (backward) launch(k_distill_grad<T>, dim3(grid), kDistThreads, 0, st, a);
+    if (backward) {
+        if (a.v <= 64 * 8) launch(k_distill_grad<T, 64, 8>, dim3((unsigned)a.rows), 64, 0, st, a, 1);
+        else if (a.v <= 64 * 32) launch(k_distill_grad<T, 64, 32>, dim3((unsigned)a.rows), 64, 0, st, a, 1);
+        else launch(k_distill_grad<T, kDistThreads, kDistItems>, dim3(grid), kDistThreads, 0, st, a, a.chunks);
+    }
     return hipGetLastError();
 }
 
