@@ -502,12 +502,20 @@ int ncf_shard_predict(const ncf_shape_t* shape, const ncf_model_t* model, int32_
  * 1 <= k <= NCF_SCORE_MAX_K; n_users <= the max_users the workspace was sized for. */
 #define NCF_SCORE_FP16 0
 #define NCF_SCORE_FP32 1
+#define NCF_SCORE_FP8 2
 #define NCF_SCORE_MAX_K 32
 int ncf_score_supported(const ncf_shape_t* shape, int32_t precision);
 int ncf_score_workspace_size(const ncf_shape_t* shape, int64_t max_users, size_t* bytes);
 int ncf_score_topk(const ncf_shape_t* shape, const ncf_model_t* model, const int32_t* users, int64_t n_users,
                    int32_t k, int32_t precision, int32_t* top_items, float* top_scores, void* ws, size_t ws_bytes,
                    void* stream);
+/* The logits (output/Sigmoid's input) of n_users users for every item: logits[n_users][num_items].  A user
+ * outside [0, num_users) gives a row of NaN.
+ *   NCF_SCORE_FP16, NCF_SCORE_FP32: as above; NCF_SCORE_FP8: GMF-only models, the product of the block-scaled
+ *   8-bit factors (ncf_matmul_blocks).  ncf_score_supported() says which a shape has. */
+int ncf_score_logits_workspace_size(const ncf_shape_t* shape, int64_t max_users, int32_t precision, size_t* bytes);
+int ncf_score_logits(const ncf_shape_t* shape, const ncf_model_t* model, const int32_t* users, int64_t n_users,
+                     int32_t precision, float* logits, void* ws, size_t ws_bytes, void* stream);
 
 /* Catalogue operators: a user's logits over all items, drawing items from them, and learning them
  * from a teacher (movierec/catalogue.py).  Matrices are row-major with their last dimension dense;

@@ -1529,7 +1529,7 @@ int ncf_matmul_blocks(const void* a, int64_t a_ld, const float* a_scale, const v
     if ((m + 15) / 16 > INT32_MAX / ((n + 15) / 16))
         return fail(NCF_EINVAL, "%lld x %lld is too large a product", (long long)m, (long long)n);
     return hip_check(ncf::launch_matmul_blocks(static_cast<const uint8_t*>(a), a_ld, a_scale,
-                                               static_cast<const uint8_t*>(b), b_ld, b_scale, b_tile != 0, bias, m, n,
+                                               static_cast<const uint8_t*>(b), b_ld, b_scale, b_tile != 0, bias, 1, m, n,
                                                (int)k, out_dtype, y, y_ld, (hipStream_t)stream),
                      "ncf_matmul_blocks");
 }
@@ -1627,6 +1627,62 @@ int ncf_score_supported(const ncf_shape_t* s, int32_t precision) {
     if (check_shape(s)) return 0;
     if (precision == NCF_SCORE_FP32) return 1;
     if (precision == NCF_SCORE_FP16) return ncf::score_fast_supported(*s) ? 1 : 0;
+    if (precision == NCF_SCORE_FP8) return s->num_layers == 0 ? 1 : 0;
+    return 0;
+}
+
+int ncf_score_logits_workspace_size(const ncf_shape_t* s, int64_t max_users, int32_t precision, size_t* bytes) {
+    if (int r = check_shape(s)) return r;
+    if (!bytes) return fail(NCF_EINVAL, "bytes is NULL");
+    if (max_users <= 0 || max_users > ((int64_t)1 << 26))
+        return fail(NCF_EINVAL, "max_users must be in [1, 2^26], got %lld", (long long)max_users);
+    if (!ncf_score_supported(s, precision))
+        return fail(NCF_EINVAL, "this model's logits are not computed in precision %d", precision);
+    *bytes = precision == NCF_SCORE_FP8 ? ncf::gmf_layout(*s, max_users).total
+                                        : ncf::make_score_layout(*s, max_users).total;
+    return 0;
+}
+
+int ncf_score_logits(const ncf_shape_t* s, const ncf_model_t* model, const int32_t* users, int64_t n,
+                     int32_t precision, float* logits, void* ws, size_t ws_bytes, void* stream) {
+    if (int r = check_shape(s)) return r;
+    if (n < 0) return fail(NCF_EINVAL, "n_users must be >= 0, got %lld", (long long)n);
+    if (n == 0) return 0;
+    size_t need = 0;
+    if (int r = ncf_score_logits_workspace_size(s, n, precision, &need)) return r;
+    if (!model || !model->emb || !model->mlp || !users || !logits) return fail(NCF_EINVAL, "NULL device pointer");
+    if (!ws || ws_bytes < need)
+        return fail(NCF_EINVAL, "logits workspace of %zu bytes for %lld users (need %zu)", ws ? ws_bytes : (size_t)0,
+                    (long long)n, need);
+    hipStream_t st = (hipStream_t)stream;
+    if (precision == NCF_SCORE_FP8) {
+        if (n > INT32_MAX / s->gmf_dim)
+            return fail(NCF_EINVAL, "%lld users are too many in one call", (long long)n);
+        return hip_check(ncf::launch_gmf_logits(*s, ws, model->emb, model->mlp, users, n, logits, st), "GMF logits");
+    }
+    const ncf::ScoreLayout L = ncf::make_score_layout(*s, n);
+    hipError_t e;
+    if (precision == NCF_SCORE_FP16) {
+        e = ncf::launch_score_prep(*s, L, ws, model->emb, model->mlp, users, n, st);
+        if (e != hipSuccess) return hip_check(e, "score preparation");
+        return hip_check(ncf::launch_score_logits(*s, L, ws, n, logits, st), "score logits");
+    }
+    const int64_t I = s->num_items;
+    if (I > ncf::kMaxBatch)
+        return fail(NCF_EINVAL, "the fp32 scorer handles catalogues of up to %lld items", (long long)ncf::kMaxBatch);
+    void* pws = ncf::at<char>(ws, L.pred_ws);
+    const ncf::WsLayout PL = ncf::make_layout(*s, L.chunk * I);
+    for (int64_t q0 = 0; q0 < n; q0 += L.chunk) {
+        const int64_t nq = n - q0 < L.chunk ? n - q0 : L.chunk;
+        int32_t* pu = ncf::at<int32_t>(ws, L.pu);
+        int32_t* pi = ncf::at<int32_t>(ws, L.pi);
+        e = ncf::launch_score_pairs(users + q0, nq, (int)I, pu, pi, st);
+        if (e != hipSuccess) return hip_check(e, "score pairs");
+        int nbce = 0;
+        e = ncf::launch_predict_generic(*s, PL, pws, model->emb, model->mlp, pu, pi, nullptr, nq * I,
+                                        logits + q0 * I, ncf::table_ids(*s), &nbce, st, true);
+        if (e != hipSuccess) return hip_check(e, "score forward");
+    }
     return 0;
 }
 

@@ -222,11 +222,11 @@ struct MmArgs {
     const uint8_t* b;
     const float* sa;    // [m][kb]
     const float* sb;    // [n][kb], or [ceil(n / 128)][kb] with b_tile
-    const float* bias;  // [n] or NULL
+    const float* bias;  // [n], bias_step apart, or NULL
     void* y;
     int64_t lda, ldb, ldy;
     int64_t m, n;
-    int k, kb, b_tile;
+    int k, kb, b_tile, bias_step;
     int64_t mt, nt;     // tiles along m and n
 };
 
@@ -302,7 +302,7 @@ __global__ __launch_bounds__(kBlock) void k_mm_direct(MmArgs p) {
         if (p.bias)
 #pragma unroll
             for (int r = 0; r < 4; ++r)
-                if (r < valid) bias[r] = p.bias[n + r];
+                if (r < valid) bias[r] = p.bias[(n + r) * p.bias_step];
 #pragma unroll
         for (int x = 0; x < MI; ++x) {
             const int64_t m = m0 + 16 * x + i;
@@ -449,7 +449,7 @@ __global__ __launch_bounds__(kTileThreads, 2) void k_mm_tile(MmArgs p) {
         if (p.bias)
 #pragma unroll
             for (int r = 0; r < 4; ++r)
-                if (r < valid) bias[r] = p.bias[n + r];
+                if (r < valid) bias[r] = p.bias[(n + r) * p.bias_step];
 #pragma unroll
         for (int x = 0; x < kTileMI; ++x) {
             const int64_t m = m0 + wm + 16 * x + i;
@@ -591,7 +591,7 @@ __global__ __launch_bounds__(kBlock, 4) void k_mm_short(MmArgs p, int cols, int 
     for (int c = threadIdx.x; c < cols; c += kBlock) {
         const int64_t n = c0 + min(c, width - 1);
         col_scale[c] = p.sb[p.b_tile ? n / kScaleBlock : n];
-        col_bias[c] = p.bias ? p.bias[n] : 0.0f;
+        col_bias[c] = p.bias ? p.bias[n * p.bias_step] : 0.0f;
     }
     __syncthreads();
     if (m0 >= p.m) return;
@@ -740,13 +740,68 @@ static hipError_t mm_t(const MmArgs& p, hipStream_t st) {
 }
 
 hipError_t launch_matmul_blocks(const uint8_t* a, int64_t lda, const float* sa, const uint8_t* b, int64_t ldb,
-                                const float* sb, int b_tile, const float* bias, int64_t m, int64_t n, int k,
-                                int out_dtype, void* y, int64_t ldy, hipStream_t st) {
+                                const float* sb, int b_tile, const float* bias, int bias_step, int64_t m, int64_t n,
+                                int k, int out_dtype, void* y, int64_t ldy, hipStream_t st) {
     if (m <= 0 || n <= 0) return hipSuccess;
-    MmArgs p{a, b, sa, sb, bias, y, lda, ldb, ldy, m, n, k, (k + kScaleBlock - 1) / kScaleBlock, b_tile, 0, 0};
+    MmArgs p{a, b, sa, sb, bias, y, lda, ldb, ldy, m, n, k, (k + kScaleBlock - 1) / kScaleBlock, b_tile, bias_step, 0, 0};
     if (out_dtype == NCF_F32) return mm_t<float>(p, st);
     if (out_dtype == NCF_BF16) return mm_t<__bf16>(p, st);
     return mm_t<_Float16>(p, st);
+}
+
+// ----------------------------------------------------------------------------- GMF-only models
+//
+// z(u, i) = sum_f w_f e_u,f e_i,f + b (movierec/model.py:184-188 without hidden layers): the factors of the
+// users, times w, against the table's item rows.
+
+__global__ __launch_bounds__(kBlock) void k_gmf_users(const float* __restrict__ emb, const float* __restrict__ w,
+                                                      const int32_t* __restrict__ users, int64_t n, int num_users,
+                                                      int width, int dim, float* __restrict__ out) {
+    const int64_t x = (int64_t)blockIdx.x * kBlock + threadIdx.x;
+    if (x >= n * dim) return;
+    const int64_t q = x / dim;
+    const int f = (int)(x - q * dim), u = users[q];
+    out[x] = u >= 0 && u < num_users ? w[f] * emb[(int64_t)u * width + f] : __int_as_float(0x7fc00000);
+}
+
+GmfLayout gmf_layout(const ncf_shape_t& s, int64_t n) {
+    GmfLayout l{};
+    size_t off = 0;
+    auto take = [&](size_t bytes) {
+        const size_t at = off;
+        off = (off + bytes + 255) / 256 * 256;
+        return at;
+    };
+    const int64_t kb = (s.gmf_dim + kScaleBlock - 1) / kScaleBlock;
+    l.q_ld = (s.gmf_dim + 15) / 16 * 16;
+    l.uf = take((size_t)n * s.gmf_dim * 4);
+    l.uq = take((size_t)n * l.q_ld);
+    l.us = take((size_t)n * kb * 4);
+    l.iq = take((size_t)s.num_items * l.q_ld);
+    l.is = take((size_t)s.num_items * kb * 4);
+    l.total = off;
+    return l;
+}
+
+hipError_t launch_gmf_logits(const ncf_shape_t& s, void* ws, const float* emb, const float* mlp, const int32_t* users,
+                             int64_t n, float* logits, hipStream_t st) {
+    const GmfLayout l = gmf_layout(s, n);
+    const int dim = s.gmf_dim;
+    float* uf = at<float>(ws, l.uf);
+    const float* w = mlp + s.layer_off[0];
+    launch(k_gmf_users, dim3((unsigned)((n * dim + kBlock - 1) / kBlock)), kBlock, 0, st, emb, w, users, n, s.num_users,
+           s.row_width, dim, uf);
+    hipError_t e = hipGetLastError();
+    if (e == hipSuccess)
+        e = launch_quantize(uf, NCF_F32, n, dim, dim, 0, at<uint8_t>(ws, l.uq), l.q_ld, at<float>(ws, l.us), st);
+    if (e == hipSuccess)
+        e = launch_quantize(emb + (int64_t)s.num_users * s.row_width, NCF_F32, s.num_items, dim, s.row_width, 0,
+                            at<uint8_t>(ws, l.iq), l.q_ld, at<float>(ws, l.is), st);
+    if (e == hipSuccess)
+        e = launch_matmul_blocks(at<uint8_t>(ws, l.uq), l.q_ld, at<float>(ws, l.us), at<uint8_t>(ws, l.iq), l.q_ld,
+                                 at<float>(ws, l.is), 0, w + s.out_features, 0, n, s.num_items, dim, NCF_F32, logits,
+                                 s.num_items, st);
+    return e;
 }
 
 }  // namespace ncf

@@ -62,7 +62,8 @@ static GenShape make_gen_shape(const ncf_shape_t& s, IdSpace ids) {
 
 constexpr int kLdsWeightsMax = 12288;  // floats (48 KB) of dense weights staged in LDS
 
-template <bool TRAIN>
+// LOGIT: probs takes the logits, not their sigmoids
+template <bool TRAIN, bool LOGIT = false>
 __global__ __launch_bounds__(kBlock) void k_fb_generic(GenShape S, const float* __restrict__ emb,
                                                        const float* __restrict__ mlp,
                                                        const int32_t* __restrict__ users,
@@ -117,7 +118,7 @@ __global__ __launch_bounds__(kBlock) void k_fb_generic(GenShape S, const float* 
                 for (int o = 0; o < S.L[S.n - 1]; ++o) z += hl[o] * wo[S.G + o];
             }
             z += wo[S.F];
-            p = 1.0f / (1.0f + expf(-z));
+            p = LOGIT ? z : 1.0f / (1.0f + expf(-z));
         } else {
             p = __int_as_float(0x7fc00000);
             for (int k = 0; k < S.A; ++k) a[k] = 0.0f;
@@ -247,11 +248,11 @@ hipError_t launch_fb_generic(const ncf_shape_t& s, const WsLayout& L, void* ws, 
 hipError_t launch_predict_generic(const ncf_shape_t& s, const WsLayout& L, void* ws, const float* emb,
                                   const float* mlp, const int32_t* users, const int32_t* items,
                                   const float* labels, int64_t n, float* probs, IdSpace ids, int* nbce,
-                                  hipStream_t st) {
+                                  hipStream_t st, bool logit) {
     const GenShape S = make_gen_shape(s, ids);
     const int use_lds = s.mlp_params <= kLdsWeightsMax ? 1 : 0;
     const int grid = (int)((n + kBlock - 1) / kBlock);
-    launch(k_fb_generic<false>, grid, kBlock, use_lds ? (size_t)s.mlp_params * 4 : 0, st, 
+    launch(logit ? k_fb_generic<false, true> : k_fb_generic<false>, grid, kBlock, use_lds ? (size_t)s.mlp_params * 4 : 0, st, 
         S, emb, mlp, users, items, labels, n, 0.0f, probs, at<float>(ws, L.act), nullptr, nullptr,
         labels ? at<float>(ws, L.part_bce) : nullptr, use_lds);
     *nbce = labels ? grid : 0;

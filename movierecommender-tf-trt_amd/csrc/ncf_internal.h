@@ -756,7 +756,7 @@ hipError_t launch_fb_generic(const ncf_shape_t& s, const WsLayout& L, void* ws, 
 hipError_t launch_predict_generic(const ncf_shape_t& s, const WsLayout& L, void* ws, const float* emb,
                                   const float* mlp, const int32_t* users, const int32_t* items,
                                   const float* labels, int64_t n, float* probs, IdSpace ids, int* nbce,
-                                  hipStream_t st);
+                                  hipStream_t st, bool logit = false);
 
 // fused MFMA forward+backward (shapes with s.fast_path); same outputs as the generic kernel
 // also computes the hr/dcg group metrics in-kernel when group divides 32 (*nmet = partial count, else 0)
@@ -990,6 +990,8 @@ hipError_t launch_score_prep(const ncf_shape_t& s, const ScoreLayout& L, void* w
                              const float* mlp, const int32_t* users, int64_t n, hipStream_t st);
 hipError_t launch_score_main(const ncf_shape_t& s, const ScoreLayout& L, void* ws, int64_t n, int k,
                              int32_t* top_items, float* top_scores, hipStream_t st);
+hipError_t launch_score_logits(const ncf_shape_t& s, const ScoreLayout& L, void* ws, int64_t n, float* logits,
+                               hipStream_t st);
 hipError_t launch_score_pairs(const int32_t* users, int64_t nq, int I, int32_t* pu, int32_t* pi, hipStream_t st);
 hipError_t launch_topk_rows(const float* probs, int64_t rows, int I, int k, int32_t* top_items, float* top_scores,
                             hipStream_t st);
@@ -998,8 +1000,16 @@ hipError_t launch_topk_rows(const float* probs, int64_t rows, int I, int k, int3
 hipError_t launch_quantize(const void* x, int dtype, int64_t rows, int cols, int64_t ld, int tile, uint8_t* q,
                            int64_t q_ld, float* scale, hipStream_t st);
 hipError_t launch_matmul_blocks(const uint8_t* a, int64_t lda, const float* sa, const uint8_t* b, int64_t ldb,
-                                const float* sb, int b_tile, const float* bias, int64_t m, int64_t n, int k,
-                                int out_dtype, void* y, int64_t ldy, hipStream_t st);
+                                const float* sb, int b_tile, const float* bias, int bias_step, int64_t m, int64_t n,
+                                int k, int out_dtype, void* y, int64_t ldy, hipStream_t st);
+// logits of a GMF-only model: w * user factors (NaN for an id outside the table), both sides quantised, product
+struct GmfLayout {
+    size_t uf, uq, us, iq, is, total;
+    int64_t q_ld;
+};
+GmfLayout gmf_layout(const ncf_shape_t& s, int64_t n);
+hipError_t launch_gmf_logits(const ncf_shape_t& s, void* ws, const float* emb, const float* mlp, const int32_t* users,
+                             int64_t n, float* logits, hipStream_t st);
 
 // drawing items (ncf_draw.hip), distillation (ncf_distill.hip)
 hipError_t launch_draw(const ncf_draw_t& d, hipStream_t st);

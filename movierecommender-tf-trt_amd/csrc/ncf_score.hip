@@ -196,6 +196,7 @@ struct ScoreArgs {
     float* top_scores;
     float2* part;           // splits > 1: per-range lists [split][nub*32][k] of (logit, item)
     int32_t* gthr;          // per user: best k-th logit published by any of its ranges (ordered key)
+    float* logits;          // LOGITS: [n][num_items]
 };
 
 // float <-> int key with the same order (atomicMax on floats of either sign)
@@ -207,7 +208,8 @@ __device__ __forceinline__ float unkey(int k) { return __int_as_float(k >= 0 ? k
 // admission bound from another range's k-th best g: admit z >= g (ties resolve in the merge)
 __device__ __forceinline__ float below(float g) { return g - fmaxf(fabsf(g) * 1e-6f, 1e-30f); }
 
-template <int KS2, int KS3, int NR3, int KSG>
+// LOGITS: every logit to memory, no lists.
+template <int KS2, int KS3, int NR3, int KSG, bool LOGITS = false>
 __global__ __launch_bounds__(kBlock, 2) void k_score_topk(ScoreArgs a) {
     constexpr int L1P = 16 * KS2;
     __shared__ __attribute__((aligned(16))) _Float16 s_nega[4][32][L1P];
@@ -400,6 +402,16 @@ __global__ __launch_bounds__(kBlock, 2) void k_score_topk(ScoreArgs a) {
 #endif
 #undef NCF_SCORE_LAYER2
 #undef NCF_SCORE_USER_OPS
+        if constexpr (LOGITS) {
+            // two users' 128 bytes an instruction; an id outside the table gives NaN
+            flagged = 0;
+            const uint64_t known = __builtin_amdgcn_ballot_w64(lane < 32 && thr < 0.0f);
+#pragma unroll 4
+            for (int q = h; q < 32; q += 2)
+                if (q0 + q < a.n && 32 * t + j < a.num_items)
+                    a.logits[(q0 + q) * a.num_items + 32 * t + j] =
+                        (known >> q & 1u) ? s_z[w][q][j] : __int_as_float(0x7fc00000);
+        }
         // the next tile's item operands: loads in flight over the insertions below
 #if NCF_DIAG_SCORE == 2
         flagged = 0;
@@ -449,6 +461,7 @@ __global__ __launch_bounds__(kBlock, 2) void k_score_topk(ScoreArgs a) {
             }
         }
     }
+    if constexpr (LOGITS) return;
     for (int q = 0; q < 32; ++q) {
         if (q0 + q >= a.n) break;
         if (lane < K) {
@@ -638,11 +651,9 @@ hipError_t launch_score_prep(const ncf_shape_t& s, const ScoreLayout& L, void* w
     return hipGetLastError();
 }
 
-hipError_t launch_score_main(const ncf_shape_t& s, const ScoreLayout& L, void* ws, int64_t n, int k,
-                             int32_t* top_items, float* top_scores, hipStream_t st) {
-    const ScoreDims d = score_dims(s);
+static ScoreArgs score_args(const ncf_shape_t& s, const ScoreLayout& L, void* ws, int64_t n) {
     const int nub = cdiv_i(n, 32);
-    ScoreArgs a;
+    ScoreArgs a{};
     a.ic = at<const f16x8>(ws, L.ic);
     a.ig = at<const f16x8>(ws, L.ig);
     a.nega = at<const _Float16>(ws, L.nega);
@@ -658,13 +669,36 @@ hipError_t launch_score_main(const ncf_shape_t& s, const ScoreLayout& L, void* w
     a.nub = nub;
     a.ntiles = cdiv_i(s.num_items, 32);
     a.num_items = s.num_items;
-    a.k = k;
-    a.top_items = top_items;
-    a.top_scores = top_scores;
     a.splits = score_splits(a.ntiles);
     a.tiles_per = cdiv_i(a.ntiles, a.splits);
     a.part = at<float2>(ws, L.part);
     a.gthr = at<int32_t>(ws, L.gthr);
+    return a;
+}
+
+// Every logit of n users (after launch_score_prep).
+hipError_t launch_score_logits(const ncf_shape_t& s, const ScoreLayout& L, void* ws, int64_t n, float* logits,
+                               hipStream_t st) {
+    const ScoreDims d = score_dims(s);
+    ScoreArgs a = score_args(s, L, ws, n);
+    a.logits = logits;
+    const int grid = cdiv_i((int64_t)a.nub * a.splits, 4);
+    if (d.ks2 == 4 && d.ks3 == 2 && d.nr3 == 8 && d.ksg == 4) launch(k_score_topk<4, 2, 8, 4, true>, grid, kBlock, 0, st, a);
+    else if (d.ks2 == 4 && d.ks3 == 2 && d.nr3 == 8 && d.ksg == 0) launch(k_score_topk<4, 2, 8, 0, true>, grid, kBlock, 0, st, a);
+    else if (d.ks2 == 2 && d.ks3 == 1 && d.nr3 == 4 && d.ksg == 1) launch(k_score_topk<2, 1, 4, 1, true>, grid, kBlock, 0, st, a);
+    else if (d.ks2 == 2 && d.ks3 == 1 && d.nr3 == 4 && d.ksg == 0) launch(k_score_topk<2, 1, 4, 0, true>, grid, kBlock, 0, st, a);
+    else return hipErrorInvalidValue;
+    return hipGetLastError();
+}
+
+hipError_t launch_score_main(const ncf_shape_t& s, const ScoreLayout& L, void* ws, int64_t n, int k,
+                             int32_t* top_items, float* top_scores, hipStream_t st) {
+    const ScoreDims d = score_dims(s);
+    ScoreArgs a = score_args(s, L, ws, n);
+    const int nub = a.nub;
+    a.k = k;
+    a.top_items = top_items;
+    a.top_scores = top_scores;
     const int grid = cdiv_i((int64_t)nub * a.splits, 4);
 #define NCF_SCORE_LAUNCH(A, B, C, D) launch(k_score_topk<A, B, C, D>, grid, kBlock, 0, st, a)
     if (d.ks2 == 4 && d.ks3 == 2 && d.nr3 == 8 && d.ksg == 4) NCF_SCORE_LAUNCH(4, 2, 8, 4);       // ml-20m NeuMF (configs C/E)

@@ -152,6 +152,9 @@ _SIGNATURES = {
     "ncf_score_workspace_size": (ctypes.c_int, [_P(NcfShape), _i64, _P(ctypes.c_size_t)]),
     "ncf_score_topk": (ctypes.c_int, [_P(NcfShape), _P(NcfModel), _vp, _i64, _i32, _i32, _vp, _vp, _vp,
                                       ctypes.c_size_t, _vp]),
+    "ncf_score_logits_workspace_size": (ctypes.c_int, [_P(NcfShape), _i64, _i32, _P(ctypes.c_size_t)]),
+    "ncf_score_logits": (ctypes.c_int, [_P(NcfShape), _P(NcfModel), _vp, _i64, _i32, _vp, _vp, ctypes.c_size_t,
+                                        _vp]),
     "ncf_quantize_blocks": (ctypes.c_int, [_vp, _i32, _i64, _i64, _i64, _i32, _vp, _i64, _vp, _vp]),
     "ncf_matmul_blocks": (ctypes.c_int, [_vp, _i64, _vp, _vp, _i64, _vp, _i32, _vp, _i64, _i64, _i64, _i32, _vp,
                                          _i64, _vp]),
@@ -170,7 +173,7 @@ EXPORTED = sorted(_SIGNATURES)
 K_INDEX, K_FWD_BWD, K_EMB_UPDATE, K_MLP_UPDATE, K_METRICS, K_SCORE, K_SAMPLE, K_CATCHUP = 1, 2, 3, 4, 5, 6, 7, 8
 NCF_F32, NCF_BF16, NCF_F16 = 0, 1, 2
 NCF_DISTILL_MAX_K, NCF_DISTILL_STATE = 1024, 5
-NCF_SCORE_FP16, NCF_SCORE_FP32, NCF_SCORE_MAX_K = 0, 1, 32
+NCF_SCORE_FP16, NCF_SCORE_FP32, NCF_SCORE_FP8, NCF_SCORE_MAX_K = 0, 1, 2, 32
 
 
 def profile_enable(kernels, capacity):

@@ -20,6 +20,7 @@ from . import _native as N
 from .layout import Layout
 
 KERAS_EPSILON = 1e-7
+SAMPLE_LOGITS = 1 << 28   # logits that sample_items holds at a time (1 GiB)
 
 
 def keras_weight_names(layers, gmf_dim):
@@ -424,6 +425,104 @@ class NCFEngine(object):
                                  N.ptr(items), N.ptr(scores), N.ptr(self._score_ws), self._score_ws.numel(),
                                  N.stream_handle(self.device)))
         return items, scores
+
+    # ------------------------------- logits of the catalogue, draws, distillation
+    def score_logits(self, users, precision=None):
+        """The logits of ``users`` for every item, float32 (n, num_items); a user outside the table
+        gives a row of NaN.  precision "fp16" (4-layer models of ``score_topk``'s MFMA scorer), "fp8"
+        (GMF-only models: the product of their factors in 8 bits with block scales,
+        ``catalogue.matmul_blocks``), "fp32" (any shape, slow); None: the first of these that the
+        shape has."""
+        codes = {"fp16": N.NCF_SCORE_FP16, "fp8": N.NCF_SCORE_FP8, "fp32": N.NCF_SCORE_FP32}
+        L = N.lib()
+        if precision is None:
+            precision = next(p for p in codes if L.ncf_score_supported(ctypes.byref(self.shape), codes[p]))
+        prec = codes.get(precision)
+        if prec is None:
+            raise ValueError("precision must be 'fp16', 'fp8', 'fp32' or None, got %r" % (precision,))
+        if not L.ncf_score_supported(ctypes.byref(self.shape), prec):
+            raise ValueError("model shape not supported by the %s scorer" % precision)
+        self.flush()
+        u = self._ids(users)
+        n = u.numel()
+        logits = torch.empty(n, self.num_items, dtype=torch.float32, device=self.device)
+        if n == 0:
+            return logits
+        nbytes = ctypes.c_size_t()
+        N.check(L.ncf_score_logits_workspace_size(ctypes.byref(self.shape), n, prec, ctypes.byref(nbytes)))
+        ws = torch.empty(int(nbytes.value), dtype=torch.uint8, device=self.device)
+        N.check(L.ncf_score_logits(ctypes.byref(self.shape), ctypes.byref(self.model_s), N.ptr(u), n, prec,
+                                   N.ptr(logits), N.ptr(ws), ws.numel(), N.stream_handle(self.device)))
+        return logits
+
+    def sample_items(self, users, u, temperature=1.0, top_k=0, top_p=1.0, min_p=0.0, mask=None, precision=None):
+        """Items drawn for ``users`` from the softmax of their logits over the catalogue, by the uniform
+        numbers ``u`` (n,) or (n, draws) on the device: ``catalogue.sample_items`` on ``score_logits``,
+        for as many users at a time as 1 GiB of logits holds.  Settings as there; one per user as a
+        tensor.  Returns (items int32, probabilities float32) of u's shape."""
+        from . import catalogue
+        ids = self._ids(users)
+        n = ids.numel()
+        if not torch.is_tensor(u) or u.dim() not in (1, 2) or u.shape[0] != n:
+            raise ValueError("u must have shape (%d,) or (%d, draws)" % (n, n))
+        step = max(1, SAMPLE_LOGITS // self.num_items)
+        settings = dict(temperature=temperature, top_k=top_k, top_p=top_p, min_p=min_p)
+        items = torch.empty(u.shape, dtype=torch.int32, device=self.device)
+        probs = torch.empty(u.shape, dtype=torch.float32, device=self.device)
+
+        def part(x, rows):
+            return x[rows] if torch.is_tensor(x) and x.shape and x.shape[0] == n else x
+
+        for i in range(0, n, step):
+            rows = slice(i, min(n, i + step))
+            m = mask if mask is None or mask.dim() == 1 else mask[rows]
+            items[rows], probs[rows] = catalogue.sample_items(
+                self.score_logits(ids[rows], precision), u[rows], mask=m,
+                **{name: part(x, rows) for name, x in settings.items()})
+        return items, probs
+
+    def distill_step(self, users, items, teacher_items, teacher_logits, temperature=1.0, teacher_lse=None, k=1,
+                     weight=1.0):
+        """One training step towards a teacher's ranking of candidate lists.
+
+        ``users`` (b,), ``items`` (b, c): c candidates per user; ``teacher_items`` (b, t) the places in
+        the user's candidates (0 .. c - 1) of the teacher's best, ``teacher_logits`` (b, t) float32,
+        ``teacher_lse`` (b,) its log-sum-exp over all c at this temperature or None
+        (``catalogue.distill_loss``).  The loss is weight * temperature ** 2 times the mean divergence
+        of the student's softmax over its candidates; its gradient with respect to the logits enters
+        ``train_step`` as labels y = p - b c dz, whose cross-entropy has exactly that gradient (zero,
+        as Keras' clip has it, where p is within 1e-7 of 0 or 1).  The optimizer's step, deferred decay
+        and counters are the training step's; ``stats`` are not touched.  Returns the per-user losses
+        (b,) on the device (NaN, and no part in the step, for a user with an id outside the table)."""
+        from . import catalogue
+        if self.precision != "fp32":
+            raise ValueError("distill_step needs precision='fp32': its labels stand for the fp32 forward's p")
+        it = torch.as_tensor(np.asarray(items)) if not torch.is_tensor(items) else items
+        if it.dim() != 2 or it.shape[1] < 1:
+            raise ValueError("items must have shape (users, candidates), got %s" % (tuple(it.shape),))
+        b, c = it.shape
+        self.check_ids(users, items)
+        iv = self._ids(it)
+        ids = self._ids(users)
+        if ids.numel() != b:
+            raise ValueError("%d users for %d lists of candidates" % (ids.numel(), b))
+        if b == 0:
+            return torch.empty(0, dtype=torch.float32, device=self.device)
+        uv = ids.view(b, 1).expand(b, c).reshape(-1)
+        p = self.predict(uv, iv)
+        loss, dz = catalogue.distill_loss_grad(torch.logit(p).view(b, c), teacher_items, teacher_logits,
+                                               grad_loss=weight * temperature ** 2 / b, temperature=temperature,
+                                               teacher_lse=teacher_lse)
+        labels = torch.sub(p, dz.view(-1), alpha=float(b * c))
+        # an id outside the table: its user's whole list has no loss (NaN) and takes no part
+        labels = torch.where(torch.isnan(labels), p, labels)
+        stats = self.stats
+        self.stats = torch.zeros_like(stats)
+        try:
+            self.train_step(uv, iv, labels, group=c, k=min(int(k), c))
+        finally:
+            self.stats = stats
+        return loss
 
     # ------------------------------------------------- data-parallel split
     def alloc_grads(self, rows=None):

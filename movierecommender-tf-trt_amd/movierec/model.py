@@ -459,6 +459,53 @@ class MovierecModel(object):
         items, scores = self.model.engine.score_topk(user_ids, k=k, precision=precision)
         return items.cpu().numpy(), scores.cpu().numpy()
 
+    def recommend_sampled(self, user_ids, draws=1, temperature=1.0, top_k=0, top_p=1.0, min_p=0.0, mask=None,
+                          seed=None, precision=None):
+        """Items drawn at random, in proportion to their softmax over the whole catalogue (new; the
+        exploring counterpart of :meth:`recommend`): per user ``draws`` items from its ``top_k`` best
+        (0: all), of them the shortest leading list with ``top_p`` of the weight
+        exp(logit / temperature), without items of less than ``min_p`` of the best one's weight.
+        ``mask`` (n, num_items) or (num_items,): False items, such as seen ones, are never drawn.  The
+        uniform numbers come from numpy's generator with ``seed``.  Returns numpy ``(items (n, draws)
+        int32, probabilities (n, draws) float32)``; item -1 where the mask leaves nothing."""
+        import torch
+        user_ids = np.asarray(user_ids).reshape(-1)
+        if user_ids.size and (user_ids.min() < 0 or user_ids.max() >= self._num_users):
+            raise ValueError("user id out of range [0, %d)" % self._num_users)
+        if draws < 1:
+            raise ValueError("draws must be >= 1, found {}".format(draws))
+        user_ids = self.model.local_user_ids(user_ids)   # data-parallel: this rank's users
+        eng = self.model.engine
+        u = torch.from_numpy(np.random.default_rng(seed).random((user_ids.size, int(draws)))).to(eng.device)
+        if mask is not None:
+            mask = torch.as_tensor(np.asarray(mask, dtype=bool)).to(eng.device)
+        items, probs = eng.sample_items(user_ids, u, temperature=temperature, top_k=top_k, top_p=top_p, min_p=min_p,
+                                        mask=mask, precision=precision)
+        return items.cpu().numpy(), probs.cpu().numpy()
+
+    def distill_on_batch(self, x, teacher, top=10, temperature=1.0, weight=1.0):
+        """One step towards another model's ranking (new; the counterpart of Keras' train_on_batch with a
+        teacher in the place of labels): ``x`` = [users (b,), items (b, c)], c candidates per user;
+        ``teacher`` a :class:`MovierecModel` over the same ids.  The teacher's ``top`` best candidates
+        and its mass over the rest are the target (``NCFEngine.distill_step``).  Returns the mean
+        divergence before the step."""
+        import torch
+        if self.model.dp is not None or teacher.model.dp is not None:
+            raise ValueError("distill_on_batch runs on one device (world_size 1)")
+        users, items = np.asarray(x[0]).reshape(-1), np.asarray(x[1])
+        if items.ndim != 2 or items.shape[0] != users.size or items.size == 0:
+            raise ValueError("x must be [users (b,), items (b, c)], found {} and {}".format(users.shape, items.shape))
+        if not 0 < temperature < math.inf:
+            raise ValueError("temperature must be positive and finite, found {}".format(temperature))
+        b, c = items.shape
+        for m in (self, teacher):
+            m.model.engine.check_ids(users, items)
+        z = torch.logit(teacher.model.engine.predict(np.repeat(users, c), items.reshape(-1))).view(b, c)
+        best, places = torch.topk(z, min(int(top), c, 1024), dim=1)
+        loss = self.model.engine.distill_step(users, items, places, best.contiguous(), temperature=temperature,
+                                              teacher_lse=torch.logsumexp(z / temperature, 1), weight=weight)
+        return float(loss.mean())
+
 
 def _prefetch(gen, order, depth):
     """Produce ``gen[i]`` for i in order on one background thread (Keras'
