@@ -19,15 +19,18 @@ LIB = os.path.join(OUT_DIR, "libmovierec_ncf.so")
 SOURCES = ["ncf_index.hip", "ncf_update.hip", "ncf_generic.hip", "ncf_fused.hip", "ncf_unit.hip", "ncf_wave.hip", "ncf_layered.hip", "ncf_layer1.hip", "ncf_laymid.hip", "ncf_score.hip", "ncf_sample.hip", "ncf_fp8.hip", "ncf_draw.hip", "ncf_distill.hip", "ncf_comm.hip", "ncf_capi.hip"]
 # per-source extra flags: the scorer keeps its MFMA accumulators in VGPRs (no v_accvgpr_read
 # before every epilogue op; its 226 registers fit the unified file at 2 waves/SIMD), and so does the
-# 8-bit product, whose every accumulator is read once per block of 128
-EXTRA = {"ncf_score.hip": ["-mllvm", "-amdgpu-mfma-vgpr-form"], "ncf_fp8.hip": ["-mllvm", "-amdgpu-mfma-vgpr-form"]}
+# 8-bit product, whose every accumulator is read once per block of 128.  The catalogue operators hold no
+# packed fp32 instruction (v_pk_add/mul/fma_f32), some of whose forms have given wrong results on MI355X.
+# The training kernels are not compiled that way: deferred decay's replays would no longer be bitwise the
+# dense sweep, and config C's step takes 10 % longer (590-604 against 534-540 M samples/s).
+NO_PACKED = ["-Xclang", "-target-feature", "-Xclang", "-packed-fp32-ops"]
+VGPR_MFMA = ["-mllvm", "-amdgpu-mfma-vgpr-form"]
+EXTRA = {"ncf_score.hip": VGPR_MFMA, "ncf_fp8.hip": VGPR_MFMA + NO_PACKED, "ncf_draw.hip": NO_PACKED,
+         "ncf_distill.hip": NO_PACKED}
 HIPCC = os.environ.get("HIPCC", "/opt/rocm/bin/hipcc")
 ARCH = "gfx950"
 CFLAGS = ["--offload-arch=" + ARCH, "-O3", "-fPIC", "-std=c++17", "-I" + INCLUDE, "-I" + HERE,
-          "-Wno-unused-result",
-          # no packed fp32 (v_pk_add/mul/fma_f32): some of their forms have given wrong results on
-          # MI355X; the scalar forms round alike
-          "-Xclang", "-target-feature", "-Xclang", "-packed-fp32-ops"]
+          "-Wno-unused-result"]
 
 
 HASH_MARK = b"NCF_SRC_SHA256="
