@@ -420,20 +420,61 @@ __global__ __launch_bounds__(kTileThreads, 2) void k_mm_tile(MmArgs p) {
             sa[x] = s.sa[wm + 16 * x + i];
             if constexpr (B_TILE) sa[x] *= s.sb[wn];   // (the wave's 128 columns are one tile of b)
         }
+        auto b_frag = [&](int j) { return tile_frag(s.b + at_b + piece, s.b + at_b + (piece ^ 64), 16 * j); };
+        vf32x4 d[kTileMI], sb;
+        auto add = [&](int j) {
 #pragma unroll
-        for (int j = 0; j < kTileNI; ++j) {
-            Operand<WIDE> fb;
-            fb.set(tile_frag(s.b + at_b + piece, s.b + at_b + (piece ^ 64), 16 * j));
-            vf32x4 sb;
-            if constexpr (!B_TILE) sb = *reinterpret_cast<const vf32x4*>(&s.sb[wn + 16 * j + 4 * g]);
-#pragma unroll
-            for (int x = 0; x < kTileMI; ++x) {
-                const vf32x4 d = Operand<WIDE>::product(fb, fa[x]);
+            for (int x = 0; x < kTileMI; ++x)
 #pragma unroll
                 for (int r = 0; r < 4; ++r)
-                    acc[x][j][r] = fmaf(B_TILE ? sa[x] : sa[x] * sb[r], d[r], acc[x][j][r]);
+                    acc[x][j][r] = fmaf(B_TILE ? sa[x] : sa[x] * sb[r], d[x][r], acc[x][j][r]);
+        };
+        auto scales = [&](int j) {
+            if constexpr (!B_TILE) sb = *reinterpret_cast<const vf32x4*>(&s.sb[wn + 16 * j + 4 * g]);
+        };
+        if constexpr (WIDE) {   // (widened fragments leave no registers for more than one column tile)
+#pragma unroll
+            for (int j = 0; j < kTileNI; ++j) {
+                Operand<WIDE> fb;
+                fb.set(b_frag(j));
+                vf32x4 t = {0.0f, 0.0f, 0.0f, 0.0f};
+                if constexpr (!B_TILE) t = *reinterpret_cast<const vf32x4*>(&s.sb[wn + 16 * j + 4 * g]);
+#pragma unroll
+                for (int x = 0; x < kTileMI; ++x) {
+                    const vf32x4 e = Operand<WIDE>::product(fb, fa[x]);
+#pragma unroll
+                    for (int r = 0; r < 4; ++r)
+                        acc[x][j][r] = fmaf(B_TILE ? sa[x] : sa[x] * t[r], e[r], acc[x][j][r]);
+                }
+                __builtin_amdgcn_sched_barrier(0);
             }
-            __builtin_amdgcn_sched_barrier(0);
+        } else {
+            // A column tile's products are scaled and added while the next one's are formed (an MFMA takes 32
+            // cycles, the instructions of one product 16 or 32), and the one after that is read.
+            mi32x8 ahead = b_frag(0);
+#pragma unroll
+            for (int j = 0; j < kTileNI; ++j) {
+                Operand<WIDE> fb;
+                fb.set(ahead);
+                if (j + 1 < kTileNI) ahead = b_frag(j + 1);
+                vf32x4 e[kTileMI];
+#pragma unroll
+                for (int x = 0; x < kTileMI; ++x) e[x] = Operand<WIDE>::product(fb, fa[x]);
+                if (j > 0) {
+                    add(j - 1);
+                    __builtin_amdgcn_sched_group_barrier(0x100, 2, 0);
+#pragma unroll
+                    for (int x = 0; x < kTileMI; ++x) {
+                        __builtin_amdgcn_sched_group_barrier(0x8, 1, 0);
+                        __builtin_amdgcn_sched_group_barrier(0x2, B_TILE ? 4 : 8, 0);
+                    }
+                }
+#pragma unroll
+                for (int x = 0; x < kTileMI; ++x) d[x] = e[x];
+                scales(j);
+                __builtin_amdgcn_sched_barrier(0);
+            }
+            add(kTileNI - 1);
         }
         // (also after the last step, where nobody reads it: a branch here would draw the sums behind it and
         // hold all 32 products in registers)
