@@ -586,8 +586,8 @@ int ncf_draw_items(const ncf_draw_t* draw, void* stream);
  * whose logits are all -inf, has loss and gradient 0.
  *   ncf_distill_loss       writes loss and state (double[rows][NCF_DISTILL_STATE])
  *   ncf_distill_grad       writes grad from the state of the same inputs (no workspace)
- *   ncf_distill_loss_grad  both
- * ws: ncf_distill_workspace_size bytes; nothing persists in it between calls. */
+ *   ncf_distill_loss_grad  both (state may be NULL)
+ * ws: ncf_distill_workspace_size bytes, NULL where that is 0; nothing persists in it between calls. */
 #define NCF_DISTILL_MAX_K 1024
 #define NCF_DISTILL_STATE 5
 typedef struct ncf_distill {

@@ -1583,14 +1583,14 @@ static int distill(const ncf_distill_t* d, void* ws, size_t ws_bytes, bool forwa
         return fail(NCF_EINVAL, "k must be in [1, %d], got %lld", NCF_DISTILL_MAX_K, (long long)d->k);
     if (!(d->temperature > 0.0) || std::isinf(d->temperature))
         return fail(NCF_EINVAL, "temperature must be positive and finite, got %g", d->temperature);
-    if (!d->state || (forward && !d->loss)) return fail(NCF_EINVAL, "NULL device pointer");
+    if ((!d->state && forward != backward) || (forward && !d->loss)) return fail(NCF_EINVAL, "NULL device pointer");
     size_t need = 0;
     if (int r = ncf_distill_workspace_size(d->rows, d->v, &need)) return r;
-    if (forward && (!ws || ws_bytes < need))
+    if (forward && need && (!ws || ws_bytes < need))
         return fail(NCF_EINVAL, "workspace of %zu bytes, need %zu", ws ? ws_bytes : (size_t)0, need);
     if (backward)
         if (int r = check_output("grad", d->grad, d->rows, d->v, d->grad_ld)) return r;
-    return hip_check(ncf::launch_distill(*d, ws, forward, backward, (hipStream_t)stream), "ncf_distill");
+    return hip_check(ncf::launch_distill(*d, need ? ws : nullptr, forward, backward, (hipStream_t)stream), "ncf_distill");
 }
 
 int ncf_distill_loss(const ncf_distill_t* d, void* ws, size_t ws_bytes, void* stream) {

@@ -309,12 +309,14 @@ __device__ __forceinline__ void write_row(const DistArgs& a, int64_t row, const 
     double loss = l.q_log_q - (l.q_z - l.q * ((double)st.base * a.inv_t)) + l.q * log(out + in);
     const double q0 = 1.0 - l.q;
     if (a.ref && q0 > 0.0 && !(out <= 0.0)) loss += q0 * (log1p(-l.q) + log1p(in / out));
-    double* to = a.state + row * kState;
-    to[0] = st.base;
-    to[1] = st.inv_sum;
-    to[2] = st.c_in;
-    to[3] = st.c_out;
-    to[4] = st.ref;
+    if (a.state) {
+        double* to = a.state + row * kState;
+        to[0] = st.base;
+        to[1] = st.inv_sum;
+        to[2] = st.c_in;
+        to[3] = st.c_out;
+        to[4] = st.ref;
+    }
     a.loss[row] = st.inv_sum == 0.0 || (l.q == 0.0 && !a.ref) ? 0.0f : (float)loss;
 }
 
@@ -537,13 +539,23 @@ static DistArgs dist_args(const ncf_distill_t& c, void* ws) {
     a.grad = c.grad;
     a.grad_ld = c.grad_ld;
     a.sums = static_cast<double2*>(ws);
-    a.tops = ws ? reinterpret_cast<float*>(a.sums + c.rows * a.chunks) : nullptr;
+    if (ws) {
+        const int64_t n = c.rows * a.chunks;
+        a.tops = reinterpret_cast<float*>(a.sums + n);
+        if (!a.state) a.state = reinterpret_cast<double*>(a.tops + n + (n & 1));
+    }
     return a;
 }
 
+// A row goes to one workgroup where it fits its registers; few rows of more than a chunk each would leave
+// CUs idle, so those go by chunks.
+static bool by_row(int64_t rows, int64_t v) { return v <= kDistChunk || (v <= 512 * 56 && rows >= 128); }
+
+// for the chunks' sums and, behind them, the state where the caller takes none
 size_t distill_workspace(int64_t rows, int v) {
+    if (by_row(rows, v)) return 0;
     const size_t n = (size_t)rows * ((v + kDistChunk - 1) / kDistChunk);
-    return n * (sizeof(double2) + sizeof(float));
+    return n * sizeof(double2) + (n + (n & 1)) * sizeof(float) + (size_t)rows * kState * sizeof(double);
 }
 int64_t distill_blocks(int64_t rows, int v) {
     const int64_t c = (v + kDistChunk - 1) / kDistChunk;
@@ -560,9 +572,7 @@ static void distill_row(const DistArgs& a, bool backward, hipStream_t st) {
 template <typename T>
 static hipError_t distill_t(const DistArgs& a, bool forward, bool backward, hipStream_t st) {
     const unsigned grid = (unsigned)(a.rows * a.chunks);
-    // few rows of more than a chunk each would leave CUs idle: those go by chunks
-    const bool by_row = a.v <= kDistChunk || (a.v <= 512 * 56 && a.rows >= 128);
-    if (forward && by_row) {
+    if (forward && by_row(a.rows, a.v)) {
         if (a.v <= 64 * 8) distill_row<T, 64, 8>(a, backward, st);
         else if (a.v <= 64 * 32) distill_row<T, 64, 32>(a, backward, st);
         else if (a.v <= 256 * 32) distill_row<T, 256, 32>(a, backward, st);

@@ -270,10 +270,9 @@ def distill_loss_grad(logits, teacher_items, teacher_logits, grad_loss=1.0, temp
     d = _distill(logits, teacher_items, teacher_logits, temperature, teacher_lse)
     dev = logits.device
     loss = torch.empty(d.rows, dtype=torch.float32, device=dev)
-    state = torch.empty(d.rows, N.NCF_DISTILL_STATE, dtype=torch.float64, device=dev)
     grad = _distill_outputs(d, logits, grad_loss)
     ws = _workspace(N.lib().ncf_distill_workspace_size, d.rows, d.v, dev)
-    d.loss, d.state = loss.data_ptr(), state.data_ptr()
+    d.loss = loss.data_ptr()
     if d.rows:
         _call(N.lib().ncf_distill_loss_grad, dev, ctypes.byref(d), N.ptr(ws), ws.numel() if ws is not None else 0)
     return loss, grad
