@@ -58,41 +58,61 @@ __device__ __forceinline__ float unukey(uint32_t k) {
     return __uint_as_float((k & 0x80000000u) ? k & 0x7fffffffu : ~k);
 }
 
-// 2^(j / 256) in units of the weights
-constexpr int kPowerBits = 8, kPowers = 1 << kPowerBits;
-
-// w = exp(z), z = (x - m) / t, as an integer in units of 2^-S.  With z = j ln 2 / 256 + r,
-// w = 2^(j / 256) e^r: the powers of two from a table in LDS (their whole part into the exponent), the
-// rest, |r| <= ln 2 / 512, by its Taylor polynomial to the fourth power (the next term is below 2^-54).
-// Adding 2^52 rounds to an integer.  13 instructions of 64 bits; exp() takes about 40.
+// w = exp(z), z = (x - m) / t, as an integer in units of 2^-S.  With z = (j + r) ln 2 / 2^BITS, |r| <= 1 / 2,
+// w = 2^(j / 2^BITS) e^(r ln 2 / 2^BITS): the power of two from a table in LDS (its whole part into the exponent),
+// the rest by its Taylor polynomial, to the third power for a table of 2,048 and to the fourth for one of 256
+// (the next term is below 2^-54 in both).  Adding 1.5 2^52 rounds to j, adding 2^52 to the integer.  About 17
+// instructions; exp() and a conversion take about 50.  A long row's workgroups of 1,024 fill the larger table
+// (weights of 16 rows of 1,000,000: 24 us with 256 powers), a row in registers the smaller.
+template <int BITS>
 struct Weigher {
-    double m, inv_t, unit;
-    float top;
+    static constexpr int kPowers = 1 << BITS;
+    double m, a, unit;     // a = 2^BITS / (t ln 2), finite
     const double* power;   // [kPowers], times unit
 
-    // w 2^S, not rounded
-    __device__ __forceinline__ double real(float x) const {
-        if (x == top) return unit;
-        // (below -60 less than half a unit; fmax also where infinities in both made a NaN)
-        const double z = fmax(((double)x - m) * inv_t, -60.0);
-        const double j = rint(z * (kPowers * 1.4426950408889634074));
-        const double r = fma(j, -0.69314718055994530942 / kPowers, z);
-        double e = fma(r, 1.0 / 24.0, 1.0 / 6.0);
-        e = fma(r, e, 0.5);
+    __device__ __forceinline__ Weigher(float top, double t, double unit, const double* power)
+        // (under an infinite best item every finite one weighs nothing)
+        : m(top < INFINITY ? (double)top : 1e300), a(fmin(1.0 / t, 1e280) * (kPowers * 1.4426950408889634074)),
+          unit(unit), power(power) {}
+
+    // w 2^S = e p
+    __device__ __forceinline__ void factors(float x, double& e, double& p) const {
+        constexpr double kMagic = 0x1.8p52, kStep = 0.69314718055994530942 / kPowers;
+        // (at -60 less than half a unit; a NaN, of an infinite best item in an infinite temperature, becomes 0)
+        const double y = fmax(fmin(((double)x - m) * a, 0.0), -60.0 * kPowers * 1.4426950408889634074);
+        const double j = y + kMagic, r = y - (j - kMagic);
+        e = BITS < 11 ? fma(r, kStep * kStep * kStep * kStep / 24.0, kStep * kStep * kStep / 6.0)
+                      : kStep * kStep * kStep / 6.0;
+        e = fma(r, e, kStep * kStep / 2.0);
+        e = fma(r, e, kStep);
         e = fma(r, e, 1.0);
-        e = fma(r, e, 1.0);
-        const int n = (int)j;
-        const uint64_t p = (uint64_t)__double_as_longlong(power[n & (kPowers - 1)]);
-        return __longlong_as_double((long long)(p + ((uint64_t)(int64_t)(n >> kPowerBits) << 52))) * e;
+        const uint32_t n = (uint32_t)__double_as_longlong(j);
+        p = power[n & (kPowers - 1)];
+        p = __hiloint2double(__double2hiint(p) + (int)((n & ~(uint32_t)(kPowers - 1)) << (20 - BITS)),
+                             __double2loint(p));
     }
-    __device__ __forceinline__ unsigned long long fixed(float x) const { return round(real(x)); }
-    __device__ __forceinline__ static unsigned long long round(double w) {
-        return (unsigned long long)__double_as_longlong(w + 0x1p52) & 0xfffffffffffffull;
+    __device__ __forceinline__ static unsigned long long round(double e, double p) {
+        return (unsigned long long)__double_as_longlong(fma(e, p, 0x1p52)) & 0xfffffffffffffull;
+    }
+    __device__ __forceinline__ unsigned long long fixed(float x) const {
+        double e, p;
+        factors(x, e, p);
+        return round(e, p);
+    }
+    // 0 where the weight does not reach `least`, which is min-p's
+    __device__ __forceinline__ unsigned long long fixed(float x, unsigned long long least) const {
+        const unsigned long long w = fixed(x);
+        return w >= least ? w : 0ull;
+    }
+    __device__ __forceinline__ unsigned long long least(double min_p) const {
+        return min_p > 0.0 ? (unsigned long long)ceil(min_p * unit) : 0ull;
     }
 };
+constexpr int kRowPowers = 8, kLongPowers = 11;   // BITS of a row in registers, and of a long one
 
-__device__ __forceinline__ void fill_powers(double* power, double unit, int threads) {
-    for (int j = threadIdx.x; j < kPowers; j += threads) power[j] = exp2(j * (1.0 / kPowers)) * unit;
+template <int BITS>
+__device__ __forceinline__ void fill_powers(double (&power)[1 << BITS], double unit, int threads) {
+    for (int j = threadIdx.x; j < 1 << BITS; j += threads) power[j] = exp2(j * (1.0 / (1 << BITS))) * unit;
 }
 
 // (double)c >= p total, for a positive c: the one comparison that top-p makes
@@ -172,7 +192,7 @@ struct RowShared {
     float wave_top[kWaves], wave_sum[kWaves], wave_n[kWaves];
     unsigned long long seg[NT / 4];         // weights ahead of each segment of the row: a wave's vector j
     uint32_t seg_ties[NT / 4];              // equals of the bound ahead of it
-    double power[kPowers];
+    double power[1 << kRowPowers];
 };
 
 // exclusive sums over the workgroup, the total to *sum
@@ -274,6 +294,11 @@ struct Digits {
     __device__ static uint32_t mask(int level) {
         return (1u << (level == kLevels - 1 ? 32 - kBits * (kLevels - 1) : kBits)) - 1u;
     }
+    // 16-bit logits have bits only in the first 19 of the float, and so of the key: the rest are the sign's
+    template <typename T> static constexpr int levels() { return sizeof(T) == 2 ? (19 + kBits - 1) / kBits : kLevels; }
+    __device__ static uint32_t filled(uint32_t prefix, int levels) {
+        return (prefix & 0x80000000u) || levels == kLevels ? prefix : prefix | ((1u << shift(levels - 1)) - 1u);
+    }
     __device__ static bool same(uint32_t a, uint32_t b, int level) {
         return level == 0 || (a >> shift(level - 1)) == (b >> shift(level - 1));
     }
@@ -307,11 +332,12 @@ __device__ __forceinline__ bool count_bin(uint32_t k, const Bins& bins, RowShare
 }
 
 // The k-th best of the items that each() gives, digit by digit of the key.
-template <int NT, typename Each>
+template <typename T, int NT, typename Each>
 __device__ __forceinline__ Cut digits_count(uint32_t left, RowShared<NT>& s, Each each) {
     const int tid = threadIdx.x;
     uint32_t prefix = 0, equal = 0;
-    for (int level = 0; level < Digits<NT>::kLevels; ++level) {
+    constexpr int kLevels = Digits<NT>::template levels<T>();
+    for (int level = 0; level < kLevels; ++level) {
         __syncthreads();
         s.count[2 * tid] = s.count[2 * tid + 1] = 0;
         __syncthreads();
@@ -330,18 +356,19 @@ __device__ __forceinline__ Cut digits_count(uint32_t left, RowShared<NT>& s, Eac
         left -= (uint32_t)s.pick;
         equal = s.count[s.pick_bin];
     }
-    return Cut{unukey(prefix), left, equal > left, equal};
+    return Cut{unukey(Digits<NT>::filled(prefix, kLevels)), left, equal > left, equal};
 }
 
 // The item of those that each() gives at which the weight, from `ahead` on, reaches p of `all`; `over` is
 // what those equals of was.bound weigh that are beyond its ties and among these items.
-template <int NT, typename Each>
+template <typename T, int NT, typename W, typename Each>
 __device__ __forceinline__ Cut digits_weight(double p, double all, unsigned long long ahead, Cut was,
-                                             unsigned long long over, const Weigher& wt, RowShared<NT>& s, Each each) {
+                                             unsigned long long over, const W& wt, RowShared<NT>& s, Each each) {
     const int tid = threadIdx.x;
     uint32_t prefix = 0;
     const uint32_t bound_key = ukey(was.bound + 0.0f);
-    for (int level = 0; level < Digits<NT>::kLevels; ++level) {
+    constexpr int kLevels = Digits<NT>::template levels<T>();
+    for (int level = 0; level < kLevels; ++level) {
         __syncthreads();
         s.weight[2 * tid] = s.weight[2 * tid + 1] = 0;
         __syncthreads();
@@ -363,7 +390,7 @@ __device__ __forceinline__ Cut digits_weight(double p, double all, unsigned long
         prefix |= (mask - s.pick_bin) << Digits<NT>::shift(level);
         ahead = s.pick;
     }
-    const float bound = unukey(prefix);
+    const float bound = unukey(Digits<NT>::filled(prefix, kLevels));
     uint32_t equal = 0;
     each([&](float x, uint32_t) { equal += x == bound; });
     before32(equal, s, &equal);
@@ -378,7 +405,7 @@ __device__ __forceinline__ Cut digits_weight(double p, double all, unsigned long
 }
 
 // Its bound.
-template <int NT, typename Each>
+template <typename T, int NT, typename Each>
 __device__ __forceinline__ Cut cut_count(uint32_t k, const CountBin& in, const Bins& bins, RowShared<NT>& s,
                                          Each each) {
     const int tid = threadIdx.x;
@@ -411,12 +438,12 @@ __device__ __forceinline__ Cut cut_count(uint32_t k, const CountBin& in, const B
         __syncthreads();
         return Cut{s.bound, s.ties, s.equal > s.ties, s.equal};
     }
-    return digits_count(k, s, each);
+    return digits_count<T>(k, s, each);
 }
 
 // The shortest leading list with at least p of the weight, inside what `was` keeps.
-template <int NT, typename Each>
-__device__ __forceinline__ Cut cut_weight(double p, Cut was, const Bins& bins, const Weigher& wt, RowShared<NT>& s,
+template <typename T, int NT, typename W, typename Each>
+__device__ __forceinline__ Cut cut_weight(double p, Cut was, const Bins& bins, const W& wt, RowShared<NT>& s,
                                           Each each) {
     const int tid = threadIdx.x;
     // equals of the bound beyond its ties: counted with the others, then taken off
@@ -481,7 +508,7 @@ __device__ __forceinline__ Cut cut_weight(double p, Cut was, const Bins& bins, c
         __syncthreads();
         return Cut{s.bound, s.ties, s.equal > s.ties, s.equal};
     }
-    return digits_weight(p, all, 0ull, was, over, wt, s, each);
+    return digits_weight<T>(p, all, 0ull, was, over, wt, s, each);
 }
 
 struct RowSettings {
@@ -561,7 +588,7 @@ __global__ __launch_bounds__(NT) void k_draw_row(DrawArgs a) {
             for (int e = 0; e < V; ++e) x[V * j + e] = -INFINITY;
         }
     }
-    fill_powers(s.power, a.unit, NT);
+    fill_powers<kRowPowers>(s.power, a.unit, NT);
 
     // the best item, and the mean of the first logits of every thread for the bins' range
     float top = -INFINITY, sum = 0.0f, num = 0.0f;
@@ -602,8 +629,8 @@ __global__ __launch_bounds__(NT) void k_draw_row(DrawArgs a) {
         }
         return;
     }
-    const Weigher wt{(double)top, 1.0 / set.t, a.unit, top, s.power};
-    const double min_w = set.min_p * a.unit;
+    const Weigher<kRowPowers> wt(top, set.t, a.unit, s.power);
+    const unsigned long long least = wt.least(set.min_p);
     // twice the way from the best to the mean holds what top-k and top-p cut between
     const float range = 2.0f * (top - sum / num);
     const Bins bins = make_bins(top, range, 2 * NT);
@@ -670,7 +697,7 @@ __global__ __launch_bounds__(NT) void k_draw_row(DrawArgs a) {
         if (count_bin(set.k, bins, s, each, &cb)) {
             limit = bins.below(cb.bin);
             if (cb.above + cb.in <= (uint32_t)kList) count = count_from(limit);
-            if (count > (uint32_t)kList) cut = cut_count(set.k, cb, bins, s, each);
+            if (count > (uint32_t)kList) cut = cut_count<T>(set.k, cb, bins, s, each);
         }
     }
     if (count <= (uint32_t)kList) {
@@ -711,8 +738,8 @@ __global__ __launch_bounds__(NT) void k_draw_row(DrawArgs a) {
         Cut in = keep_all();
         CountBin cb;
         if (top_k && count > set.k && count_bin(set.k, fine, s, each_listed, &cb))
-            in = cut_count(set.k, cb, fine, s, each_listed);
-        if (!set.all_p) in = cut_weight(set.p, in, fine, wt, s, each_listed);
+            in = cut_count<T>(set.k, cb, fine, s, each_listed);
+        if (!set.all_p) in = cut_weight<T>(set.p, in, fine, wt, s, each_listed);
         __syncthreads();
         // weights in the order of the ids, which is the list's
         uint32_t seen = 0;
@@ -726,8 +753,7 @@ __global__ __launch_bounds__(NT) void k_draw_row(DrawArgs a) {
 #pragma unroll
         for (int e = 0; e < P; ++e) {
             const bool out = y[e] < in.bound || (in.partial && y[e] == in.bound && seen++ >= in.ties);
-            const double real = wt.real(y[e]);
-            w[e] = !out && (real >= min_w || !(min_w > 0.0)) ? Weigher::round(real) : 0ull;
+            w[e] = out ? 0ull : wt.fixed(y[e], least);
             mine += w[e];
         }
         unsigned long long c = before64(mine, s, &total);
@@ -752,7 +778,7 @@ __global__ __launch_bounds__(NT) void k_draw_row(DrawArgs a) {
     }
 
     // ---- from the registers
-    if (!set.all_p) cut = cut_weight(set.p, cut, bins, wt, s, each);
+    if (!set.all_p) cut = cut_weight<T>(set.p, cut, bins, wt, s, each);
     // equals of the bound ahead of the lane's first of V neighbours
     auto ties_before = [&](const float* y, uint32_t ahead) {
 #pragma unroll
@@ -781,8 +807,7 @@ __global__ __launch_bounds__(NT) void k_draw_row(DrawArgs a) {
     auto weigh = [&](float y, uint32_t& seen) -> unsigned long long {
         if (y < cut.bound) return 0;   // (-inf too)
         if (cut.partial && y == cut.bound && seen++ >= cut.ties) return 0;
-        const double real = wt.real(y);
-        return real >= min_w || !(min_w > 0.0) ? Weigher::round(real) : 0ull;
+        return wt.fixed(y, least);
     };
 #pragma unroll
     for (int j = 0; j < J; ++j) {
@@ -847,7 +872,7 @@ __global__ __launch_bounds__(NT) void k_draw_row(DrawArgs a) {
 // again instead); the weight of every segment of 64 vectors; the draws.  The row comes from memory once
 // and from the caches after that (1,000,000 items are 2 or 4 MB).
 
-constexpr int kLongThreads = 256;
+constexpr int kLongThreads = 1024;
 constexpr int kLongWaves = kLongThreads / 64;
 constexpr int kLongBins = 2048;
 constexpr int kResolveThreads = 512;
@@ -911,12 +936,14 @@ struct LongShared {
     union {
         uint32_t count[kLongBins];
         unsigned long long weight[kLongBins];
+        uint2 staged[kLongBins];
     };
-    double power[kPowers];
+    double power[1 << kLongPowers];
     unsigned long long wave64[kLongWaves], pick;
     uint32_t wave32[kLongWaves];
     float wavef[3][kLongWaves];
     int pick_bin;
+    uint32_t items;
 };
 
 template <typename T>
@@ -987,9 +1014,9 @@ __device__ __forceinline__ Bins long_bins(const LongArgs& l, int64_t r) {
     }
     return make_bins(top, 2.0f * (top - sum / num), kLongBins);
 }
-__device__ __forceinline__ Weigher long_weigher(const LongArgs& l, const Bins& bins, const RowSettings& set,
+__device__ __forceinline__ Weigher<kLongPowers> long_weigher(const LongArgs& l, const Bins& bins, const RowSettings& set,
                                                 const double* power) {
-    return Weigher{(double)bins.top, 1.0 / set.t, l.a.unit, bins.top, power};
+    return Weigher<kLongPowers>(bins.top, set.t, l.a.unit, power);
 }
 __device__ __forceinline__ Cut row_cut(const LongRow& w) { return Cut{w.bound, w.ties, w.partial != 0, w.equal}; }
 __device__ __forceinline__ bool wants_cut(const LongArgs& l, const RowSettings& set, bool weights) {
@@ -1009,15 +1036,19 @@ __global__ __launch_bounds__(kLongThreads) void k_long_histogram(LongArgs l) {
         if constexpr (WEIGHTS) s.weight[b] = 0;
         else s.count[b] = 0;
     }
-    fill_powers(s.power, l.a.unit, kLongThreads);
+    fill_powers<kLongPowers>(s.power, l.a.unit, kLongThreads);
     __syncthreads();
-    const Weigher wt = long_weigher(l, bins, set, s.power);
+    const Weigher<kLongPowers> wt = long_weigher(l, bins, set, s.power);
     const float bound = l.row[r].bound;
     each_vector<T>(l, r, part, [&](const float* y, int) {
+        constexpr int V = Elem<T>::kVec;
+        unsigned long long w[V];
 #pragma unroll
-        for (int e = 0; e < Elem<T>::kVec; ++e) {
+        for (int e = 0; e < V; ++e) w[e] = WEIGHTS ? wt.fixed(y[e]) : 1ull;
+#pragma unroll
+        for (int e = 0; e < V; ++e) {
             if (!(y[e] >= bound)) continue;   // (-inf too)
-            if constexpr (WEIGHTS) atomicAdd(&s.weight[bins.of(y[e])], wt.fixed(y[e]));
+            if constexpr (WEIGHTS) atomicAdd(&s.weight[bins.of(y[e])], w[e]);
             else atomicAdd(&s.count[bins.of(y[e])], 1u);
         }
     });
@@ -1060,10 +1091,13 @@ __global__ __launch_bounds__(kLongThreads) void k_long_gather(LongArgs l) {
     if (!wants_cut(l, set, WEIGHTS)) return;
     const Bins bins = long_bins(l, r);
     if (!(bins.top > -INFINITY)) return;
-    fill_powers(s.power, l.a.unit, kLongThreads);
-    if (tid == 0) s.pick_bin = -1;
-    __syncthreads();
     const Cut was = row_cut(l.row[r]);
+    if (WEIGHTS && was.partial) fill_powers<kLongPowers>(s.power, l.a.unit, kLongThreads);
+    if (tid == 0) {
+        s.pick_bin = -1;
+        s.items = 0;
+    }
+    __syncthreads();
     unsigned long long c[kPer], mine = 0, total;
 #pragma unroll
     for (int b = 0; b < kPer; ++b) {
@@ -1071,7 +1105,7 @@ __global__ __launch_bounds__(kLongThreads) void k_long_gather(LongArgs l) {
         c[b] = WEIGHTS ? l.weight[at] : (unsigned long long)l.count[at];
     }
     if (WEIGHTS && was.partial) {   // equals of top-k's bound beyond its ties
-        const Weigher wt = long_weigher(l, bins, set, s.power);
+        const Weigher<kLongPowers> wt = long_weigher(l, bins, set, s.power);
         const int at = bins.of(was.bound);
 #pragma unroll
         for (int b = 0; b < kPer; ++b)
@@ -1103,27 +1137,36 @@ __global__ __launch_bounds__(kLongThreads) void k_long_gather(LongArgs l) {
         l.row[r].total_w = total;
     }
     if (bin < 0) return;
-    // counted, a place in the row's list reserved for all of them at once, then stored (with an atomic for
-    // each wave's items this kernel took 57 us, so 20: they all meet at one address; 16 rows of 1,000,000)
-        uint32_t items = 0;
-    each_vector<T>(l, r, part, [&](const float* y, int) {
-#pragma unroll
-        for (int e = 0; e < Elem<T>::kVec; ++e) items += y[e] >= was.bound && bins.of(y[e]) == bin;
-    });
-    unsigned long long part_items;
-    const uint32_t ahead_items = (uint32_t)long_before(items, s, &part_items);
-    if (part_items == 0) return;
-    __syncthreads();
-    if (tid == 0) s.wave32[0] = atomicAdd(&l.row[r].members, (uint32_t)part_items);
-    __syncthreads();
-    uint32_t at = s.wave32[0] + ahead_items;
-    if (items == 0) return;
+    // to LDS first: one place in the row's list for all of them (with an atomic on it for each wave's items this
+    // kernel took 57 us, counted in a pass of its own 20; 16 rows of 1,000,000)
     each_vector<T>(l, r, part, [&](const float* y, int id) {
 #pragma unroll
         for (int e = 0; e < Elem<T>::kVec; ++e)
             if (y[e] >= was.bound && bins.of(y[e]) == bin) {
+                const uint32_t at = atomicAdd(&s.items, 1u);
+                if (at < kLongBins) s.staged[at] = make_uint2(__float_as_uint(y[e]), (uint32_t)(id + e));
+            }
+    });
+    __syncthreads();
+    const uint32_t items = s.items;
+    if (items == 0) return;
+    if (tid == 0) s.wave32[0] = atomicAdd(&l.row[r].members, items);
+    __syncthreads();
+    const uint32_t first = s.wave32[0];
+    if (first >= l.cap) return;   // (the list is not used then)
+    if (items <= (uint32_t)kLongBins) {
+        for (uint32_t at = tid; at < items; at += kLongThreads)
+            if (first + at < l.cap) l.list[r * l.cap + first + at] = s.staged[at];
+        return;
+    }
+    if (tid == 0) s.items = 0;
+    __syncthreads();
+    each_vector<T>(l, r, part, [&](const float* y, int id) {
+#pragma unroll
+        for (int e = 0; e < Elem<T>::kVec; ++e)
+            if (y[e] >= was.bound && bins.of(y[e]) == bin) {
+                const uint32_t at = first + atomicAdd(&s.items, 1u);
                 if (at < l.cap) l.list[r * l.cap + at] = make_uint2(__float_as_uint(y[e]), (uint32_t)(id + e));
-                ++at;
             }
     });
 }
@@ -1132,6 +1175,7 @@ __global__ __launch_bounds__(kLongThreads) void k_long_gather(LongArgs l) {
 template <typename T, bool WEIGHTS>
 __global__ __launch_bounds__(kResolveThreads) void k_long_resolve(LongArgs l) {
     __shared__ RowShared<kResolveThreads> s;
+    __shared__ double power[1 << kLongPowers];
     const int64_t r = blockIdx.x;
     const int tid = threadIdx.x;
     const RowSettings set = row_settings(l.a, r);
@@ -1139,18 +1183,18 @@ __global__ __launch_bounds__(kResolveThreads) void k_long_resolve(LongArgs l) {
     const LongRow w = l.row[r];
     const Bins bins = long_bins(l, r);
     if (!(bins.top > -INFINITY) || w.bin < 0) return;
-    fill_powers(s.power, l.a.unit, kResolveThreads);
+    fill_powers<kLongPowers>(power, l.a.unit, kResolveThreads);
     __syncthreads();
     const Cut was = row_cut(w);
-    const Weigher wt = long_weigher(l, bins, set, s.power);
+    const Weigher<kLongPowers> wt = long_weigher(l, bins, set, power);
     const unsigned long long over =
         WEIGHTS && was.partial && bins.of(was.bound) == w.bin
             ? (unsigned long long)(was.equal - was.ties) * wt.fixed(was.bound) : 0ull;
     auto bound_of = [&](auto each) {
         if constexpr (WEIGHTS)
-            return digits_weight(set.p, (double)w.total_w, w.above_w, was, over, wt, s, each);
+            return digits_weight<T>(set.p, (double)w.total_w, w.above_w, was, over, wt, s, each);
         else
-            return digits_count(set.k - w.above_n, s, each);
+            return digits_count<T>(set.k - w.above_n, s, each);
     };
     Cut cut;
     if (w.members <= l.cap) {
@@ -1187,78 +1231,49 @@ __global__ __launch_bounds__(kResolveThreads) void k_long_resolve(LongArgs l) {
 // weights of V neighbours, of which `seen` equals of the bound lie ahead
 template <int V>
 __device__ __forceinline__ unsigned long long weigh_vector(const float* y, uint32_t seen, const Cut& cut,
-                                                           const Weigher& wt, double min_w, unsigned long long* w) {
+                                                           const Weigher<kLongPowers>& wt, unsigned long long least,
+                                                           unsigned long long* w) {
     unsigned long long sum = 0;
 #pragma unroll
     for (int e = 0; e < V; ++e) {
         w[e] = 0;
-        if (y[e] >= cut.bound && !(cut.partial && y[e] == cut.bound && seen++ >= cut.ties)) {
-            const double real = wt.real(y[e]);
-            if (real >= min_w || !(min_w > 0.0)) w[e] = Weigher::round(real);
-        }
+        if (y[e] >= cut.bound && !(cut.partial && y[e] == cut.bound && seen++ >= cut.ties)) w[e] = wt.fixed(y[e], least);
         sum += w[e];
     }
     return sum;
 }
 
-// Equals of a partial bound in every segment.
-template <typename T>
-__global__ __launch_bounds__(kLongThreads) void k_long_ties(LongArgs l) {
-    const int64_t r = blockIdx.x / l.parts;
-    const int part = (int)(blockIdx.x - r * l.parts);
-    const Cut cut = row_cut(l.row[r]);
-    if (!cut.partial) return;
-    each_vector<T>(l, r, part, [&](const float* y, int id) {
-        int n = 0;
-#pragma unroll
-        for (int e = 0; e < Elem<T>::kVec; ++e) n += lane_count(__ballot(y[e] == cut.bound));
-        if ((threadIdx.x & 63) == 0) l.seg_ties[r * l.segs + id / seg_items<T>()] = (uint32_t)n;
-    });
-}
-
-// equals of the bound in the segments before `to`, for threads i, i + n, .. of those who ask
-__device__ __forceinline__ uint32_t ties_ahead(const LongArgs& l, int64_t r, int to, int i, int n) {
-    uint32_t sum = 0;
-#pragma unroll 8
-    for (int g = i; g < to; g += n) sum += l.seg_ties[r * l.segs + g];
-    return lane63(lane_sums32(sum));   // of this wave
-}
-
-// The weight of every segment.
+// The weight of every segment; under a partial bound that of what lies above it, and the number of its equals.
 template <typename T>
 __global__ __launch_bounds__(kLongThreads) void k_long_weigh(LongArgs l) {
-    __shared__ double power[kPowers];
+    __shared__ double power[1 << kLongPowers];
     constexpr int V = Elem<T>::kVec;
     const int64_t r = blockIdx.x / l.parts;
     const int part = (int)(blockIdx.x - r * l.parts), lane = threadIdx.x & 63;
     const RowSettings set = row_settings(l.a, r);
     const Bins bins = long_bins(l, r);
     if (!(bins.top > -INFINITY)) return;
-    fill_powers(power, l.a.unit, kLongThreads);
+    fill_powers<kLongPowers>(power, l.a.unit, kLongThreads);
     __syncthreads();
-    const Weigher wt = long_weigher(l, bins, set, power);
-    const double min_w = set.min_p * l.a.unit;
+    const Weigher<kLongPowers> wt = long_weigher(l, bins, set, power);
+    const unsigned long long least = wt.least(set.min_p);
     const Cut cut = row_cut(l.row[r]);
-    uint32_t ahead = 0;   // equals of the bound before this wave's next segment
-    if (cut.partial) {
-        int s0, s1;
-        wave_segments<T>(l, part, &s0, &s1);
-        ahead = ties_ahead(l, r, s0, lane, 64);
-    }
     each_vector<T>(l, r, part, [&](const float* y, int id) {
-        const int g = id / seg_items<T>();
-        uint32_t seen = ahead;
-        if (cut.partial) {
+        const int64_t g = r * l.segs + id / seg_items<T>();
+        unsigned long long sum = 0;
 #pragma unroll
-            for (int e = 0; e < V; ++e) {
-                const uint64_t m = __ballot(y[e] == cut.bound);
-                seen = lanes_before(m, seen);
-                ahead += (uint32_t)lane_count(m);
-            }
+        for (int e = 0; e < V; ++e) {   // (of all, without a branch: the chains of a vector side by side)
+            const unsigned long long w = wt.fixed(y[e], least);
+            sum += y[e] > cut.bound || (!cut.partial && y[e] == cut.bound) ? w : 0ull;
         }
-        unsigned long long w[V];
-        const unsigned long long sum = lane_sums64(weigh_vector<V>(y, seen, cut, wt, min_w, w));
-        if (lane == 63) l.seg[r * l.segs + g] = sum;
+        sum = lane_sums64(sum);
+        if (lane == 63) l.seg[g] = sum;
+        if (cut.partial) {
+            int n = 0;
+#pragma unroll
+            for (int e = 0; e < V; ++e) n += lane_count(__ballot(y[e] == cut.bound));
+            if (lane == 0) l.seg_ties[g] = (uint32_t)n;
+        }
     });
 }
 
@@ -1278,46 +1293,65 @@ __global__ __launch_bounds__(kLongThreads) void k_long_draw(LongArgs l) {
         }
         return;
     }
-    fill_powers(s.power, l.a.unit, kLongThreads);
+    fill_powers<kLongPowers>(s.power, l.a.unit, kLongThreads);
+    const Weigher<kLongPowers> wt = long_weigher(l, bins, set, s.power);
+    const Cut cut = row_cut(l.row[r]);
+    const unsigned long long least = wt.least(set.min_p);
     // a thread's share of the segments
     const int per = (l.segs + kLongThreads - 1) / kLongThreads;
     const int g0 = min(tid * per, l.segs), g1 = min(g0 + per, l.segs);
     const unsigned long long* seg = l.seg + r * l.segs;
+    const uint32_t* equals = l.seg_ties + r * l.segs;
+    uint32_t ties = 0;          // equals of a partial bound ahead of the share
+    unsigned long long tie_w = 0;
+    if (cut.partial) {
+        for (int g = g0; g < g1; ++g) ties += equals[g];
+        unsigned long long all;
+        ties = (uint32_t)long_before(ties, s, &all);   // (and the powers)
+        tie_w = wt.fixed(cut.bound, least);
+    }
+    // a segment's weight, `ahead` equals of the bound before it
+    auto weight = [&](int g, uint32_t ahead) {
+        unsigned long long w = seg[g];
+        if (cut.partial && ahead < cut.ties) w += tie_w * min(equals[g], cut.ties - ahead);
+        return w;
+    };
     unsigned long long mine = 0, total;
-    for (int g = g0; g < g1; ++g) mine += seg[g];
+    {
+        uint32_t ahead = ties;
+        for (int g = g0; g < g1; ++g) {
+            mine += weight(g, ahead);
+            if (cut.partial) ahead += equals[g];
+        }
+    }
     unsigned long long c = long_before(mine, s, &total);
     const unsigned long long target = draw_target(l.a, o, total);
     if (c <= target && target < c + mine) {
         for (int g = g0; g < g1; ++g) {
-            if (target < c + seg[g]) {
+            const unsigned long long w = weight(g, ties);
+            if (target < c + w) {
                 s.pick_bin = g;
                 s.pick = c;
+                s.items = ties;
                 break;
             }
-            c += seg[g];
+            c += w;
+            if (cut.partial) ties += equals[g];
         }
     }
     __syncthreads();
-    const int g = s.pick_bin, at = g * seg_items<T>() + lane * V;
-    const Weigher wt = long_weigher(l, bins, set, s.power);
-    const Cut cut = row_cut(l.row[r]);
-    if (cut.partial) {
-        const uint32_t n = ties_ahead(l, r, g, tid, kLongThreads);
-        if (lane == 0) s.wave32[tid >> 6] = n;
-        __syncthreads();
-    }
     if (tid >= 64) return;
+    const int g = s.pick_bin, at = g * seg_items<T>() + lane * V;
     float y[V];
     load_logits<T>(l.a, r, at, y);
     uint32_t seen = 0;
     if (cut.partial) {
-#pragma unroll
-        for (int w = 0; w < kLongWaves; ++w) seen += s.wave32[w];
+        seen = s.items;
 #pragma unroll
         for (int e = 0; e < V; ++e) seen = lanes_before(__ballot(y[e] == cut.bound), seen);
     }
     unsigned long long w[V];
-    const unsigned long long sum = weigh_vector<V>(y, seen, cut, wt, set.min_p * l.a.unit, w);
+    const unsigned long long sum = weigh_vector<V>(y, seen, cut, wt, least, w);
     c = s.pick + lane_sums64(sum) - sum;
     if (c <= target && target < c + sum) {
         bool open = true;
@@ -1342,8 +1376,8 @@ static LongLayout long_layout(int64_t rows, int64_t n, int vec) {
     LongLayout l{};
     const int64_t seg = 64 * vec;
     l.segs = (n + seg - 1) / seg;
-    // about 1024 workgroups, four a CU, of at least four segments for each of their waves
-    l.parts = 1024 / rows;
+    // about 4,096 waves, four a SIMD, of at least four segments each
+    l.parts = 4096 / kLongWaves / rows;
     const int64_t most = (l.segs + 4 * kLongWaves - 1) / (4 * kLongWaves);
     l.parts = l.parts < 1 ? 1 : l.parts > most ? most : l.parts;
     // lists of 64 MB together: 2,048 items at least, 65,536 at most
@@ -1406,7 +1440,6 @@ static void draw_long(const DrawArgs& a, void* ws, bool may_k, bool may_p, hipSt
         launch(k_long_gather<T, true>, grid, kLongThreads, 0, st, l);
         launch(k_long_resolve<T, true>, rows, kResolveThreads, 0, st, l);
     }
-    if (may_k || may_p) launch(k_long_ties<T>, grid, kLongThreads, 0, st, l);
     launch(k_long_weigh<T>, grid, kLongThreads, 0, st, l);
     launch(k_long_draw<T>, dim3((unsigned)(a.rows * a.draws)), kLongThreads, 0, st, l);
 }
