@@ -622,15 +622,21 @@ __global__ __launch_bounds__(kBlock, 4) void k_mm_short(MmArgs p, int cols, int 
     constexpr int NX = kShortRows / 16, NJ = 2, Step = 16 * NJ;   // columns of a step: a line takes C / Step
     constexpr int kPitch = 2 * kLine + 16;
     __shared__ __attribute__((aligned(16))) uint8_t rings[kShortWaves][kShortRows * kPitch];
-    __shared__ __attribute__((aligned(16))) float col_scale[kShortCols], col_bias[kShortCols];
+    __shared__ __attribute__((aligned(16))) float col_scale[kShortCols + C], col_bias[kShortCols + C];
     const int lane = threadIdx.x & 63, g = lane >> 4, i = lane & 15;
     const int wave = __builtin_amdgcn_readfirstlane((int)(threadIdx.x >> 6));
     const uint32_t mt = (uint32_t)p.mt;
     const int64_t m0 = ((int64_t)(blockIdx.x % mt) * kShortWaves + wave) * kShortRows;
-    const int64_t c0 = (int64_t)(blockIdx.x / mt) * cols;
-    const int width = (int)min((int64_t)cols, p.n - c0);   // columns of this workgroup, from c0 on
-    for (int c = threadIdx.x; c < cols; c += kBlock) {
-        const int64_t n = c0 + min(c, width - 1);
+    const int64_t part = blockIdx.x / mt;
+    const bool last = (part + 1) * cols >= p.n;
+    // Columns of this workgroup, from c0 on.  Where rows do not start on a line it writes the lines that start
+    // up to C columns ahead of its own part, and forms those columns too: only a row's ends are written in
+    // parts of lines (8,192 x 27,278 fp32: a part's ends written so by both its sides took 215 us).
+    const int lead = unit < kLine && part > 0 ? C : 0;
+    const int64_t c0 = part * cols - lead;
+    const int width = (int)min((int64_t)cols + lead, p.n - c0);
+    for (int c = threadIdx.x; c < width; c += kBlock) {
+        const int64_t n = c0 + c;
         col_scale[c] = p.sb[p.b_tile ? n / kScaleBlock : n];
         col_bias[c] = p.bias ? p.bias[n * p.bias_step] : 0.0f;
     }
@@ -671,9 +677,9 @@ __global__ __launch_bounds__(kBlock, 4) void k_mm_short(MmArgs p, int cols, int 
         for (int j = 0; j < NJ; ++j) raw[j].load(b + (int64_t)min(n + 16 * j + i, width - 1) * p.ldb, g, p.k);
     };
     load_b(0);
-    // after the columns from n on are in the ring the line that starts n - off is whole; a last turn
-    // without columns writes what is left
-    for (int n = 0; n < width + C; n += C) {
+    // after the columns from n on are in the ring the line that starts n - off is whole; at a row's end a last
+    // turn without columns writes what is left
+    for (int n = 0; n < width + (last ? C : 0); n += C) {
 #pragma unroll
         for (int h = n; h < n + C; h += Step) {
             if (h >= width) continue;
@@ -706,7 +712,8 @@ __global__ __launch_bounds__(kBlock, 4) void k_mm_short(MmArgs p, int cols, int 
             else put_all(std::integral_constant<int, 1>());
         }
         asm volatile("" ::: "memory");   // (the wave's own LDS, written and read in order)
-        if (n >= C && n <= width - C && m0 + kShortRows <= p.m) {
+        if (n < lead) continue;
+        if ((n >= C || unit >= kLine) && n <= width - C && m0 + kShortRows <= p.m) {
 #pragma unroll
             for (int q = 0; q < NQ; ++q)
                 *reinterpret_cast<vu32x4*>(to[q] + n) = *reinterpret_cast<const vu32x4*>(
@@ -736,9 +743,9 @@ static void mm_short(MmArgs p, hipStream_t st) {
     const int64_t split = std::max<int64_t>(1, std::min<int64_t>((lines + 7) / 8, 2048 / p.mt));
     const int64_t cols = std::min<int64_t>((lines + split - 1) / split * C, kShortCols);
     const int64_t grid = p.mt * ((p.n + cols - 1) / cols);
-    // the largest power of two, up to four outputs, that divides every row's distance from a line's start
+    // the largest power of two, up to a line, that divides every row's distance from a line's start
     const uint64_t bytes = (uint64_t)(uintptr_t)p.y | (p.m > 1 ? (uint64_t)p.ldy * sizeof(TO) : 0);
-    const int unit = (int)std::min<uint64_t>(bytes & (0 - bytes), 16);
+    const int unit = (int)std::min<uint64_t>(bytes & (0 - bytes), kLine);
     launch(k_mm_short<E, TO>, dim3((unsigned)grid), kBlock, 0, st, p, (int)cols, unit);
 }
 
