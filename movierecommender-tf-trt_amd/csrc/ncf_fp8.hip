@@ -546,7 +546,6 @@ struct ShortRaw {
     }
     // the part with zeros past column k
     __device__ __forceinline__ void settle(int g, int k) {
-        if (k == 32 * E) return;
 #pragma unroll
         for (int e = 0; e < E; e += 2) {
             const int n = max(past(e, g, k), 0);
@@ -566,8 +565,9 @@ struct ShortOperand;
 template <int E>
 struct ShortOperand<true, E> {
     mf16x8 v[E];
+    template <bool EXACT>
     __device__ __forceinline__ void set(ShortRaw<E> raw, int g, int k) {
-        raw.settle(g, k);
+        if constexpr (!EXACT) raw.settle(g, k);
 #pragma unroll
         for (int e = 0; e < E; ++e) {
             const mi32x8 f = {(int)raw.v[e].x, (int)raw.v[e].y, 0, 0, 0, 0, 0, 0};
@@ -584,8 +584,9 @@ struct ShortOperand<true, E> {
 template <int E>
 struct ShortOperand<false, E> {
     mi32x8 v;
+    template <bool EXACT>
     __device__ __forceinline__ void set(ShortRaw<E> raw, int g, int k) {
-        raw.settle(g, k);
+        if constexpr (!EXACT) raw.settle(g, k);
         v = mi32x8{0, 0, 0, 0, 0, 0, 0, 0};
 #pragma unroll
         for (int e = 0; e < E; ++e) {
@@ -615,7 +616,8 @@ __device__ __forceinline__ void ring_put(uint8_t* ring, int col, vf32x4 y) {
 
 constexpr int kShortCols = 512;   // most columns of a workgroup (four workgroups a CU in LDS)
 
-template <int E, typename TO>
+// EXACT: k = 32 E, no part passes a row's end
+template <int E, typename TO, bool EXACT>
 __global__ __launch_bounds__(kBlock, 4) void k_mm_short(MmArgs p, int cols, int unit) {
     constexpr bool WIDE = std::is_same<TO, float>::value;
     constexpr int S = (int)sizeof(TO), C = kLine / S;      // columns of a line
@@ -655,7 +657,7 @@ __global__ __launch_bounds__(kBlock, 4) void k_mm_short(MmArgs p, int cols, int 
         const int64_t m = min(m0 + 16 * x + i, p.m - 1);
         ShortRaw<E> raw;
         raw.load(p.a + m * p.lda, g, p.k);
-        fa[x].set(raw, g, p.k);
+        fa[x].template set<EXACT>(raw, g, p.k);
         sa[x] = p.sa[m];
         put[x] = off_of(m) + 4 * g;
     }
@@ -663,12 +665,10 @@ __global__ __launch_bounds__(kBlock, 4) void k_mm_short(MmArgs p, int cols, int 
     constexpr int NQ = kShortRows / 8, P = 16 / S;
     const int piece = lane & 7;
     TO* to[NQ];         // where the lane's piece of the first line lies
-    int first[NQ];      // its first column, from c0
 #pragma unroll
     for (int q = 0; q < NQ; ++q) {
         const int64_t m = min(m0 + 8 * q + (lane >> 3), p.m - 1);
-        first[q] = P * piece - off_of(m);
-        to[q] = static_cast<TO*>(p.y) + m * p.ldy + c0 + first[q];
+        to[q] = static_cast<TO*>(p.y) + m * p.ldy + c0 + P * piece - off_of(m);
     }
     const uint8_t* b = p.b + c0 * p.ldb;
     ShortRaw<E> raw[NJ];
@@ -677,16 +677,15 @@ __global__ __launch_bounds__(kBlock, 4) void k_mm_short(MmArgs p, int cols, int 
         for (int j = 0; j < NJ; ++j) raw[j].load(b + (int64_t)min(n + 16 * j + i, width - 1) * p.ldb, g, p.k);
     };
     load_b(0);
-    // after the columns from n on are in the ring the line that starts n - off is whole; at a row's end a last
-    // turn without columns writes what is left
-    for (int n = 0; n < width + (last ? C : 0); n += C) {
+    // after the columns from n on are in the ring the line that starts n - off is whole
+    auto form = [&](int n, auto ragged) {
 #pragma unroll
         for (int h = n; h < n + C; h += Step) {
-            if (h >= width) continue;
+            if (decltype(ragged)::value && h >= width) continue;
             ShortOperand<WIDE, E> fb[NJ];
             vf32x4 y[NJ][NX];
 #pragma unroll
-            for (int j = 0; j < NJ; ++j) fb[j].set(raw[j], g, p.k);
+            for (int j = 0; j < NJ; ++j) fb[j].template set<EXACT>(raw[j], g, p.k);
             load_b(min(h + Step, width - 1));
 #pragma unroll
             for (int j = 0; j < NJ; ++j) {
@@ -712,23 +711,50 @@ __global__ __launch_bounds__(kBlock, 4) void k_mm_short(MmArgs p, int cols, int 
             else put_all(std::integral_constant<int, 1>());
         }
         asm volatile("" ::: "memory");   // (the wave's own LDS, written and read in order)
-        if (n < lead) continue;
-        if ((n >= C || unit >= kLine) && n <= width - C && m0 + kShortRows <= p.m) {
+    };
+    auto store_lines = [&](int n) {
 #pragma unroll
-            for (int q = 0; q < NQ; ++q)
-                *reinterpret_cast<vu32x4*>(to[q] + n) = *reinterpret_cast<const vu32x4*>(
-                    ring + (8 * q + (lane >> 3)) * kPitch + ((n * S + 16 * piece) & (2 * kLine - 1)));
-        } else {
+        for (int q = 0; q < NQ; ++q)
+            *reinterpret_cast<vu32x4*>(to[q] + n) = *reinterpret_cast<const vu32x4*>(
+                ring + (8 * q + (lane >> 3)) * kPitch + ((n * S + 16 * piece) & (2 * kLine - 1)));
+        asm volatile("" ::: "memory");
+    };
+    // Turns from `whole` on to `rest` write whole lines of whole tiles of rows.  For 16-bit outputs they have a
+    // loop without a branch around its stores: those and the next columns' loads are then counted together, and a
+    // turn no longer waits for the stores of the one before (8,192 x 27,264 x 64 bf16: 133 -> 111 us).  fp32
+    // outputs write twice as much, and waiting keeps the operands' loads from queueing behind their stores (in
+    // that loop 177 -> 187 us; with k = 128 221 -> 250).
+    const int whole = unit < kLine ? C : 0;
+    const int rest = m0 + kShortRows <= p.m && width >= whole + C ? width / C * C : whole;
+    const int end = width + (last ? C : 0);   // at a row's end a last turn without columns writes what is left
+    for (int n = 0; n < end;) {
+        if (!WIDE && n == whole && rest > whole) {
+            __builtin_amdgcn_s_waitcnt(0x0f70);   // vmcnt(0): nothing from before the loop counts in it
+#pragma unroll 1
+            for (; n < rest; n += C) {
+                form(n, std::false_type());
+                store_lines(n);
+            }
+            continue;
+        }
+        form(n, std::true_type());
+        if (WIDE && n >= whole && n < rest) {
+            store_lines(n);
+        } else if (n >= lead) {
 #pragma unroll 1
             for (int q = 0; q < NQ; ++q) {
-                const int row = 8 * q + (lane >> 3), c = n + first[q];
+                const int row = 8 * q + (lane >> 3);
+                if (m0 + row >= p.m) break;
+                const int c = n + P * piece - off_of(m0 + row);
+                TO* y = static_cast<TO*>(p.y) + (m0 + row) * p.ldy + c0;
                 const TO* from = reinterpret_cast<const TO*>(ring + row * kPitch +
                                                              ((n * S + 16 * piece) & (2 * kLine - 1)));
                 for (int e = 0; e < P; ++e)
-                    if (m0 + row < p.m && c + e >= 0 && c + e < width) to[q][n + e] = from[e];
+                    if (c + e >= 0 && c + e < width) y[c + e] = from[e];
             }
         }
         asm volatile("" ::: "memory");
+        n += C;
     }
 }
 
@@ -746,7 +772,8 @@ static void mm_short(MmArgs p, hipStream_t st) {
     // the largest power of two, up to a line, that divides every row's distance from a line's start
     const uint64_t bytes = (uint64_t)(uintptr_t)p.y | (p.m > 1 ? (uint64_t)p.ldy * sizeof(TO) : 0);
     const int unit = (int)std::min<uint64_t>(bytes & (0 - bytes), kLine);
-    launch(k_mm_short<E, TO>, dim3((unsigned)grid), kBlock, 0, st, p, (int)cols, unit);
+    if (p.k == 32 * E) launch(k_mm_short<E, TO, true>, dim3((unsigned)grid), kBlock, 0, st, p, (int)cols, unit);
+    else launch(k_mm_short<E, TO, false>, dim3((unsigned)grid), kBlock, 0, st, p, (int)cols, unit);
 }
 
 template <int MI, int NI, typename TO>
