@@ -178,8 +178,8 @@ struct RowShared {
         unsigned long long weight[kBins];
         unsigned long long before[kList];   // the list's running sums
     };
-    float list_x[kList];
-    uint32_t list_id[kList];
+    float list_x[kList + 64];   // behind the list a place for what does not belong there, one a lane
+    uint32_t list_id[kList + 64];
     unsigned long long member_w[NT];
     float member_x[NT];
     uint32_t member_id[NT];
@@ -710,18 +710,21 @@ __global__ __launch_bounds__(NT) void k_draw_row(DrawArgs a) {
                 for (int e = 0; e < V; ++e) any |= m[e] = __ballot(x[V * j + e] >= limit);
                 if (any != 0) {
                     uint32_t mine = at;
+                    int id = first + 64 * V * j;
+                    asm volatile("" : "+v"(id));   // (computed here, not kept from the passes before)
 #pragma unroll
                     for (int e = 0; e < V; ++e) {
                         mine = lanes_before(m[e], mine);
                         at += (uint32_t)lane_count(m[e]);
                     }
 #pragma unroll
-                    for (int e = 0; e < V; ++e)
-                        if (x[V * j + e] >= limit) {
-                            s.list_x[mine] = x[V * j + e];
-                            s.list_id[mine] = (uint32_t)(first + 64 * V * j + e);
-                            ++mine;
-                        }
+                    for (int e = 0; e < V; ++e) {   // (without a branch)
+                        const bool in = x[V * j + e] >= limit;
+                        const uint32_t to = in ? mine : (uint32_t)(kList + lane);
+                        s.list_x[to] = x[V * j + e];
+                        s.list_id[to] = (uint32_t)(id + e);
+                        mine += in;
+                    }
                 }
             }
             __builtin_amdgcn_sched_barrier(0);
