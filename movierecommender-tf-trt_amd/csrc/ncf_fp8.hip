@@ -17,6 +17,7 @@
 // The reference scores one user against a list of items (movierec/trt_client.py:43-57).
 
 #include <algorithm>
+#include <atomic>
 #include <cmath>
 #include <type_traits>
 
@@ -786,9 +787,16 @@ static void mm_direct(MmArgs p, hipStream_t st) {
 template <typename TO, bool B_TILE>
 static hipError_t mm_tile(MmArgs p, hipStream_t st) {
     constexpr size_t lds = 2 * sizeof(TileStage);
-    static const hipError_t attr = hipFuncSetAttribute(reinterpret_cast<const void*>(k_mm_tile<TO, B_TILE>),
-                                                       hipFuncAttributeMaxDynamicSharedMemorySize, (int)lds);
-    if (attr != hipSuccess) return attr;
+    static std::atomic<uint64_t> allowed{0};   // devices on which the kernel may use this much LDS
+    int dev = 0;
+    if (hipError_t e = hipGetDevice(&dev)) return e;
+    const uint64_t bit = 1ull << (dev & 63);
+    if (!(allowed.load(std::memory_order_relaxed) & bit)) {
+        if (hipError_t e = hipFuncSetAttribute(reinterpret_cast<const void*>(k_mm_tile<TO, B_TILE>),
+                                               hipFuncAttributeMaxDynamicSharedMemorySize, (int)lds))
+            return e;
+        allowed.fetch_or(bit, std::memory_order_relaxed);
+    }
     p.mt = (p.m + kTile - 1) / kTile;
     p.nt = (p.n + kTile - 1) / kTile;
     const int64_t per = (p.mt * p.nt + 7) / 8;

@@ -228,3 +228,10 @@ def test_refusals():
     for call in bad:
         with pytest.raises(ValueError):
             call()
+
+
+@pytest.mark.parametrize("dtype", [F, BF, HF])
+@pytest.mark.parametrize("shape", [(4096, 3200, 64), (2080, 6144, 32), (4001, 3201, 96), (130, 40003, 128)], ids=str)
+def test_short_rows_on_and_off_their_lines(shape, dtype):
+    """Rows of outputs that are whole lines of 128 bytes, and rows that start anywhere in one."""
+    check_product(*operands(*shape, False, seed=12), dtype, False)

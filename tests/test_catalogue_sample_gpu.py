@@ -245,3 +245,30 @@ def test_empty_and_refusals():
     for f in bad:
         with pytest.raises(ValueError):
             f()
+
+
+@pytest.mark.parametrize("shift", [-20.0, 20.0])
+@pytest.mark.parametrize("n", [300, 5000, 20000, 60000])
+@pytest.mark.parametrize("dtype", ["bfloat16", "float16"])
+def test_sixteen_bit_logits_of_either_sign_with_many_equals(dtype, n, shift):
+    """Few distinct values, all of one sign: the bound is found digit by digit of a 16-bit logit."""
+    x = (torch.randint(0, 24, (3, n), generator=gen(n)) / 16 + shift).to(getattr(torch, dtype))
+    x[1, ::2] = -x[1, ::2]
+    u = torch.rand(3, 6, generator=gen(n + 2))
+    for s in (dict(k=n // 2), dict(k=n - 1, p=0.8), dict(p=0.35), dict(p=0.9, t=3.0), dict(k=n // 3, min_p=0.4)):
+        check(x, u, *call(x, u, **s), **s)
+
+
+@pytest.mark.parametrize("n", [64, 3000, 27278, 40000])
+def test_min_p_and_infinite_temperature(n):
+    """Every item weighs the same in an infinite temperature, infinite logits included; min_p = 1 keeps what
+    equals the best."""
+    x = logits(3, n, "float32", 12)
+    x[1, : n // 4] = float("inf")
+    x[2, 5] = x[2].max()
+    u = torch.rand(3, 4, generator=gen(13))
+    hot = torch.full((3,), float("inf"))
+    it, pr = C.sample_items(x.cuda()[:1], u.cuda()[:1], temperature=hot.cuda()[:1])
+    check(x[:1], u[:1], it, pr, t=np.inf)
+    check(x, u, *call(x, u, min_p=1.0), min_p=1.0)
+    check(x, u, *call(x, u, min_p=1e-30), min_p=1e-30)
