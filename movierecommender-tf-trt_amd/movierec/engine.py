@@ -465,6 +465,8 @@ class NCFEngine(object):
         n = ids.numel()
         if not torch.is_tensor(u) or u.dim() not in (1, 2) or u.shape[0] != n:
             raise ValueError("u must have shape (%d,) or (%d, draws)" % (n, n))
+        if mask is not None and not torch.is_tensor(mask):
+            raise ValueError("mask must be a bool or uint8 tensor")
         step = max(1, SAMPLE_LOGITS // self.num_items)
         settings = dict(temperature=temperature, top_k=top_k, top_p=top_p, min_p=min_p)
         items = torch.empty(u.shape, dtype=torch.int32, device=self.device)

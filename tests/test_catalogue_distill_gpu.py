@@ -21,12 +21,12 @@ if gpu_available():
 
 
 def reference(x, items, y, t, lse, gl):
-    """Loss and gradient in float64, row by row: (loss, grad, p c, q, sum q + q0)."""
+    """Loss and gradient in float64, row by row: (loss, grad, p c, q, sum q + q0, p q0 in / out)."""
     x, y = x.double().numpy(), y.double().numpy()
     items = items.numpy()
     rows, v = x.shape
     loss, grad = np.zeros(rows), np.zeros((rows, v))
-    pc, qv, mass = np.zeros((rows, v)), np.zeros((rows, v)), np.zeros(rows)
+    pc, qv, mass, part = np.zeros((rows, v)), np.zeros((rows, v)), np.zeros(rows), np.zeros((rows, v))
     with np.errstate(all="ignore"):
         for r in range(rows):
             m = x[r].max()
@@ -56,17 +56,18 @@ def reference(x, items, y, t, lse, gl):
                     loss[r] += q0 * (np.log(q0) + np.log1p(w[listed].sum() / out))
                     cin = q.sum() + q0
                     cout = cin - q0 * s / out
+                    part[r] = np.where(listed, 0, w / s * q0 * w[listed].sum() / out)
             np.add.at(qv[r], it, q)
             pc[r] = w / s * np.where(listed, cin, cout)
             mass[r] = abs(cin) + q.sum()
             grad[r] = (pc[r] - qv[r]) * gl[r] / t
-    return loss, grad, pc, qv, mass
+    return loss, grad, pc, qv, mass, part
 
 
 def check(x, items, y, t=1.0, lse=None, gl=None, got=None):
     rows = x.shape[0]
     g = np.ones(rows) if gl is None else gl.double().numpy()
-    loss, grad, pc, qv, mass = reference(x, items, y, t, None if lse is None else lse.double().numpy(), g)
+    loss, grad, pc, qv, mass, part = reference(x, items, y, t, None if lse is None else lse.double().numpy(), g)
     xd = x.double().numpy()
     with np.errstate(all="ignore"):
         z = np.abs(np.where(np.isfinite(xd), xd - xd.max(1, keepdims=True), 0) / t)
@@ -75,7 +76,9 @@ def check(x, items, y, t=1.0, lse=None, gl=None, got=None):
     assert np.all(np.abs(got[0].double().cpu().numpy() - loss) <= 2 * mass * e + np.abs(loss) * 2.0 ** -23 + 1e-30)
     if len(got) > 1:
         fi = torch.finfo(x.dtype)
-        tol = (np.abs(pc) * (2 * e[:, None] + 2.0 ** -21) + qv * 2.0 ** -22) * np.abs(g)[:, None] / t
+        # c outside = sum q - q0 in / out is a difference of the two: in and out are each off by e, so the second
+        # term by 2 e of itself, which is more than 2 e of a c that cancels (k = 1, q = 0.0208, q0 in / out = 0.0210)
+        tol = (np.abs(pc) * (2 * e[:, None] + 2.0 ** -21) + qv * 2.0 ** -22 + part * 2 * e[:, None]) * np.abs(g)[:, None] / t
         tol = tol + np.maximum((np.abs(grad) + tol) * fi.eps / 2, fi.smallest_normal * fi.eps)
         assert got[1].dtype == x.dtype
         err = np.abs(got[1].double().cpu().numpy() - grad)
@@ -267,3 +270,20 @@ def test_empty_and_refusals():
     for f in bad:
         with pytest.raises(ValueError):
             f()
+
+
+@pytest.mark.parametrize("k", [1, 63, 64, 65])
+@pytest.mark.parametrize("dtype", ["float32", "bfloat16"])
+def test_many_long_rows_with_padding_and_duplicates(dtype, k):
+    """Rows that a workgroup of several waves holds, lists on both sides of a wave's 64 entries."""
+    x, items, y, lse = problem(130, 9001, k, dtype=dtype, seed=k, lse_t=1.0)
+    items[0] = -1
+    items[1] = items[1, 0]
+    items[2, k // 2:] = 9001 + 2 ** 33
+    items[3] = 9000                          # the last item, in the row's last, partial vector
+    y[4] = -float("inf")
+    x[5] = -float("inf")
+    x[6, items[6, 0]] = -float("inf")        # a listed item whose logit is masked: the loss is infinite
+    y[6, 0] = -float("inf")                  # (but not when it has no mass)
+    both(x, items, y)
+    both(x, items, y, 1.0, lse + 0.2, torch.rand(130, generator=torch.Generator().manual_seed(2)))

@@ -146,6 +146,8 @@ def test_engine_draws_are_those_of_its_logits(monkeypatch):
     assert torch.equal(parts[0], items) and torch.equal(parts[1], probs)
     with pytest.raises(ValueError):
         eng.sample_items(users, u[:49])
+    with pytest.raises(ValueError):
+        eng.sample_items(users, u, mask=mask.cpu().numpy())
 
 
 def model(tmp_path, name, layers=(64, 32, 16, 8), gmf=8, seed=1, l2=0.0):
