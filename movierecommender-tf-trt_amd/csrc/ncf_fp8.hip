@@ -508,6 +508,8 @@ __global__ __launch_bounds__(kTileThreads, 2) void k_mm_tile(MmArgs p) {
 // two such pieces in LDS, placed by their address in y, so that every store writes whole, aligned lines of
 // 128 bytes whatever the distance of the rows (8,192 x 27,278 fp32, rows 8 bytes off: 16-byte stores at
 // their own addresses took 100 us of 303).
+// Measured, 8,192 x 27,278 x 64: fp32 175 us (5.1 TB/s written; these stores alone, without a product, take
+// 162), bf16 105; rows on their lines (27,264) 167 and 89.
 
 constexpr int kShortRows = 32;
 constexpr int kShortWaves = kBlock / 64;
@@ -628,9 +630,13 @@ __global__ __launch_bounds__(kBlock, 4) void k_mm_short(MmArgs p, int cols, int 
     __shared__ __attribute__((aligned(16))) float col_scale[kShortCols + C], col_bias[kShortCols + C];
     const int lane = threadIdx.x & 63, g = lane >> 4, i = lane & 15;
     const int wave = __builtin_amdgcn_readfirstlane((int)(threadIdx.x >> 6));
-    const uint32_t mt = (uint32_t)p.mt;
-    const int64_t m0 = ((int64_t)(blockIdx.x % mt) * kShortWaves + wave) * kShortRows;
-    const int64_t part = blockIdx.x / mt;
+    // Parts of the same rows follow each other on one XCD: its writes stay close to each other, and its L2 holds
+    // the rows' operand (parts spread over the XCDs, rows first: 8,192 x 27,278 x 64 fp32 197 us, bf16 126)
+    const uint32_t parts = (uint32_t)((p.n + cols - 1) / cols), total = parts * (uint32_t)p.mt;
+    const uint32_t at = (blockIdx.x & 7) * ((total + 7) / 8) + (blockIdx.x >> 3);
+    if (at >= total) return;
+    const int64_t m0 = ((int64_t)(at / parts) * kShortWaves + wave) * kShortRows;
+    const int64_t part = at % parts;
     const bool last = (part + 1) * cols >= p.n;
     // Columns of this workgroup, from c0 on.  Where rows do not start on a line it writes the lines that start
     // up to C columns ahead of its own part, and forms those columns too: only a row's ends are written in
@@ -724,7 +730,7 @@ __global__ __launch_bounds__(kBlock, 4) void k_mm_short(MmArgs p, int cols, int 
     // loop without a branch around its stores: those and the next columns' loads are then counted together, and a
     // turn no longer waits for the stores of the one before (8,192 x 27,264 x 64 bf16: 133 -> 111 us).  fp32
     // outputs write twice as much, and waiting keeps the operands' loads from queueing behind their stores (in
-    // that loop 177 -> 187 us; with k = 128 221 -> 250).
+    // that loop 8,192 x 27,278 x 128 took 206-212 us, so 202; with k = 64 180, so 182).
     const int whole = unit < kLine ? C : 0;
     const int rest = m0 + kShortRows <= p.m && width >= whole + C ? width / C * C : whole;
     const int end = width + (last ? C : 0);   // at a row's end a last turn without columns writes what is left
@@ -764,12 +770,14 @@ static void mm_short(MmArgs p, hipStream_t st) {
     constexpr int C = kLine / (int)sizeof(TO);
     constexpr int64_t rows = kShortWaves * kShortRows;
     p.mt = (p.m + rows - 1) / rows;
-    // columns of a workgroup: whole lines, at least eight of them where there are, and no more than LDS
-    // holds scales for; about 2048 workgroups together
+    // Columns of a workgroup: whole lines, about 2,048 workgroups together.  At least four lines (two and eight:
+    // 2,000 x 3,706 x 128 bf16 15.8 and 21 us, so 13.6) and at most eight, or for k > 64 as many as LDS holds
+    // scales for (8,192 x 27,278 fp32 at most eight and sixteen: k = 64 175 and 182 us, k = 128 210 and 202).
     const int64_t lines = (p.n + C - 1) / C;
-    const int64_t split = std::max<int64_t>(1, std::min<int64_t>((lines + 7) / 8, 2048 / p.mt));
-    const int64_t cols = std::min<int64_t>((lines + split - 1) / split * C, kShortCols);
-    const int64_t grid = p.mt * ((p.n + cols - 1) / cols);
+    constexpr int64_t least = 4, most = E == 4 ? kShortCols / C : 8;
+    const int64_t split = std::max<int64_t>(1, std::min<int64_t>((lines + least - 1) / least, 2048 / p.mt));
+    const int64_t cols = std::min<int64_t>((lines + split - 1) / split, most) * C;
+    const int64_t grid = (p.mt * ((p.n + cols - 1) / cols) + 7) / 8 * 8;
     // the largest power of two, up to a line, that divides every row's distance from a line's start
     const uint64_t bytes = (uint64_t)(uintptr_t)p.y | (p.m > 1 ? (uint64_t)p.ldy * sizeof(TO) : 0);
     const int unit = (int)std::min<uint64_t>(bytes & (0 - bytes), kLine);
