@@ -518,7 +518,7 @@ __global__ __launch_bounds__(NT, 4) void k_distill_row(DistArgs a) {
 
 // The same for lists of up to 64 entries: the first wave holds the list, an entry a lane, and works on it
 // while the row is on its way, without a barrier; the gradient's q are taken off the written row at the end.
-// (Rows of 27,278 bf16 logits, lists of 32: 88 us by the kernel above for 2,048 rows, MEASURED here.)
+// 2,048 rows of 27,278 bf16 logits, lists of 32: 59 us, by the kernel above 88; 27,278 fp32 96 and 125.
 constexpr int kWaveList = 64;
 
 template <typename T, int NT, int EPT, bool GRAD>
@@ -654,13 +654,16 @@ static DistArgs dist_args(const ncf_distill_t& c, void* ws) {
     return a;
 }
 
-// A row goes to one workgroup where it fits its registers; few rows of more than a chunk each would leave
-// CUs idle, so those go by chunks.
-static bool by_row(int64_t rows, int64_t v) { return v <= kDistChunk || (v <= 512 * 56 && rows >= 128); }
+// A row goes to one workgroup where its registers hold it, however few the rows (27,278 fp32 logits by chunks:
+// one row 18.7 us, so 13.1; 512 rows 44 and 23; 2,048 rows 146 and 96).
+// Twice as long a row, a CU's registers full, only with a list that a wave holds (40,000 logits, lists of 32: one
+// row 18.7 us, so 14.6; 1,024 rows 93 and 86).
+constexpr int64_t kRowMost = 512 * 56;
+static bool by_row(int64_t v, int64_t k) { return v <= kRowMost || (v <= 2 * kRowMost && k <= kWaveList); }
 
 // for the chunks' sums and, behind them, the state where the caller takes none
 size_t distill_workspace(int64_t rows, int v) {
-    if (by_row(rows, v)) return 0;
+    if (v <= kRowMost) return 0;
     const size_t n = (size_t)rows * ((v + kDistChunk - 1) / kDistChunk);
     return n * sizeof(double2) + (n + (n & 1)) * sizeof(float) + (size_t)rows * kState * sizeof(double);
 }
@@ -684,11 +687,13 @@ static void distill_row(const DistArgs& a, bool backward, hipStream_t st) {
 template <typename T>
 static hipError_t distill_t(const DistArgs& a, bool forward, bool backward, hipStream_t st) {
     const unsigned grid = (unsigned)(a.rows * a.chunks);
-    if (forward && by_row(a.rows, a.v)) {
+    if (forward && by_row(a.v, a.k)) {
         if (a.v <= 64 * 8) distill_row<T, 64, 8>(a, backward, st);
         else if (a.v <= 64 * 32) distill_row<T, 64, 32>(a, backward, st);
         else if (a.v <= 256 * 32) distill_row<T, 256, 32>(a, backward, st);
-        else distill_row<T, 512, 56>(a, backward, st);
+        else if (a.v <= 512 * 56) distill_row<T, 512, 56>(a, backward, st);
+        else if (backward) launch(k_distill_row_wave<T, 1024, 56, true>, dim3((unsigned)a.rows), 1024, 0, st, a);
+        else launch(k_distill_row_wave<T, 1024, 56, false>, dim3((unsigned)a.rows), 1024, 0, st, a);
         return hipGetLastError();
     }
     if (forward) {

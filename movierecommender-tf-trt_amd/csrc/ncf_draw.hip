@@ -1403,7 +1403,7 @@ static LongLayout long_layout(int64_t rows, int64_t n, int vec) {
     return l;
 }
 
-constexpr int kRowMost = 512 * 56;   // the longest row that two workgroups a CU hold in registers
+constexpr int kRowMost = 1024 * 40;   // the longest row that a CU holds in registers, nothing spilled
 
 size_t draw_workspace(int64_t rows, int64_t n) {
     return rows > 0 && n > kRowMost ? long_layout(rows, n, Elem<float>::kVec).total : 0;
@@ -1447,13 +1447,17 @@ static void draw_long(const DrawArgs& a, void* ws, bool may_k, bool may_p, hipSt
     launch(k_long_draw<T>, dim3((unsigned)(a.rows * a.draws)), kLongThreads, 0, st, l);
 }
 
+// The smallest workgroup that holds a row, and the next one (us for 4,096 rows, top-50, top-p 0.9): 500 items 15.2
+// and 15.6, 2,000 20.6 and 41.5, 8,000 58 and 115.  A row in registers, and by the launches over parts of it: one row
+// of 27,278 17.3 and 59.5, 2,048 88 and 408; one of 40,000 18.9 and 57.5, 1,024 84 and 269.
 template <typename T>
 static void draw_t(const DrawArgs& a, void* ws, bool may_k, bool may_p, hipStream_t st) {
     const dim3 grid((unsigned)a.rows);
     if (a.n <= 64 * 8) launch(k_draw_row<T, 64, 8>, grid, 64, 0, st, a);
     else if (a.n <= 64 * 32) launch(k_draw_row<T, 64, 32>, grid, 64, 0, st, a);
     else if (a.n <= 256 * 32) launch(k_draw_row<T, 256, 32>, grid, 256, 0, st, a);
-    else if (a.n <= kRowMost) launch(k_draw_row<T, 512, 56>, grid, 512, 0, st, a);
+    else if (a.n <= 512 * 56) launch(k_draw_row<T, 512, 56>, grid, 512, 0, st, a);
+    else if (a.n <= kRowMost) launch(k_draw_row<T, 1024, 40>, grid, 1024, 0, st, a);
     else draw_long<T>(a, ws, may_k, may_p, st);
 }
 

@@ -812,12 +812,19 @@ static hipError_t mm_tile(MmArgs p, hipStream_t st) {
     return hipGetLastError();
 }
 
+// Which kernel, and both sides of each choice (us):
+//   more than 64 tiles of 256 x 256, k > 128: k_mm_tile (2,304 x 2,304 x 1,024, 81 tiles: bf16 31, fp32 45, so 46 and
+//     58 by k_mm_direct; 2,048 x 2,048, 64 tiles: 28.6 and 44, so 28.5 and 29; 4,096 x 4,096 x 144: 22, so 24)
+//   k <= 128 and 1,024 waves of 64 x 64: k_mm_short (4,096 x 4,096 x 64 fp32 15, so 36; 2,048 x 1,682: both 10.5)
+//   up to 16 rows: a tile a wave (8 x 4,096 x 4,096: 18, with 2 x 2 tiles 34, 4 x 4 70)
+//   1,024 waves of 64 x 64: 4 x 4 tiles a wave, else 2 x 2 (2,000 x 2,000 x 256 fp32 14 and 16.5;
+//     333 x 1,682 x 200 19 and 10.5)
 template <typename TO>
 static hipError_t mm_t(const MmArgs& p, hipStream_t st) {
     const bool aligned = ((uintptr_t)p.a | (uintptr_t)p.b | (uint64_t)p.lda | (uint64_t)p.ldb) % 16 == 0;
     // (rows up to 16 MB apart: a thread's offsets in 32 bits)
     const bool near = p.lda <= 1 << 24 && p.ldb <= 1 << 24;
-    if (aligned && near && p.k > kScaleBlock && ((p.m + kTile - 1) / kTile) * ((p.n + kTile - 1) / kTile) >= 128)
+    if (aligned && near && p.k > kScaleBlock && ((p.m + kTile - 1) / kTile) * ((p.n + kTile - 1) / kTile) > 64)
         return p.b_tile ? mm_tile<TO, true>(p, st) : mm_tile<TO, false>(p, st);
     const int64_t waves = ((p.m + 63) / 64) * ((p.n + 63) / 64);   // of 64 x 64
     if (p.k <= kScaleBlock && waves >= 1024) {

@@ -287,3 +287,12 @@ def test_many_long_rows_with_padding_and_duplicates(dtype, k):
     y[6, 0] = -float("inf")                  # (but not when it has no mass)
     both(x, items, y)
     both(x, items, y, 1.0, lse + 0.2, torch.rand(130, generator=torch.Generator().manual_seed(2)))
+
+
+@pytest.mark.parametrize("k", [5, 64, 65])
+@pytest.mark.parametrize("v", [28673, 40001, 57344, 57345])
+def test_rows_around_the_longest_that_a_workgroup_holds(v, k):
+    x, items, y, lse = problem(3, v, k, dtype="bfloat16" if v % 2 else "float32", seed=v + k, lse_t=1.2)
+    items[1, 1] = items[1, 0]
+    both(x, items, y, 1.2)
+    both(x, items, y, 1.2, lse, torch.rand(3, generator=torch.Generator().manual_seed(2)))

@@ -91,7 +91,7 @@ def test_distill_arguments(call):
         refused(distill(call, **kw))
     if call != "grad":
         refused(distill(call, loss=None))
-        long = dict(v=9000, ld=9000, grad_ld=9000)   # a row of several chunks
+        long = dict(v=60000, ld=60000, grad_ld=60000)   # longer than a workgroup holds
         refused(distill(call, ws=None, **long))
         refused(distill(call, ws_bytes=8, **long))
     if call != "both":

@@ -272,3 +272,15 @@ def test_min_p_and_infinite_temperature(n):
     check(x[:1], u[:1], it, pr, t=np.inf)
     check(x, u, *call(x, u, min_p=1.0), min_p=1.0)
     check(x, u, *call(x, u, min_p=1e-30), min_p=1e-30)
+
+
+@pytest.mark.parametrize("dtype", ["float32", "bfloat16"])
+@pytest.mark.parametrize("n", [28672, 28673, 40960, 40961])
+def test_rows_around_the_longest_that_a_workgroup_holds(n, dtype):
+    x = logits(4, n, dtype, n)
+    x[3] = (x[3] * 2).round()                # many equals
+    mask = torch.rand(4, n, generator=gen(5)) < 0.8
+    mask[2] = False
+    u = torch.rand(4, 7, generator=gen(n + 1))
+    for s in (dict(), dict(k=5000, p=0.9), dict(k=n // 2, t=3.0), dict(p=0.4, min_p=0.01), dict(k=100)):
+        check(x, u, *call(x, u, mask=mask, **s), mask=mask, **s)
