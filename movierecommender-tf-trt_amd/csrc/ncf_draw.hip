@@ -131,8 +131,8 @@ __device__ __forceinline__ bool reaches(unsigned long long c, double p, double t
 // For top-k with k <= 4 NT the histogram sees one of V neighbours only and gives a limit that the k best
 // most likely pass; the items that pass it, if they are at least k and at most 4 NT, move to a list in LDS
 // in the order of the ids, and the row is not looked at again.  (Otherwise the whole row is counted.)
-// 2,048 rows of 27,278 fp32 with a mask, top-1,000, top-p, min-p: 138 us, 2.0 TB/s.  Of a row's 69,000 cycles 33,000
-// are its load, 10,600 the list, 12,600 the two cuts; two workgroups a CU overlap theirs.  One row: 16 us.
+// 2,048 rows of 27,278 fp32 with a mask, top-1,000, top-p, min-p: 101 us, 2.8 TB/s.  36,000 cycles of a row are its
+// work: the list 10,600, the two cuts 12,600; two workgroups a CU overlap theirs.  One row: 15 us.
 
 __device__ __forceinline__ int lane_count(uint64_t mask) { return (int)__popcll(mask); }
 // set bits of the mask below this lane, plus `more`
@@ -539,27 +539,50 @@ __device__ __forceinline__ unsigned long long draw_target(const DrawArgs& a, int
     return t >= total ? total - 1 : t;
 }
 
-// V neighbours' logits from item i on; -inf where not allowed or past the row's end
+// V neighbours' logits as they are stored (-inf past the row's end) and their mask bytes: loaded ahead, settled
+// when they are used.  (Settled as they came, a row's vectors were loaded one behind the other: 33,000 of a row's
+// 69,000 cycles in k_draw_row.)
 template <typename T>
-__device__ __forceinline__ void load_logits(const DrawArgs& a, int64_t row, int i, float* r) {
-    constexpr int V = Elem<T>::kVec;
-    const T* x = static_cast<const T*>(a.logits) + row * a.ld;
-    const uint8_t* mask = a.mask ? a.mask + row * a.mask_ld : nullptr;
-    if (i + V <= a.n) {
-        const typename Elem<T>::vec w = *reinterpret_cast<const typename Elem<T>::vec*>(x + i);
+struct RawLogits {
+    static constexpr int V = Elem<T>::kVec;
+    typedef T own __attribute__((ext_vector_type(V)));
+    own v;
+    uint32_t on[V / 4];
+
+    // from item i on
+    __device__ __forceinline__ void load(const DrawArgs& a, int64_t row, int i) {
+        const T* x = static_cast<const T*>(a.logits) + row * a.ld;
+        const uint8_t* mask = a.mask ? a.mask + row * a.mask_ld : nullptr;
+        if (i + V <= a.n) {
+            v = *reinterpret_cast<const typename Elem<T>::vec*>(x + i);
+            if (mask) __builtin_memcpy(on, mask + i, V);
+        } else {
 #pragma unroll
-        for (int e = 0; e < V; ++e) r[e] = fmaxf((float)w[e], -INFINITY);   // (a NaN becomes -inf)
-        if (mask) {
-            uint32_t on[V / 4];
-            __builtin_memcpy(on, mask + i, V);
+            for (int e = 0; e < V; ++e) v[e] = i + e < a.n ? x[i + e] : (T)(-INFINITY);
+            if (mask) {
+#pragma unroll
+                for (int w = 0; w < V / 4; ++w) on[w] = 0;
+#pragma unroll
+                for (int e = 0; e < V; ++e)
+                    if (i + e < a.n) on[e / 4] |= (uint32_t)mask[i + e] << (8 * (e & 3));
+            }
+        }
+    }
+    // -inf where not allowed
+    __device__ __forceinline__ void settle(const DrawArgs& a, float* r) const {
+#pragma unroll
+        for (int e = 0; e < V; ++e) r[e] = fmaxf((float)v[e], -INFINITY);   // (a NaN becomes -inf)
+        if (a.mask) {
 #pragma unroll
             for (int e = 0; e < V; ++e) r[e] = (on[e / 4] >> (8 * (e & 3)) & 0xffu) ? r[e] : -INFINITY;
         }
-    } else {
-#pragma unroll
-        for (int e = 0; e < V; ++e)
-            r[e] = i + e < a.n && (mask == nullptr || mask[i + e] != 0) ? fmaxf((float)x[i + e], -INFINITY) : -INFINITY;
     }
+};
+template <typename T>
+__device__ __forceinline__ void load_logits(const DrawArgs& a, int64_t row, int i, float* r) {
+    RawLogits<T> raw;
+    raw.load(a, row, i);
+    raw.settle(a, r);
 }
 
 // a copy the compiler takes for a new value: what one pass over the row derives from its logits (bins,
@@ -580,11 +603,16 @@ __global__ __launch_bounds__(NT) void k_draw_row(DrawArgs a) {
     // a wave's vectors, of 64 V neighbours each: the row spread evenly over the waves
     const int jn = (a.n + NT * V - 1) / (NT * V), segs = jn * W;
     const int first = wave * jn * 64 * V + lane * V;   // of the thread's vector 0; vector j: 64 V j further
+    RawLogits<T> raw[J];
+#pragma unroll
+    for (int j = 0; j < J; ++j)
+        if (j < jn) raw[j].load(a, row, first + 64 * V * j);
+    __builtin_amdgcn_sched_barrier(0);
     float x[EPT];
 #pragma unroll
     for (int j = 0; j < J; ++j) {
         if (j < jn) {
-            load_logits<T>(a, row, first + 64 * V * j, x + V * j);
+            raw[j].settle(a, x + V * j);
         } else {
 #pragma unroll
             for (int e = 0; e < V; ++e) x[V * j + e] = -INFINITY;
@@ -875,8 +903,8 @@ __global__ __launch_bounds__(NT) void k_draw_row(DrawArgs a) {
 // top-p by weights) the histogram over kLongBins steps of the logit, the items of the bin that holds the
 // cut, and the bound among them (one workgroup a row; where the items outgrow their list it reads the row
 // again instead); the weight of every segment of 64 vectors; the draws.  The row comes from memory once
-// and from the caches after that (1,000,000 items are 2 or 4 MB).  16 rows of 1,000,000 bf16, top-p: 91 us, of them
-// histogram 24, segments' weights 23 (64-bit exponentials both), gather 15, bound 10, draws 9, best 8.  Workgroups of
+// and from the caches after that (1,000,000 items are 2 or 4 MB).  16 rows of 1,000,000 bf16, top-p: 87 us, of them
+// histogram 23, segments' weights 22 (64-bit exponentials both), gather 14, bound 11, draws 9, best 8.  Workgroups of
 // 1,024: of 256 the same, but four times as many histograms to join.
 
 constexpr int kLongThreads = 1024;
@@ -929,13 +957,18 @@ __device__ __forceinline__ void each_vector(const LongArgs& l, int64_t r, int pa
     int s0, s1;
     wave_segments<T>(l, part, &s0, &s1);
     for (int sg = s0; sg < s1; sg += U) {
-        float y[U][V];
-#pragma unroll
-        for (int u = 0; u < U; ++u)   // (past the part: as past the row's end)
-            load_logits<T>(l.a, r, sg + u < s1 ? (sg + u) * seg_items<T>() + lane * V : l.a.n, y[u]);
+        RawLogits<T> raw[U];
 #pragma unroll
         for (int u = 0; u < U; ++u)
-            if (sg + u < s1) f(y[u], (sg + u) * seg_items<T>() + lane * V);
+            if (sg + u < s1) raw[u].load(l.a, r, (sg + u) * seg_items<T>() + lane * V);
+        __builtin_amdgcn_sched_barrier(0);
+#pragma unroll
+        for (int u = 0; u < U; ++u) {
+            if (sg + u >= s1) break;
+            float y[V];
+            raw[u].settle(l.a, y);
+            f(y, (sg + u) * seg_items<T>() + lane * V);
+        }
     }
 }
 
@@ -1407,7 +1440,7 @@ static LongLayout long_layout(int64_t rows, int64_t n, int vec) {
     return l;
 }
 
-constexpr int kRowMost = 1024 * 40;   // the longest row that a CU holds in registers, nothing spilled
+constexpr int kRowMost = 512 * 56;   // the longest row that two workgroups a CU hold; behind it one of 1,024 does
 
 size_t draw_workspace(int64_t rows, int64_t n) {
     return rows > 0 && n > kRowMost ? long_layout(rows, n, Elem<float>::kVec).total : 0;
@@ -1453,15 +1486,16 @@ static void draw_long(const DrawArgs& a, void* ws, bool may_k, bool may_p, hipSt
 
 // The smallest workgroup that holds a row, and the next one (us for 4,096 rows, top-50, top-p 0.9): 500 items 15.2
 // and 15.6, 2,000 20.6 and 41.5, 8,000 58 and 115.  A row in registers, and by the launches over parts of it: one row
-// of 27,278 17.3 and 59.5, 2,048 88 and 408; one of 40,000 18.9 and 57.5, 1,024 84 and 269.
+// of 27,278 17.3 and 59.5, 2,048 88 and 408; one of 40,000 18.9 and 57.5, 1,024 84 and 269 (fp32).
 template <typename T>
 static void draw_t(const DrawArgs& a, void* ws, bool may_k, bool may_p, hipStream_t st) {
+    constexpr int kMost = sizeof(T) == 4 ? 40 : 32;   // (nothing spilled)
     const dim3 grid((unsigned)a.rows);
     if (a.n <= 64 * 8) launch(k_draw_row<T, 64, 8>, grid, 64, 0, st, a);
     else if (a.n <= 64 * 32) launch(k_draw_row<T, 64, 32>, grid, 64, 0, st, a);
     else if (a.n <= 256 * 32) launch(k_draw_row<T, 256, 32>, grid, 256, 0, st, a);
-    else if (a.n <= 512 * 56) launch(k_draw_row<T, 512, 56>, grid, 512, 0, st, a);
-    else if (a.n <= kRowMost) launch(k_draw_row<T, 1024, 40>, grid, 1024, 0, st, a);
+    else if (a.n <= kRowMost) launch(k_draw_row<T, 512, 56>, grid, 512, 0, st, a);
+    else if (a.n <= 1024 * kMost) launch(k_draw_row<T, 1024, kMost>, grid, 1024, 0, st, a);
     else draw_long<T>(a, ws, may_k, may_p, st);
 }
 

@@ -275,7 +275,7 @@ def test_min_p_and_infinite_temperature(n):
 
 
 @pytest.mark.parametrize("dtype", ["float32", "bfloat16"])
-@pytest.mark.parametrize("n", [28672, 28673, 40960, 40961])
+@pytest.mark.parametrize("n", [28672, 28673, 32768, 32769, 40960, 40961])
 def test_rows_around_the_longest_that_a_workgroup_holds(n, dtype):
     x = logits(4, n, dtype, n)
     x[3] = (x[3] * 2).round()                # many equals
