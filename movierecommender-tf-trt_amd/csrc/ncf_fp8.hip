@@ -4,15 +4,12 @@
 // per 128 x 128 tile): x ~ s q, s = max(max|x| / 448, 2^-126), q = e4m3(x / s), both roundings to
 // nearest even.  The product is
 //     y[m][n] = bias[n] + sum_j sa[m][j] sb[n][j] (sum over block j of qa[m][k] qb[n][k]),
-// a block's sum on MFMA from a zero accumulator, then added, scaled, to the fp32 total.  Two forms of
-// the block's sum, by the output's type:
-//   fp32 outputs    the e4m3 values widened to fp16 (exact) on v_mfma_f32_16x16x32_f16: products and
-//                   sums in fp32 (relative error of a random 128-block 9e-9)
-//   16-bit outputs  v_mfma_f32_16x16x128_f8f6f4, twice the rate.  It aligns the products of each 8
-//                   neighbouring k to the largest and drops what lies more than 13 binary places
-//                   below its exponent (measured: 448 * 448 + 4 gives 448 * 448; a random 128-block
-//                   is off by 1.5e-5) — below half a step of bf16 (2^-9) and fp16 (2^-12) but not of
-//                   fp32.  v_mfma_f32_16x16x32_fp8_fp8 drops the same.
+// a block's sum on MFMA from a zero accumulator, then added, scaled, to the fp32 total, which is rounded
+// once to the output's type.  The e4m3 values are widened to fp16 (exact) for v_mfma_f32_16x16x32_f16, whose
+// products and sums are fp32 (relative error of a random 128-block 9e-9).  The 8-bit instruction
+// v_mfma_f32_16x16x128_f8f6f4 has twice the rate, but it aligns the products of each 8 neighbouring k to the
+// largest and drops what lies more than 13 binary places below its exponent (448 * 448 + 4 - 448 * 448 gives
+// 0): where products cancel, 16-bit outputs see that too.  v_mfma_f32_16x16x32_fp8_fp8 drops the same.
 //
 // The reference scores one user against a list of items (movierec/trt_client.py:43-57).
 
@@ -193,19 +190,7 @@ __device__ __forceinline__ mi32x8 load_frag(const uint8_t* row, int c, int k) {
 }
 
 // a fragment as the MFMA takes it: widened once, for all the products it enters
-template <bool WIDE>
-struct Operand;
-template <>
-struct Operand<false> {
-    mi32x8 v;
-    __device__ __forceinline__ void set(mi32x8 f) { v = f; }
-    __device__ __forceinline__ static vf32x4 product(const Operand& a, const Operand& b) {
-        const vf32x4 zero = {0.0f, 0.0f, 0.0f, 0.0f};
-        return __builtin_amdgcn_mfma_scale_f32_16x16x128_f8f6f4(a.v, b.v, zero, 0, 0, 0, 0, 0, 0);
-    }
-};
-template <>
-struct Operand<true> {
+struct Operand {
     mf16x8 v[4];
     __device__ __forceinline__ void set(mi32x8 f) {
 #pragma unroll
@@ -253,7 +238,6 @@ __device__ __forceinline__ void store_y4(TO* p, vf32x4 v, int valid) {
 // products, bound by latency (1 x 27,278 x 64 fp32: 3.9 us), operands at any alignment.
 template <int MI, int NI, typename TO>
 __global__ __launch_bounds__(kBlock) void k_mm_direct(MmArgs p) {
-    constexpr bool WIDE = std::is_same<TO, float>::value;
     const int lane = threadIdx.x & 63, g = lane >> 4, i = lane & 15;
     const int64_t wave = (int64_t)blockIdx.x * (kBlock / 64) + (threadIdx.x >> 6);
     if (wave >= p.mt * p.nt) return;
@@ -272,7 +256,7 @@ __global__ __launch_bounds__(kBlock) void k_mm_direct(MmArgs p) {
     for (int j = 0; j < NI; ++j) br[j] = p.b + min(n0 + 16 * j + i, p.n - 1) * p.ldb;
     for (int kb = 0; kb < p.kb; ++kb) {
         const int c = kb * kScaleBlock + 32 * g;
-        Operand<WIDE> fb[NI];
+        Operand fb[NI];
         vf32x4 sb[NI];
 #pragma unroll
         for (int j = 0; j < NI; ++j) {
@@ -285,12 +269,12 @@ __global__ __launch_bounds__(kBlock) void k_mm_direct(MmArgs p) {
         }
 #pragma unroll
         for (int x = 0; x < MI; ++x) {
-            Operand<WIDE> fa;
+            Operand fa;
             fa.set(load_frag(ar[x], c, p.k));
             const float sa = p.sa[min(m0 + 16 * x + i, p.m - 1) * p.kb + kb];
 #pragma unroll
             for (int j = 0; j < NI; ++j) {
-                const vf32x4 d = Operand<WIDE>::product(fb[j], fa);
+                const vf32x4 d = Operand::product(fb[j], fa);
 #pragma unroll
                 for (int r = 0; r < 4; ++r) acc[x][j][r] = fmaf(sa * sb[j][r], d[r], acc[x][j][r]);
             }
@@ -320,8 +304,8 @@ __global__ __launch_bounds__(kBlock) void k_mm_direct(MmArgs p) {
 // operands' steps go straight from memory to LDS (16 bytes a lane), the next while this one is multiplied.
 // In LDS the 16-byte pieces of a row are permuted by the row (piece c at c ^ (row / 2 % 8)), so the 16
 // lanes that read a fragment touch all 64 banks; a lane's fragment is pieces g and g + 4 of its row, in
-// both operands alike.  8,192 x 4,096 x 4,096 with a scale per tile, bf16 out: 137 us, 2.0 PFLOP/s; its matrix
-// instructions alone take 103, its loads alone 96.
+// both operands alike.  8,192 x 4,096 x 4,096 with a scale per tile: bf16 out 236 us, 1.16 PFLOP/s, fp32 out 244;
+// bound by the fp16 matrix instructions (a library product of 8,192^3 in bf16 reaches 1.25).
 
 constexpr int kTile = 256, kTileThreads = 512, kTileWaves = kTileThreads / 64;
 constexpr int kTileMI = 4, kTileNI = 8;   // 16-row, 16-column tiles of a wave
@@ -368,7 +352,6 @@ __device__ __forceinline__ mi32x8 tile_frag(const uint8_t* lo_piece, const uint8
 
 template <typename TO, bool B_TILE>
 __global__ __launch_bounds__(kTileThreads, 2) void k_mm_tile(MmArgs p) {
-    constexpr bool WIDE = std::is_same<TO, float>::value;
     extern __shared__ __attribute__((aligned(16))) uint8_t tile_lds[];
     TileStage* st = reinterpret_cast<TileStage*>(tile_lds);   // [2]
     const int tid = threadIdx.x, lane = tid & 63, g = lane >> 4, i = lane & 15;
@@ -416,7 +399,7 @@ __global__ __launch_bounds__(kTileThreads, 2) void k_mm_tile(MmArgs p) {
             stage_rows(p.a, p.lda, p.m, m0, kb, next.a);
             stage_rows(p.b, p.ldb, p.n, n0, kb, next.b);
         }
-        Operand<WIDE> fa[kTileMI];
+        Operand fa[kTileMI];
         float sa[kTileMI];
 #pragma unroll
         for (int x = 0; x < kTileMI; ++x) {
@@ -424,61 +407,21 @@ __global__ __launch_bounds__(kTileThreads, 2) void k_mm_tile(MmArgs p) {
             sa[x] = s.sa[wm + 16 * x + i];
             if constexpr (B_TILE) sa[x] *= s.sb[wn];   // (the wave's 128 columns are one tile of b)
         }
-        auto b_frag = [&](int j) { return tile_frag(s.b + at_b + piece, s.b + at_b + (piece ^ 64), 16 * j); };
-        vf32x4 d[kTileMI], sb;
-        auto add = [&](int j) {
+        // (a column tile at a time: widened fragments leave no registers for more)
 #pragma unroll
-            for (int x = 0; x < kTileMI; ++x)
+        for (int j = 0; j < kTileNI; ++j) {
+            Operand fb;
+            fb.set(tile_frag(s.b + at_b + piece, s.b + at_b + (piece ^ 64), 16 * j));
+            vf32x4 sb = {0.0f, 0.0f, 0.0f, 0.0f};
+            if constexpr (!B_TILE) sb = *reinterpret_cast<const vf32x4*>(&s.sb[wn + 16 * j + 4 * g]);
+#pragma unroll
+            for (int x = 0; x < kTileMI; ++x) {
+                const vf32x4 d = Operand::product(fb, fa[x]);
 #pragma unroll
                 for (int r = 0; r < 4; ++r)
-                    acc[x][j][r] = fmaf(B_TILE ? sa[x] : sa[x] * sb[r], d[x][r], acc[x][j][r]);
-        };
-        auto scales = [&](int j) {
-            if constexpr (!B_TILE) sb = *reinterpret_cast<const vf32x4*>(&s.sb[wn + 16 * j + 4 * g]);
-        };
-        if constexpr (WIDE) {   // (widened fragments leave no registers for more than one column tile)
-#pragma unroll
-            for (int j = 0; j < kTileNI; ++j) {
-                Operand<WIDE> fb;
-                fb.set(b_frag(j));
-                vf32x4 t = {0.0f, 0.0f, 0.0f, 0.0f};
-                if constexpr (!B_TILE) t = *reinterpret_cast<const vf32x4*>(&s.sb[wn + 16 * j + 4 * g]);
-#pragma unroll
-                for (int x = 0; x < kTileMI; ++x) {
-                    const vf32x4 e = Operand<WIDE>::product(fb, fa[x]);
-#pragma unroll
-                    for (int r = 0; r < 4; ++r)
-                        acc[x][j][r] = fmaf(B_TILE ? sa[x] : sa[x] * t[r], e[r], acc[x][j][r]);
-                }
-                __builtin_amdgcn_sched_barrier(0);
+                    acc[x][j][r] = fmaf(B_TILE ? sa[x] : sa[x] * sb[r], d[r], acc[x][j][r]);
             }
-        } else {
-            // A column tile's products are scaled and added while the next one's are formed (an MFMA takes 32
-            // cycles, the instructions of one product 16 or 32), and the one after that is read.
-            mi32x8 ahead = b_frag(0);
-#pragma unroll
-            for (int j = 0; j < kTileNI; ++j) {
-                Operand<WIDE> fb;
-                fb.set(ahead);
-                if (j + 1 < kTileNI) ahead = b_frag(j + 1);
-                vf32x4 e[kTileMI];
-#pragma unroll
-                for (int x = 0; x < kTileMI; ++x) e[x] = Operand<WIDE>::product(fb, fa[x]);
-                if (j > 0) {
-                    add(j - 1);
-                    __builtin_amdgcn_sched_group_barrier(0x100, 2, 0);
-#pragma unroll
-                    for (int x = 0; x < kTileMI; ++x) {
-                        __builtin_amdgcn_sched_group_barrier(0x8, 1, 0);
-                        __builtin_amdgcn_sched_group_barrier(0x2, B_TILE ? 4 : 8, 0);
-                    }
-                }
-#pragma unroll
-                for (int x = 0; x < kTileMI; ++x) d[x] = e[x];
-                scales(j);
-                __builtin_amdgcn_sched_barrier(0);
-            }
-            add(kTileNI - 1);
+            __builtin_amdgcn_sched_barrier(0);
         }
         // (also after the last step, where nobody reads it: a branch here would draw the sums behind it and
         // hold all 32 products in registers)
@@ -512,7 +455,7 @@ __global__ __launch_bounds__(kTileThreads, 2) void k_mm_tile(MmArgs p) {
 // 128 bytes whatever the distance of the rows (8,192 x 27,278 fp32, rows 8 bytes off: 16-byte stores at
 // their own addresses took 100 us of 303).
 // Measured, 8,192 x 27,278 x 64: fp32 175 us (5.1 TB/s written; these stores alone, without a product, take
-// 162), bf16 105; rows on their lines (27,264) 167 and 89.
+// 162), bf16 95-102; rows on their lines (27,264) 167 and 90.
 
 constexpr int kShortRows = 32;
 constexpr int kShortWaves = kBlock / 64;
@@ -566,10 +509,8 @@ struct ShortRaw {
         }
     }
 };
-template <bool WIDE, int E>
-struct ShortOperand;
 template <int E>
-struct ShortOperand<true, E> {
+struct ShortOperand {
     mf16x8 v[E];
     template <bool EXACT>
     __device__ __forceinline__ void set(ShortRaw<E> raw, int g, int k) {
@@ -585,24 +526,6 @@ struct ShortOperand<true, E> {
 #pragma unroll
         for (int e = 0; e < E; ++e) d = __builtin_amdgcn_mfma_f32_16x16x32_f16(a.v[e], b.v[e], d, 0, 0, 0);
         return d;
-    }
-};
-template <int E>
-struct ShortOperand<false, E> {
-    mi32x8 v;
-    template <bool EXACT>
-    __device__ __forceinline__ void set(ShortRaw<E> raw, int g, int k) {
-        if constexpr (!EXACT) raw.settle(g, k);
-        v = mi32x8{0, 0, 0, 0, 0, 0, 0, 0};
-#pragma unroll
-        for (int e = 0; e < E; ++e) {
-            v[2 * e] = (int)raw.v[e].x;
-            v[2 * e + 1] = (int)raw.v[e].y;
-        }
-    }
-    __device__ __forceinline__ static vf32x4 product(const ShortOperand& a, const ShortOperand& b) {
-        const vf32x4 zero = {0.0f, 0.0f, 0.0f, 0.0f};
-        return __builtin_amdgcn_mfma_scale_f32_16x16x128_f8f6f4(a.v, b.v, zero, 0, 0, 0, 0, 0, 0);
     }
 };
 
@@ -625,7 +548,7 @@ constexpr int kShortCols = 512;   // most columns of a workgroup (four workgroup
 // EXACT: k = 32 E, no part passes a row's end
 template <int E, typename TO, bool EXACT>
 __global__ __launch_bounds__(kBlock, 4) void k_mm_short(MmArgs p, int cols, int unit) {
-    constexpr bool WIDE = std::is_same<TO, float>::value;
+    constexpr bool OwnLoop = sizeof(TO) == 2 && E < 4;   // (below)
     constexpr int S = (int)sizeof(TO), C = kLine / S;      // columns of a line
     constexpr int NX = kShortRows / 16, NJ = 2, Step = 16 * NJ;   // columns of a step: a line takes C / Step
     constexpr int kPitch = 2 * kLine + 16;
@@ -634,7 +557,7 @@ __global__ __launch_bounds__(kBlock, 4) void k_mm_short(MmArgs p, int cols, int 
     const int lane = threadIdx.x & 63, g = lane >> 4, i = lane & 15;
     const int wave = __builtin_amdgcn_readfirstlane((int)(threadIdx.x >> 6));
     // Parts of the same rows follow each other on one XCD: its writes stay close to each other, and its L2 holds
-    // the rows' operand (parts spread over the XCDs, rows first: 8,192 x 27,278 x 64 fp32 197 us, bf16 126)
+    // the rows' operand (parts spread over the XCDs, rows first: 8,192 x 27,278 x 64 fp32 197 us)
     const uint32_t parts = (uint32_t)((p.n + cols - 1) / cols), total = parts * (uint32_t)p.mt;
     const uint32_t at = (blockIdx.x & 7) * ((total + 7) / 8) + (blockIdx.x >> 3);
     if (at >= total) return;
@@ -659,7 +582,7 @@ __global__ __launch_bounds__(kBlock, 4) void k_mm_short(MmArgs p, int cols, int 
     auto off_of = [&](int64_t m) {
         return (int)(((uint64_t)(uintptr_t)p.y / S + (uint64_t)(m * p.ldy + c0)) & (C - 1));
     };
-    ShortOperand<WIDE, E> fa[NX];
+    ShortOperand<E> fa[NX];
     float sa[NX];
     int put[NX];        // the lane's place in a ring for its row and its columns
 #pragma unroll
@@ -692,7 +615,7 @@ __global__ __launch_bounds__(kBlock, 4) void k_mm_short(MmArgs p, int cols, int 
 #pragma unroll
         for (int h = n; h < n + C; h += Step) {
             if (decltype(ragged)::value && h >= width) continue;
-            ShortOperand<WIDE, E> fb[NJ];
+            ShortOperand<E> fb[NJ];
             vf32x4 y[NJ][NX];
 #pragma unroll
             for (int j = 0; j < NJ; ++j) fb[j].template set<EXACT>(raw[j], g, p.k);
@@ -703,7 +626,7 @@ __global__ __launch_bounds__(kBlock, 4) void k_mm_short(MmArgs p, int cols, int 
                 const vf32x4 bias = *reinterpret_cast<const vf32x4*>(&col_bias[h + 16 * j + 4 * g]);
 #pragma unroll
                 for (int x = 0; x < NX; ++x) {
-                    const vf32x4 d = ShortOperand<WIDE, E>::product(fb[j], fa[x]);
+                    const vf32x4 d = ShortOperand<E>::product(fb[j], fa[x]);
 #pragma unroll
                     for (int r = 0; r < 4; ++r) y[j][x][r] = fmaf(sa[x] * sb[r], d[r], bias[r]);
                 }
@@ -729,16 +652,17 @@ __global__ __launch_bounds__(kBlock, 4) void k_mm_short(MmArgs p, int cols, int 
                 ring + (8 * q + (lane >> 3)) * kPitch + ((n * S + 16 * piece) & (2 * kLine - 1)));
         asm volatile("" ::: "memory");
     };
-    // Turns from `whole` on to `rest` write whole lines of whole tiles of rows.  For 16-bit outputs they have a
-    // loop without a branch around its stores: those and the next columns' loads are then counted together, and a
-    // turn no longer waits for the stores of the one before (8,192 x 27,264 x 64 bf16: 133 -> 111 us).  fp32
-    // outputs write twice as much, and waiting keeps the operands' loads from queueing behind their stores (in
-    // that loop 8,192 x 27,278 x 128 took 206-212 us, so 202; with k = 64 180, so 182).
+    // Turns from `whole` on to `rest` write whole lines of whole tiles of rows.  For 16-bit outputs and k <= 64 they
+    // have a loop without a branch around its stores: those and the next columns' loads are then counted together,
+    // and a turn does not wait for the stores of the one before (8,192 x 27,278 bf16, k = 64: 101 us, so 106; k = 32:
+    // 92 and 97; fp16 97 and 100, 92 and 101).  With k = 128 its registers spill (151, so 143).  fp32 outputs write
+    // twice as much, and waiting keeps the operands' loads from queueing behind their stores (in that loop
+    // 8,192 x 27,278 x 128 took 206-212 us, so 202; with k = 64 180, so 182).
     const int whole = unit < kLine ? C : 0;
     const int rest = m0 + kShortRows <= p.m && width >= whole + C ? width / C * C : whole;
     const int end = width + (last ? C : 0);   // at a row's end a last turn without columns writes what is left
     for (int n = 0; n < end;) {
-        if (!WIDE && n == whole && rest > whole) {
+        if (OwnLoop && n == whole && rest > whole) {
             __builtin_amdgcn_s_waitcnt(0x0f70);   // vmcnt(0): nothing from before the loop counts in it
 #pragma unroll 1
             for (; n < rest; n += C) {
@@ -748,7 +672,7 @@ __global__ __launch_bounds__(kBlock, 4) void k_mm_short(MmArgs p, int cols, int 
             continue;
         }
         form(n, std::true_type());
-        if (WIDE && n >= whole && n < rest) {
+        if (!OwnLoop && n >= whole && n < rest) {
             store_lines(n);
         } else if (n >= lead) {
 #pragma unroll 1
@@ -816,8 +740,8 @@ static hipError_t mm_tile(MmArgs p, hipStream_t st) {
 }
 
 // Which kernel, and both sides of each choice (us):
-//   more than 64 tiles of 256 x 256, k > 128: k_mm_tile (2,304 x 2,304 x 1,024, 81 tiles: bf16 31, fp32 45, so 46 and
-//     58 by k_mm_direct; 2,048 x 2,048, 64 tiles: 28.6 and 44, so 28.5 and 29; 4,096 x 4,096 x 144: 22, so 24)
+//   more than 64 tiles of 256 x 256, k > 128: k_mm_tile (2,304 x 2,304 x 1,024, 81 tiles: fp32 45, so 58 by k_mm_direct;
+//     2,048 x 2,048, 64 tiles: 44, so 29; 4,096 x 4,096 x 144: 22, so 24)
 //   k <= 128 and 1,024 waves of 64 x 64: k_mm_short (4,096 x 4,096 x 64 fp32 15, so 36; 2,048 x 1,682: both 10.5)
 //   up to 16 rows: a tile a wave (8 x 4,096 x 4,096: 18, with 2 x 2 tiles 34, 4 x 4 70)
 //   1,024 waves of 64 x 64: 4 x 4 tiles a wave, else 2 x 2 (2,000 x 2,000 x 256 fp32 14 and 16.5;
