@@ -343,6 +343,13 @@ __device__ __forceinline__ void stage_tail(const uint8_t* q, int64_t ld, int64_t
             load_q16(q + min(r0 + 64 * i + t, rows - 1) * ld, c, k);
 }
 
+// A barrier behind which every wave may read what any wave has staged: a wave's loads to LDS are vector-memory
+// operations in flight, which the barrier alone does not wait for.
+__device__ __forceinline__ void staged_barrier() {
+    asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
+    __syncthreads();
+}
+
 // a fragment from its lane's two pieces, `rows` rows below the first
 __device__ __forceinline__ mi32x8 tile_frag(const uint8_t* lo_piece, const uint8_t* hi_piece, int rows) {
     const vu32x4 lo = *reinterpret_cast<const vu32x4*>(lo_piece + rows * kScaleBlock);
@@ -389,7 +396,7 @@ __global__ __launch_bounds__(kTileThreads, 2) void k_mm_tile(MmArgs p) {
         stage_rows(p.b, p.ldb, p.n, n0, 0, st[0].b);
     }
     (of_b ? st[0].sb : st[0].sa)[tid & (kTile - 1)] = sp[tail ? full : 0];
-    __syncthreads();
+    staged_barrier();
     for (int step = 0; step < p.kb; ++step) {
         const TileStage& s = st[step & 1];
         TileStage& next = st[step & 1 ^ 1];
@@ -426,7 +433,7 @@ __global__ __launch_bounds__(kTileThreads, 2) void k_mm_tile(MmArgs p) {
         // (also after the last step, where nobody reads it: a branch here would draw the sums behind it and
         // hold all 32 products in registers)
         (of_b ? next.sb : next.sa)[tid & (kTile - 1)] = scale;
-        __syncthreads();
+        staged_barrier();
     }
 #pragma unroll
     for (int j = 0; j < kTileNI; ++j) {
