@@ -233,6 +233,10 @@ int ncf_workspace_discard_counts(const ncf_shape_t* shape, int64_t max_batch, vo
  * Replaces Model.predict_on_batch output[0] (model.py:184-194). */
 int ncf_predict(const ncf_shape_t* shape, const ncf_model_t* model, const int32_t* users,
                 const int32_t* items, int64_t n, float* probs, void* ws, size_t ws_bytes, void* stream);
+/* The same forward, logits[n] = output/Sigmoid's input: what the sigmoid's float32 cannot tell apart (it is 1 from
+ * a logit of 17 on). */
+int ncf_predict_logits(const ncf_shape_t* shape, const ncf_model_t* model, const int32_t* users,
+                       const int32_t* items, int64_t n, float* logits, void* ws, size_t ws_bytes, void* stream);
 
 /* RankLayer (model.py:344-352): per group of `group` consecutive probs, the
  * stable descending order (ties: lower index first). rank_idx[n_groups*group]. */

@@ -184,11 +184,14 @@ bool use_layered(const ncf_shape_t& s, const ncf_hyper_t* h) {
 // forward only: the fused MFMA forward when the shape has it, else the generic per-sample kernel
 hipError_t launch_predict(const ncf_shape_t& s, const ncf_hyper_t* h, const ncf::WsLayout& L, void* ws,
                           const float* emb, const float* mlp, const int32_t* users, const int32_t* items,
-                          const float* labels, int64_t n, float* probs, ncf::IdSpace ids, int* nbce, hipStream_t st) {
-    if (use_fused(s, h)) return ncf::launch_fwd_fused(s, L, ws, emb, mlp, users, items, labels, n, probs, ids, nbce, st);
+                          const float* labels, int64_t n, float* probs, ncf::IdSpace ids, int* nbce, hipStream_t st,
+                          bool logit = false) {
+    if (use_fused(s, h))
+        return ncf::launch_fwd_fused(s, L, ws, emb, mlp, users, items, labels, n, probs, ids, nbce, st, logit);
     // shapes whose weights outgrow the fused kernels (config D): the layered GEMM forward
-    if (use_layered(s, h)) return ncf::launch_predict_layered(s, L, ws, emb, mlp, users, items, labels, n, probs, ids, nbce, st);
-    return ncf::launch_predict_generic(s, L, ws, emb, mlp, users, items, labels, n, probs, ids, nbce, st);
+    if (use_layered(s, h))
+        return ncf::launch_predict_layered(s, L, ws, emb, mlp, users, items, labels, n, probs, ids, nbce, st, logit);
+    return ncf::launch_predict_generic(s, L, ws, emb, mlp, users, items, labels, n, probs, ids, nbce, st, logit);
 }
 
 // Shapes the fused kernel does not hold: the layer-by-layer GEMM path when the dense weights
@@ -526,17 +529,25 @@ int ncf_workspace_discard_counts(const ncf_shape_t* s, int64_t max_batch, void* 
                      "counter clear");
 }
 
-int ncf_predict(const ncf_shape_t* s, const ncf_model_t* model, const int32_t* users, const int32_t* items,
-                int64_t n, float* probs, void* ws, size_t ws_bytes, void* stream) {
+static int predict(const ncf_shape_t* s, const ncf_model_t* model, const int32_t* users, const int32_t* items,
+                   int64_t n, float* out, void* ws, size_t ws_bytes, void* stream, bool logit, const char* name) {
     if (int r = check_shape(s)) return r;
     ncf::WsLayout L;
     if (int r = check_ws(*s, n, ws, ws_bytes, &L)) return r;
-    if (!model || !model->emb || !model->mlp || !users || !items || !probs)
+    if (!model || !model->emb || !model->mlp || !users || !items || !out)
         return fail(NCF_EINVAL, "NULL device pointer");
     int nbce = 0;
-    return hip_check(launch_predict(*s, nullptr, L, ws, model->emb, model->mlp, users, items, nullptr, n, probs,
-                                    ncf::table_ids(*s), &nbce, (hipStream_t)stream),
-                     "ncf_predict");
+    return hip_check(launch_predict(*s, nullptr, L, ws, model->emb, model->mlp, users, items, nullptr, n, out,
+                                    ncf::table_ids(*s), &nbce, (hipStream_t)stream, logit),
+                     name);
+}
+int ncf_predict(const ncf_shape_t* s, const ncf_model_t* model, const int32_t* users, const int32_t* items,
+                int64_t n, float* probs, void* ws, size_t ws_bytes, void* stream) {
+    return predict(s, model, users, items, n, probs, ws, ws_bytes, stream, false, "ncf_predict");
+}
+int ncf_predict_logits(const ncf_shape_t* s, const ncf_model_t* model, const int32_t* users, const int32_t* items,
+                       int64_t n, float* logits, void* ws, size_t ws_bytes, void* stream) {
+    return predict(s, model, users, items, n, logits, ws, ws_bytes, stream, true, "ncf_predict_logits");
 }
 
 int ncf_rank(const float* probs, int64_t n_groups, int32_t group, int32_t* rank_idx, void* stream) {

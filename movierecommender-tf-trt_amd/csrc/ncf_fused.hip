@@ -819,9 +819,10 @@ __global__ __launch_bounds__(kBlock, 1) void k_fb_fused(const float* __restrict_
 // pass of fit_generator, model.py:184-194, 329-333): the forward chain of k_fb_fused with no
 // staging, no masks and no backward.  LDS holds the dense weights only (WLDS floats), so two
 // workgroups share a CU; 128-sample tiles, persistent grid.  With labels: one Keras-BCE partial
-// per workgroup (fixed order: wave sums, then the 4 waves in order).
+// per workgroup (fixed order: wave sums, then the 4 waves in order).  LOGIT: probs takes the logits, not
+// their sigmoids.
 
-template <class S>
+template <class S, bool LOGIT = false>
 __global__ __launch_bounds__(kBlock, 2) void k_fwd_fused(const float* __restrict__ emb, const float* __restrict__ mlp,
                                                          const int32_t* __restrict__ users,
                                                          const int32_t* __restrict__ items,
@@ -985,7 +986,7 @@ __global__ __launch_bounds__(kBlock, 2) void k_fwd_fused(const float* __restrict
         const float z = (zp + __shfl_xor(zp, 32, 64)) + wl[S::SBO];
         const float p = 1.0f / (1.0f + expf(-z));
         if (h == 0 && inb) {
-            probs[si] = ok ? p : __int_as_float(0x7fc00000);
+            probs[si] = ok ? (LOGIT ? z : p) : __int_as_float(0x7fc00000);
             if (labels && ok) {
                 const float y = labels[si];
                 const float pc = fminf(fmaxf(p, eps), hi_clip);
@@ -1074,22 +1075,22 @@ hipError_t launch_fb_fused(const ncf_shape_t& s, const WsLayout& L, void* ws, co
 template <class S>
 static hipError_t launch_fwd_one(const float* emb, const float* mlp, const int32_t* users, const int32_t* items,
                                  const float* labels, int64_t n, IdSpace ids, float* probs, float* part_bce,
-                                 int* nbce, hipStream_t st) {
+                                 int* nbce, hipStream_t st, bool logit) {
     const int64_t niter = (n + 127) / 128;
     int grid = (int)(niter < 512 ? niter : 512);  // two workgroups per CU, persistent
     if (grid > kMaxSlabs) grid = kMaxSlabs;
-    launch(k_fwd_fused<S>, grid, kBlock, (size_t)S::WLDS * 4, st, emb, mlp, users, items, labels, n, ids, probs,
-           labels ? part_bce : nullptr);
+    launch(logit ? k_fwd_fused<S, true> : k_fwd_fused<S>, grid, kBlock, (size_t)S::WLDS * 4, st, emb, mlp, users,
+           items, labels, n, ids, probs, labels ? part_bce : nullptr);
     *nbce = labels ? grid : 0;
     return hipGetLastError();
 }
 
 hipError_t launch_fwd_fused(const ncf_shape_t& s, const WsLayout& L, void* ws, const float* emb, const float* mlp,
                             const int32_t* users, const int32_t* items, const float* labels, int64_t n,
-                            float* probs, IdSpace ids, int* nbce, hipStream_t st) {
+                            float* probs, IdSpace ids, int* nbce, hipStream_t st, bool logit) {
     float* part = at<float>(ws, L.part_bce);
 #define NCF_TRY(SH) \
-    if (matches<SH>(s)) return launch_fwd_one<SH>(emb, mlp, users, items, labels, n, ids, probs, part, nbce, st)
+    if (matches<SH>(s)) return launch_fwd_one<SH>(emb, mlp, users, items, labels, n, ids, probs, part, nbce, st, logit)
     NCF_TRY(ShapeC);
     NCF_TRY(ShapeB);
     NCF_TRY(ShapeR);

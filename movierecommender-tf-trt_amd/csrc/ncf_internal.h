@@ -793,7 +793,7 @@ bool unit_fill_fits(const ncf_shape_t& s, int64_t n, bool bf16, int64_t r1);
 // workgroup in ws part_bce (*nbce of them)
 hipError_t launch_fwd_fused(const ncf_shape_t& s, const WsLayout& L, void* ws, const float* emb, const float* mlp,
                             const int32_t* users, const int32_t* items, const float* labels, int64_t n,
-                            float* probs, IdSpace ids, int* nbce, hipStream_t st);
+                            float* probs, IdSpace ids, int* nbce, hipStream_t st, bool logit = false);
 // layer-by-layer path (ncf_layered.hip): hand-written fp32 MFMA kernels (k_lay_l1f, k_lay_mid,
 // k_lay_dw1, k_lay_l1b) for the shapes they hold (config D's widths); same outputs as
 // launch_fb_generic (probs, gs, part_bce, slabs).  Other shapes run the generic kernel.
@@ -826,11 +826,11 @@ bool laymid_supported(const ncf_shape_t& s);
 hipError_t launch_laymid(const ncf_shape_t& s, const float* mlp, const float* h1, const float* emb,
                          const float* labels, const int32_t* users, const int32_t* items, int64_t n, IdSpace ids,
                          float inv_batch, float* probs, float* dzo, float* g1, float* slabs, float* part_bce,
-                         int grid, hipStream_t st);
+                         int grid, hipStream_t st, bool logit = false);
 // (dzo nullptr: the forward half alone — probs, and with labels the BCE partials; predict / evaluate)
 hipError_t launch_predict_layered(const ncf_shape_t& s, const WsLayout& L, void* ws, const float* emb,
                                   const float* mlp, const int32_t* users, const int32_t* items, const float* labels,
-                                  int64_t n, float* probs, IdSpace ids, int* nbce, hipStream_t st);
+                                  int64_t n, float* probs, IdSpace ids, int* nbce, hipStream_t st, bool logit = false);
 
 // metrics / summaries
 hipError_t launch_group_metrics(const float* probs, const float* labels, int64_t n_groups, int group, int k,

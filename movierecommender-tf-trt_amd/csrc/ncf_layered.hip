@@ -35,7 +35,7 @@ bool layered_all_mfma(const ncf_shape_t& s) { return layered_supported(s); }
 // forward half of launch_fb_layered, so evaluation matches training's forward.
 hipError_t launch_predict_layered(const ncf_shape_t& s, const WsLayout& L, void* ws, const float* emb,
                                   const float* mlp, const int32_t* users, const int32_t* items, const float* labels,
-                                  int64_t n, float* probs, IdSpace ids, int* nbce, hipStream_t st) {
+                                  int64_t n, float* probs, IdSpace ids, int* nbce, hipStream_t st, bool logit) {
     if (!layered_supported(s) || n > L.max_batch) return hipErrorInvalidValue;
     const int nl = s.num_layers;
     float* act = at<float>(ws, L.act);
@@ -47,7 +47,7 @@ hipError_t launch_predict_layered(const ncf_shape_t& s, const WsLayout& L, void*
     const int64_t units = (n + 15) / 16;
     const int grid = (int)(units >= 8 * 512 ? 512 : (units + 7) / 8);
     e = launch_laymid(s, mlp, X[1], emb, labels, users, items, n, ids, 1.0f, probs, nullptr, nullptr, nullptr,
-                      at<float>(ws, L.part_bce), grid, st);
+                      at<float>(ws, L.part_bce), grid, st, logit);
     *nbce = labels ? grid : 0;
     return e;
 }

@@ -125,8 +125,8 @@ struct MidArgs {
 };
 
 // FWD: forward only (ncf_predict / ncf_evaluate): probabilities and, labels given, the BCE partial
-// of the workgroup; no gradients
-template <class S, bool FWD>
+// of the workgroup; no gradients.  LOGIT: probs takes the logits, not their sigmoids
+template <class S, bool FWD, bool LOGIT = false>
 __global__ __launch_bounds__(256, 1) void k_lay_mid(MidArgs a) {
     constexpr int L1 = S::L1, L2 = S::L2, L3 = S::L3, G = S::G, B1 = S::B1, B2 = S::B2, B3 = S::B3, GQ = S::GQ;
     extern __shared__ __attribute__((aligned(16))) float lds[];
@@ -307,7 +307,7 @@ __global__ __launch_bounds__(256, 1) void k_lay_mid(MidArgs a) {
         const float p = 1.0f / (1.0f + expf(-z));
         const float dz = ok && p >= eps && p <= hi_clip ? (p - y) * a.inv_batch : 0.0f;
         if (g == 0 && in) {
-            a.probs[s] = ok ? p : __int_as_float(0x7fc00000);
+            a.probs[s] = ok ? (LOGIT ? z : p) : __int_as_float(0x7fc00000);
             if constexpr (!FWD) a.dzo[s] = dz;
         }
         {
@@ -523,21 +523,21 @@ bool laymid_supported(const ncf_shape_t& s) {
 hipError_t launch_laymid(const ncf_shape_t& s, const float* mlp, const float* h1, const float* emb,
                          const float* labels, const int32_t* users, const int32_t* items, int64_t n, IdSpace ids,
                          float inv_batch, float* probs, float* dzo, float* g1, float* slabs, float* part_bce,
-                         int grid, hipStream_t st) {
+                         int grid, hipStream_t st, bool logit) {
     using S = MShapeD;
     const bool fwd = dzo == nullptr;
-    if (!laymid_supported(s) || grid < 1 || grid > kMaxSlabs || (!fwd && (!labels || !g1 || !slabs)))
+    if (!laymid_supported(s) || grid < 1 || grid > kMaxSlabs || (!fwd && (logit || !labels || !g1 || !slabs)))
         return hipErrorInvalidValue;
     static bool cfg = false;
     if (!cfg) {
-        for (const void* k : {(const void*)k_lay_mid<S, false>, (const void*)k_lay_mid<S, true>})
+        for (const void* k : {(const void*)k_lay_mid<S, false>, (const void*)k_lay_mid<S, true>, (const void*)k_lay_mid<S, true, true>})
             if (hipError_t e = hipFuncSetAttribute(k, hipFuncAttributeMaxDynamicSharedMemorySize, (int)S::LDS_BYTES))
                 return e;
         cfg = true;
     }
     MidArgs a{mlp, s.layer_off[2], s.layer_off[3], s.layer_off[0], s.layer_off[1] + s.layers[0] * s.layers[1], h1, emb,
               s.row_width, labels, users, items, n, ids, inv_batch, probs, dzo, g1, slabs, s.mlp_params, part_bce};
-    launch(fwd ? k_lay_mid<S, true> : k_lay_mid<S, false>, grid, 256, S::LDS_BYTES, st, a);
+    launch(logit ? k_lay_mid<S, true, true> : fwd ? k_lay_mid<S, true> : k_lay_mid<S, false>, grid, 256, S::LDS_BYTES, st, a);
     return hipGetLastError();
 }
 

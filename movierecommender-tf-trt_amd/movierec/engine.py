@@ -377,6 +377,22 @@ class NCFEngine(object):
                                     N.ptr(out), N.ptr(self.ws), self.ws_bytes, N.stream_handle(self.device)))
         return out
 
+    def predict_logits(self, users, items):
+        """The logits of pairs: ``predict`` before the sigmoid, which in float32 is 1 from 17 on (NaN for an
+        id outside the table)."""
+        u, i = self._ids(users), self._ids(items)
+        n = u.numel()
+        if i.numel() != n:
+            raise ValueError("%d users and %d items" % (n, i.numel()))
+        out = torch.empty(n, dtype=torch.float32, device=self.device)
+        if n == 0:
+            return out
+        self.flush()
+        self._ensure_ws(n)
+        N.check(N.lib().ncf_predict_logits(ctypes.byref(self.shape), ctypes.byref(self.model_s), N.ptr(u), N.ptr(i), n,
+                                           N.ptr(out), N.ptr(self.ws), self.ws_bytes, N.stream_handle(self.device)))
+        return out
+
     def rank(self, probs, group):
         probs = probs.reshape(-1).contiguous()
         if probs.numel() % group:   # RankLayer's reshape (-1, n+1) fails the same way in TF
@@ -491,11 +507,12 @@ class NCFEngine(object):
         the user's candidates (0 .. c - 1) of the teacher's best, ``teacher_logits`` (b, t) float32,
         ``teacher_lse`` (b,) its log-sum-exp over all c at this temperature or None
         (``catalogue.distill_loss``).  The loss is weight * temperature ** 2 times the mean divergence
-        of the student's softmax over its candidates; its gradient with respect to the logits enters
-        ``train_step`` as labels y = p - b c dz, whose cross-entropy has exactly that gradient (zero,
-        as Keras' clip has it, where p is within 1e-7 of 0 or 1).  The optimizer's step, deferred decay
-        and counters are the training step's; ``stats`` are not touched.  Returns the per-user losses
-        (b,) on the device (NaN, and no part in the step, for a user with an id outside the table)."""
+        of the softmax of the student's logits over its candidates; its gradient with respect to the logits
+        enters ``train_step`` as labels y = p - b c dz, whose cross-entropy has exactly that gradient (zero,
+        as Keras' clip has it, for a candidate whose p is within 1e-7 of 0 or 1: a logit beyond about 16).
+        The optimizer's step, deferred decay and counters are the training step's; ``stats`` are not
+        touched.  Returns the per-user losses (b,) on the device (NaN, and no part in the step, for a user
+        with an id outside the table or whose list holds a NaN)."""
         from . import catalogue
         if self.precision != "fp32":
             raise ValueError("distill_step needs precision='fp32': its labels stand for the fp32 forward's p")
@@ -511,12 +528,13 @@ class NCFEngine(object):
         if b == 0:
             return torch.empty(0, dtype=torch.float32, device=self.device)
         uv = ids.view(b, 1).expand(b, c).reshape(-1)
-        p = self.predict(uv, iv)
-        loss, dz = catalogue.distill_loss_grad(torch.logit(p).view(b, c), teacher_items, teacher_logits,
+        z = self.predict_logits(uv, iv)
+        p = torch.sigmoid(z)
+        loss, dz = catalogue.distill_loss_grad(z.view(b, c), teacher_items, teacher_logits,
                                                grad_loss=weight * temperature ** 2 / b, temperature=temperature,
                                                teacher_lse=teacher_lse)
         labels = torch.sub(p, dz.view(-1), alpha=float(b * c))
-        # an id outside the table: its user's whole list has no loss (NaN) and takes no part
+        # a user without a loss (NaN): its whole list takes no part
         labels = torch.where(torch.isnan(labels), p, labels)
         stats = self.stats
         self.stats = torch.zeros_like(stats)

@@ -500,7 +500,7 @@ class MovierecModel(object):
         b, c = items.shape
         for m in (self, teacher):
             m.model.engine.check_ids(users, items)
-        z = torch.logit(teacher.model.engine.predict(np.repeat(users, c), items.reshape(-1))).view(b, c)
+        z = teacher.model.engine.predict_logits(np.repeat(users, c), items.reshape(-1)).view(b, c)
         best, places = torch.topk(z, min(int(top), c, 1024), dim=1)
         loss = self.model.engine.distill_step(users, items, places, best.contiguous(), temperature=temperature,
                                               teacher_lse=torch.logsumexp(z / temperature, 1), weight=weight)
