@@ -608,7 +608,7 @@ typedef struct ncf_distill {
     float grad_loss_value;
     float* loss;                /* [rows] */
     double* state;
-    void* grad;                 /* [rows][v] of dtype, rows grad_ld apart */
+    void* grad;                 /* [rows][v] of dtype, rows grad_ld apart; not the logits' own memory */
     int64_t grad_ld;
 } ncf_distill_t;
 int ncf_distill_workspace_size(int64_t rows, int64_t v, size_t* bytes);

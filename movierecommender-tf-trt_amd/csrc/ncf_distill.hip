@@ -13,7 +13,11 @@
 //
 // The exponentials are fp32; their sums, the logarithms and everything of a list's length are 64 bits,
 // because the loss is a small difference of large logarithms and q0 of numbers near one.  Inside and
-// outside mass are summed apart, never by subtraction.
+// outside mass are summed apart, never by subtraction, both relative to the row's best logit; where that leaves
+// less than 2^-28 of the mass outside (the list leads by 19 t), it is formed again relative to its own best, so it
+// does not vanish however far the list leads.  With s_j = w_j / (its class's sum) the gradient outside is
+//     s_j ((sum q + q0) p0 - q0) / t = s_j (sum q - q0 r) / (1 + r) / t,   r = inside mass / outside mass,
+// and inside (s_j (sum q + q0) r / (1 + r) - q(j)) / t.
 //
 // The reference trains on labels alone (binary cross-entropy, movierec/model.py:213-214).
 
@@ -43,9 +47,9 @@ struct DistArgs {
     const float* ref;     // [rows] or NULL
     double inv_t;
     float c2;             // log2(e) / t
-    double2* sums;        // per chunk: mass outside and inside the list, relative to the chunk's max
-    float* tops;          // per chunk: its max
-    double* state;        // [rows][kState]: max, 1 / sum, c inside, c outside, ref
+    double2* sums;        // per chunk: mass outside and inside the list, each relative to its base
+    float2* tops;         // per chunk: these bases; -inf for no mass
+    double* state;        // [rows][kState]: bases outside and inside, factors outside and inside, ref
     float* loss;
     const float* gl;      // [rows] or NULL: gl_v
     float gl_v;
@@ -184,7 +188,57 @@ __device__ __forceinline__ void mark_list(const DistArgs& a, int64_t row, int fi
     __syncthreads();
 }
 
-// Max and masses of one chunk of a row.
+__device__ __forceinline__ float base_of(float m) { return m > -INFINITY ? m : 0.0f; }
+
+// The least mass outside, relative to the row's best logit, that is not formed again.  (A sum's relative error is
+// that of its weights on the average, 1.5 2^-23 z / ln 2 with z <= ln n + 19 < 42 then.)  A row that needs it is
+// read twice more (2,048 x 27,278 bf16, lists of 32 in every row 60 ahead: 145 us, so 62), others pay a comparison.
+// (A base for each class from the start: a pass over the list's bits for the maxima, 62 -> 97.)
+constexpr double kRestLeast = 0x1p-28;
+
+// A row's best logit, the bases of its masses outside and inside the list, and the masses.
+struct RowMass {
+    float top, base_out, base_in;
+    double out, in;
+};
+
+// f(item, logit) for those of v items that `bits` does not mark, a vector at a time: what a rare row needs once more.
+template <int NT, typename T, typename F>
+__device__ __forceinline__ void each_outside(const T* x, int v, const uint32_t* bits, F f) {
+    constexpr int V = Elem<T>::kVec;
+#pragma unroll 1
+    for (int o = V * (int)threadIdx.x; o < v; o += V * NT) {
+        Raw<V, T> raw;
+        if (o + V <= v) {
+            raw.v[0] = *reinterpret_cast<const typename Elem<T>::vec*>(x + o);
+        } else {
+#pragma unroll
+            for (int e = 0; e < V; ++e) raw.v[0][e] = o + e < v ? x[o + e] : (T)(-INFINITY);
+        }
+        const uint32_t b = bits[o >> 5] >> (o & 31);
+#pragma unroll
+        for (int e = 0; e < V; ++e)
+            if (o + e < v && !(b >> e & 1u)) f(o + e, (float)raw.v[0][e]);
+    }
+}
+// The mass outside relative to its own best logit.
+template <int NT, typename T>
+__device__ __forceinline__ void outside_again(const T* x, int v, const uint32_t* bits, float c2, float& base, double& sum,
+                                              BlockRed<NT>& red) {
+    float top = -INFINITY;
+    each_outside<NT>(x, v, bits, [&](int, float y) { top = fmaxf(top, y); });
+    const float b = base_of(block_max32(top, red));
+    double s = 0.0;
+    each_outside<NT>(x, v, bits, [&](int, float y) { s += (double)pow2((y - b) * c2); });
+    sum = block_sum64(s, red);
+    base = b;
+}
+// Whether a row (chunk) is such: most of it lies in the list.
+__device__ __forceinline__ bool little_outside(const DistArgs& a, double out, double in) {
+    return a.ref && out < kRestLeast && in != 0.0;
+}
+
+// Maxima and masses of one chunk of a row.
 template <typename T>
 __global__ __launch_bounds__(kDistThreads) void k_distill_sums(DistArgs a) {
     __shared__ BlockRed<kDistThreads> red;
@@ -201,7 +255,7 @@ __global__ __launch_bounds__(kDistThreads) void k_distill_sums(DistArgs a) {
 #pragma unroll
     for (int e = 0; e < kDistItems; ++e) m = fmaxf(m, x[e]);
     m = block_max32(m, red);
-    const float base = m > -INFINITY ? m : 0.0f;
+    float base = base_of(m);
     double out = 0.0, in = 0.0;
 #pragma unroll
     for (int j = 0; j < kDistItems / V; ++j) {
@@ -215,8 +269,11 @@ __global__ __launch_bounds__(kDistThreads) void k_distill_sums(DistArgs a) {
         }
     }
     block_sum64(out, in, red);
+    if (little_outside(a, out, in))
+        outside_again<kDistThreads>(static_cast<const T*>(a.x) + row * a.ld + first, min(a.v - first, kDistChunk), bits,
+                                    a.c2, base, out, red);
     if (threadIdx.x == 0) {
-        a.tops[blockIdx.x] = m;
+        a.tops[blockIdx.x] = make_float2(out != 0.0 ? base : -INFINITY, m);
         a.sums[blockIdx.x] = make_double2(out, in);
     }
 }
@@ -284,40 +341,65 @@ __device__ __forceinline__ ListSums list_sums(const DistArgs& a, int64_t row, co
     return l;
 }
 
-// What the gradient of a row needs.
+// What the gradient of a row needs: an item's is factor * exp2((x - base) c2) - q(item), each side of the list with
+// its own.  And for the loss what lies between the two sides.
 struct RowState {
-    float base;             // the largest logit
-    double inv_sum, c_in, c_out, ref;
+    float base_out, base_in;
+    double f_out, f_in, ref;
+    double way;     // (base_in - base_out) / t: 0, or positive where the mass outside has a base of its own
+    double less;    // inside mass / outside mass, its inverse where way > 0
+    bool rest;      // the mass outside is a class
+    bool dead;      // no logit left
 };
 
-// The state of a row from its max m, its masses outside and inside the list, and the list's sums.
-__device__ __forceinline__ RowState row_state(const DistArgs& a, float m, double out, double in, const ListSums& l) {
-    const double sum = out + in, q0 = 1.0 - l.q;
-    RowState st{m > -INFINITY ? m : 0.0f, 1.0 / sum, l.q, l.q, l.ref};
-    if (a.ref && q0 > 0.0 && !(out <= 0.0)) {
-        st.c_in = l.q + q0;
-        st.c_out = st.c_in - q0 * (sum / out);
+__device__ __forceinline__ RowState row_state(const DistArgs& a, const RowMass& m, const ListSums& l) {
+    RowState st{};
+    st.base_out = m.base_out;
+    st.base_in = m.base_in;
+    st.ref = l.ref;
+    st.dead = !(m.top > -INFINITY) && m.out + m.in == 0.0;   // (NaN logits: a NaN sum)
+    if (st.dead) {
+        st.ref = INFINITY;
+        return st;
     }
-    if (!(m > -INFINITY) && sum == 0.0) st = RowState{st.base, 0.0, 0.0, 0.0, INFINITY};   // (NaN logits: a NaN sum)
+    if (!a.ref) {   // one class, the one outside
+        st.f_out = st.f_in = 1.0 / m.out * l.q;
+        return st;
+    }
+    const double q0 = 1.0 - l.q;
+    st.rest = q0 > 0.0 && !(m.out <= 0.0);
+    st.way = ((double)m.base_in - (double)m.base_out) * a.inv_t;
+    const bool own = st.way > 0.0 || m.out == 0.0;
+    st.less = m.out == 0.0 ? 0.0 : own ? exp(-st.way) * (m.out / m.in) : m.in / m.out;
+    const double part = 1.0 / (1.0 + st.less), p0 = own ? st.less * part : part, p1 = own ? part : st.less * part;
+    const double c = st.rest ? l.q + q0 : l.q;
+    // (c p0 - q0 without its cancellation)
+    st.f_out = st.rest ? (own ? l.q * st.less - q0 : l.q - q0 * st.less) * part : c * p0;
+    st.f_out = m.out == 0.0 ? 0.0 : st.f_out / m.out;
+    st.f_in = m.in == 0.0 ? 0.0 : c * p1 / m.in;
     return st;
 }
 
 // Its loss, by one thread; and the state, for a gradient later.
-__device__ __forceinline__ void write_row(const DistArgs& a, int64_t row, const RowState& st, double out, double in,
+__device__ __forceinline__ void write_row(const DistArgs& a, int64_t row, const RowState& st, const RowMass& m,
                                           const ListSums& l) {
     // sum q (log q - log p) with log p = (x - base) / t - log sum
-    double loss = l.q_log_q - (l.q_z - l.q * ((double)st.base * a.inv_t)) + l.q * log(out + in);
-    const double q0 = 1.0 - l.q;
-    if (a.ref && q0 > 0.0 && !(out <= 0.0)) loss += q0 * (log1p(-l.q) + log1p(in / out));
+    const bool own = a.ref && (st.way > 0.0 || m.out == 0.0);
+    const double sum = (own ? m.in : m.out) * (1.0 + st.less);
+    double loss = l.q_log_q - (l.q_z - l.q * ((double)st.base_in * a.inv_t)) + l.q * log(sum);
+    if (st.rest) {   // q0 (log q0 - log p0)
+        const double log_p0 = own ? -(st.way + log(m.in / m.out) + log1p(st.less)) : -log1p(st.less);
+        loss += (1.0 - l.q) * (log1p(-l.q) - log_p0);
+    }
     if (a.state) {
         double* to = a.state + row * kState;
-        to[0] = st.base;
-        to[1] = st.inv_sum;
-        to[2] = st.c_in;
-        to[3] = st.c_out;
+        to[0] = st.base_out;
+        to[1] = st.base_in;
+        to[2] = st.f_out;
+        to[3] = st.f_in;
         to[4] = st.ref;
     }
-    a.loss[row] = st.inv_sum == 0.0 || (l.q == 0.0 && !a.ref) ? 0.0f : (float)loss;
+    a.loss[row] = st.dead || (l.q == 0.0 && !a.ref) ? 0.0f : (float)loss;
 }
 
 // The row's loss and what its gradient needs.
@@ -327,21 +409,24 @@ __global__ __launch_bounds__(kDistThreads) void k_distill_loss(DistArgs a) {
     const int64_t row = blockIdx.x;
     const T* x = static_cast<const T*>(a.x) + row * a.ld;
     const ListEntry entry = list_entry(a, row, x, threadIdx.x);
-    float m = -INFINITY;
-    for (int c = threadIdx.x; c < a.chunks; c += kDistThreads) m = fmaxf(m, a.tops[row * a.chunks + c]);
-    m = block_max32(m, red);
-    const float base = m > -INFINITY ? m : 0.0f;
-    double out = 0.0, in = 0.0;
+    float top = -INFINITY, top_out = -INFINITY;
     for (int c = threadIdx.x; c < a.chunks; c += kDistThreads) {
-        const float mc = a.tops[row * a.chunks + c];
-        const double f = mc > -INFINITY ? exp(((double)mc - (double)base) * a.inv_t) : 1.0;
-        const double2 s = a.sums[row * a.chunks + c];
-        out += s.x * f;
-        in += s.y * f;
+        const float2 t = a.tops[row * a.chunks + c];
+        top_out = fmaxf(top_out, t.x);
+        top = fmaxf(top, t.y);
     }
-    block_sum64(out, in, red);
+    top = block_max32(top, red);
+    top_out = block_max32(top_out, red);
+    RowMass m{top, base_of(top_out), base_of(top), 0.0, 0.0};
+    for (int c = threadIdx.x; c < a.chunks; c += kDistThreads) {
+        const float2 t = a.tops[row * a.chunks + c];
+        const double2 s = a.sums[row * a.chunks + c];
+        m.out += s.x * (t.x > -INFINITY ? exp(((double)t.x - (double)m.base_out) * a.inv_t) : 1.0);
+        m.in += s.y * (t.y > -INFINITY ? exp(((double)t.y - (double)m.base_in) * a.inv_t) : 1.0);
+    }
+    block_sum64(m.out, m.in, red);
     const ListSums sums = list_sums<kDistThreads>(a, row, x, entry, red);
-    if (threadIdx.x == 0) write_row(a, row, row_state(a, m, out, in, sums), out, in, sums);
+    if (threadIdx.x == 0) write_row(a, row, row_state(a, m, sums), m, sums);
 }
 
 // The list's q by item: a bit map, the marked items ahead of each of its words, and the q of each marked
@@ -437,9 +522,9 @@ __global__ __launch_bounds__(NT) void k_distill_grad(DistArgs a, int chunks) {
     Raw<EPT, T> raw;
     load_chunk<NT>(static_cast<const T*>(a.x) + row * a.ld + first, a.v - first, raw);
     const double* st = a.state + row * kState;
-    const float base = (float)st[0];
+    const float base_out = (float)st[0], base_in = (float)st[1];
     const double g = (double)(a.gl ? a.gl[row] : a.gl_v) * a.inv_t;
-    const float p_in = (float)(st[1] * st[2] * g), p_out = (float)(st[1] * st[3] * g);
+    const float p_out = (float)(st[2] * g), p_in = (float)(st[3] * g);
     mark_list<NT, WORDS>(a, row, first, l.bits);
     l.fill(a, row, first, st[4]);
     T* out = static_cast<T*>(a.grad) + row * a.grad_ld + first;
@@ -448,10 +533,16 @@ __global__ __launch_bounds__(NT) void k_distill_grad(DistArgs a, int chunks) {
 #pragma unroll
     for (int j = 0; j < EPT / V; ++j) {
         const int o = vec_at<T, NT>(j);
+        const uint32_t b = l.bits[o >> 5] >> (o & 31) & ((1u << V) - 1u);
         float w[V];
 #pragma unroll
-        for (int e = 0; e < V; ++e) w[e] = pow2((x[V * j + e] - base) * a.c2);
-        store_grad(out, o, a.v - first, w, l.bits[o >> 5] >> (o & 31), p_in, p_out, g, l);
+        for (int e = 0; e < V; ++e) w[e] = pow2((x[V * j + e] - base_out) * a.c2);
+        if (b != 0 && base_in != base_out) {
+#pragma unroll
+            for (int e = 0; e < V; ++e)
+                if (b >> e & 1u) w[e] = pow2((x[V * j + e] - base_in) * a.c2);
+        }
+        store_grad(out, o, a.v - first, w, b, p_in, p_out, g, l);
     }
 }
 
@@ -474,37 +565,48 @@ __global__ __launch_bounds__(NT, 4) void k_distill_row(DistArgs a) {
     load_chunk<NT>(px, a.v, raw);
     float x[EPT];
     to_floats(raw, x);
-    float m = -INFINITY;
+    RowMass m{};
+    m.top = -INFINITY;
 #pragma unroll
-    for (int e = 0; e < EPT; ++e) m = fmaxf(m, x[e]);
-    m = block_max32(m, red);
-    const float base = m > -INFINITY ? m : 0.0f;
-    double out = 0.0, in = 0.0;
+    for (int e = 0; e < EPT; ++e) m.top = fmaxf(m.top, x[e]);
+    m.top = block_max32(m.top, red);
+    m.base_out = m.base_in = base_of(m.top);
 #pragma unroll
     for (int j = 0; j < EPT / V; ++j) {
         const int o = vec_at<T, NT>(j);
         const uint32_t b = a.ref ? l.bits[o >> 5] >> (o & 31) & ((1u << V) - 1u) : 0u;
 #pragma unroll
         for (int e = 0; e < V; ++e) {
-            const float w = pow2((x[V * j + e] - base) * a.c2);
-            x[V * j + e] = w;
-            if (b == 0) out += (double)w;
+            x[V * j + e] = pow2((x[V * j + e] - m.base_in) * a.c2);
+            if (b == 0) m.out += (double)x[V * j + e];
         }
         if (b != 0) {
 #pragma unroll
             for (int e = 0; e < V; ++e) {
-                if (b >> e & 1u) in += (double)x[V * j + e];
-                else out += (double)x[V * j + e];
+                if (b >> e & 1u) m.in += (double)x[V * j + e];
+                else m.out += (double)x[V * j + e];
             }
         }
         __builtin_amdgcn_sched_barrier(0);   // (a vector at a time: registers for one)
     }
-    block_sum64(out, in, red);
-    const RowState st = row_state(a, m, out, in, sums);
-    if constexpr (GRAD) {
+    block_sum64(m.out, m.in, red);
+    const bool again = little_outside(a, m.out, m.in);
+    if (again) outside_again<NT>(px, a.v, l.bits, a.c2, m.base_out, m.out, red);
+    const RowState st = row_state(a, m, sums);
+    if (GRAD && again) {
         const double g = (double)(a.gl ? a.gl[row] : a.gl_v) * a.inv_t;
-        const float p_in = (float)(st.inv_sum * st.c_in * g), p_out = (float)(st.inv_sum * st.c_out * g);
-        const double q_g = st.inv_sum != 0.0 ? g : 0.0;   // (a row with no logit left has no gradient)
+        const float p_in = (float)(st.f_in * g), p_out = (float)(st.f_out * g);
+        T* to = static_cast<T*>(a.grad) + row * a.grad_ld;
+        each_outside<NT>(px, a.v, l.bits, [&](int o, float y) { to[o] = (T)(pow2((y - st.base_out) * a.c2) * p_out); });
+        for (int k = threadIdx.x; k < a.k; k += NT) {   // (entries that name one item write the same there)
+            const ListEntry e = list_entry(a, row, px, k);
+            if (e.item >= 0)
+                to[e.item] = (T)(pow2((e.x - st.base_in) * a.c2) * p_in - (float)(l.at((int)e.item) * g));
+        }
+    } else if constexpr (GRAD) {
+        const double g = (double)(a.gl ? a.gl[row] : a.gl_v) * a.inv_t;
+        const float p_in = (float)(st.f_in * g), p_out = (float)(st.f_out * g);
+        const double q_g = st.dead ? 0.0 : g;   // (a row with no logit left has no gradient)
         T* to = static_cast<T*>(a.grad) + row * a.grad_ld;
 #pragma unroll
         for (int j = 0; j < EPT / V; ++j) {
@@ -514,7 +616,7 @@ __global__ __launch_bounds__(NT, 4) void k_distill_row(DistArgs a) {
         }
     }
     // (the logarithms last: they and the row do not fit the registers together)
-    if (threadIdx.x == 0) write_row(a, row, st, out, in, sums);
+    if (threadIdx.x == 0) write_row(a, row, st, m, sums);
 }
 
 // The same for lists of up to 64 entries: the first wave holds the list, an entry a lane, and works on it
@@ -566,51 +668,58 @@ __global__ __launch_bounds__(NT, 4) void k_distill_row_wave(DistArgs a) {
     __builtin_amdgcn_sched_barrier(0);
     float x[EPT];
     to_floats(raw, x);
-    float m = -INFINITY;
+    RowMass m{};
+    m.top = -INFINITY;
 #pragma unroll
-    for (int e = 0; e < EPT; ++e) m = fmaxf(m, x[e]);
-    m = block_max32(m, red);
+    for (int e = 0; e < EPT; ++e) m.top = fmaxf(m.top, x[e]);
+    m.top = block_max32(m.top, red);
     __syncthreads();   // (and the list)
-    const float base = m > -INFINITY ? m : 0.0f;
-    double out = 0.0, in = 0.0;
+    m.base_out = m.base_in = base_of(m.top);
 #pragma unroll
     for (int j = 0; j < EPT / V; ++j) {
         const int o = vec_at<T, NT>(j);
         const uint32_t b = a.ref ? bits[o >> 5] >> (o & 31) & ((1u << V) - 1u) : 0u;
 #pragma unroll
         for (int e = 0; e < V; ++e) {
-            x[V * j + e] = pow2((x[V * j + e] - base) * a.c2);
-            if (b == 0) out += (double)x[V * j + e];
+            x[V * j + e] = pow2((x[V * j + e] - m.base_in) * a.c2);
+            if (b == 0) m.out += (double)x[V * j + e];
         }
         if (b != 0) {
 #pragma unroll
             for (int e = 0; e < V; ++e) {
-                if (b >> e & 1u) in += (double)x[V * j + e];
-                else out += (double)x[V * j + e];
+                if (b >> e & 1u) m.in += (double)x[V * j + e];
+                else m.out += (double)x[V * j + e];
             }
         }
         __builtin_amdgcn_sched_barrier(0);
     }
-    block_sum64(out, in, red);
-    const RowState st = row_state(a, m, out, in, list);
+    block_sum64(m.out, m.in, red);
+    const bool again = little_outside(a, m.out, m.in);
+    if (again) outside_again<NT>(px, a.v, bits, a.c2, m.base_out, m.out, red);
+    const RowState st = row_state(a, m, list);
     if constexpr (GRAD) {
         const double g = (double)(a.gl ? a.gl[row] : a.gl_v) * a.inv_t;
-        const float p_in = (float)(st.inv_sum * st.c_in * g), p_out = (float)(st.inv_sum * st.c_out * g);
+        const float p_in = (float)(st.f_in * g), p_out = (float)(st.f_out * g);
         T* to = static_cast<T*>(a.grad) + row * a.grad_ld;
+        if (again) {
+            each_outside<NT>(px, a.v, bits,
+                             [&](int o, float y) { to[o] = (T)(pow2((y - st.base_out) * a.c2) * p_out); });
+        } else {
 #pragma unroll
-        for (int j = 0; j < EPT / V; ++j) {
-            const int o = vec_at<T, NT>(j);
-            if (o + V <= a.v) {
-                typename Elem<T>::vec y;
+            for (int j = 0; j < EPT / V; ++j) {
+                const int o = vec_at<T, NT>(j);
+                if (o + V <= a.v) {
+                    typename Elem<T>::vec y;
 #pragma unroll
-                for (int e = 0; e < V; ++e) y[e] = (T)(x[V * j + e] * p_out);
-                *reinterpret_cast<typename Elem<T>::vec*>(to + o) = y;
-            } else {
+                    for (int e = 0; e < V; ++e) y[e] = (T)(x[V * j + e] * p_out);
+                    *reinterpret_cast<typename Elem<T>::vec*>(to + o) = y;
+                } else {
 #pragma unroll
-                for (int e = 0; e < V; ++e)
-                    if (o + e < a.v) to[o + e] = (T)(x[V * j + e] * p_out);
+                    for (int e = 0; e < V; ++e)
+                        if (o + e < a.v) to[o + e] = (T)(x[V * j + e] * p_out);
+                }
+                __builtin_amdgcn_sched_barrier(0);
             }
-            __builtin_amdgcn_sched_barrier(0);
         }
         // the list's items once more, when every wave's stores of the row have arrived
         asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
@@ -618,11 +727,11 @@ __global__ __launch_bounds__(NT, 4) void k_distill_row_wave(DistArgs a) {
         if (wave == 0 && entry.item >= 0) {
             double q = 0.0;   // of all entries that name the item, in their order
             for (int k = 0; k < a.k; ++k) q += list_at[k] == (int)entry.item ? list_q[k] : 0.0;
-            const float w = pow2((entry.x - base) * a.c2);
-            to[entry.item] = (T)(w * p_in - (float)(q * (st.inv_sum != 0.0 ? g : 0.0)));
+            const float w = pow2((entry.x - st.base_in) * a.c2);
+            to[entry.item] = (T)(w * p_in - (float)(q * (st.dead ? 0.0 : g)));
         }
     }
-    if (threadIdx.x == 0) write_row(a, row, st, out, in, list);
+    if (threadIdx.x == 0) write_row(a, row, st, m, list);
 }
 
 static DistArgs dist_args(const ncf_distill_t& c, void* ws) {
@@ -650,8 +759,8 @@ static DistArgs dist_args(const ncf_distill_t& c, void* ws) {
     a.sums = static_cast<double2*>(ws);
     if (ws) {
         const int64_t n = c.rows * a.chunks;
-        a.tops = reinterpret_cast<float*>(a.sums + n);
-        if (!a.state) a.state = reinterpret_cast<double*>(a.tops + n + (n & 1));
+        a.tops = reinterpret_cast<float2*>(a.sums + n);
+        if (!a.state) a.state = reinterpret_cast<double*>(a.tops + n);
     }
     return a;
 }
@@ -667,7 +776,7 @@ static bool by_row(int64_t v, int64_t k) { return v <= kRowMost || (v <= 2 * kRo
 size_t distill_workspace(int64_t rows, int v) {
     if (v <= kRowMost) return 0;
     const size_t n = (size_t)rows * ((v + kDistChunk - 1) / kDistChunk);
-    return n * sizeof(double2) + (n + (n & 1)) * sizeof(float) + (size_t)rows * kState * sizeof(double);
+    return n * (sizeof(double2) + sizeof(float2)) + (size_t)rows * kState * sizeof(double);
 }
 int64_t distill_blocks(int64_t rows, int v) {
     const int64_t c = (v + kDistChunk - 1) / kDistChunk;
