@@ -49,7 +49,7 @@ struct DistArgs {
     float c2;             // log2(e) / t
     double2* sums;        // per chunk: mass outside and inside the list, each relative to its base
     float2* tops;         // per chunk: these bases; -inf for no mass
-    double* state;        // [rows][kState]: bases outside and inside, factors outside and inside, ref
+    double* state;        // [rows][kState]: both bases (32 bits each), factors outside and inside, sum q, ref
     float* loss;
     const float* gl;      // [rows] or NULL: gl_v
     float gl_v;
@@ -393,10 +393,10 @@ __device__ __forceinline__ void write_row(const DistArgs& a, int64_t row, const 
     }
     if (a.state) {
         double* to = a.state + row * kState;
-        to[0] = st.base_out;
-        to[1] = st.base_in;
-        to[2] = st.f_out;
-        to[3] = st.f_in;
+        to[0] = __hiloint2double(__float_as_int(st.base_in), __float_as_int(st.base_out));
+        to[1] = st.f_out;
+        to[2] = st.f_in;
+        to[3] = l.q;
         to[4] = st.ref;
     }
     a.loss[row] = st.dead || (l.q == 0.0 && !a.ref) ? 0.0f : (float)loss;
@@ -429,22 +429,29 @@ __global__ __launch_bounds__(kDistThreads) void k_distill_loss(DistArgs a) {
     if (threadIdx.x == 0) write_row(a, row, row_state(a, m, sums), m, sums);
 }
 
-// The list's q by item: a bit map, the marked items ahead of each of its words, and the q of each marked
-// item in units of 2^-51 (integers: the sum of an item's entries does not depend on their order).
+// The list's q by item: a bit map, the marked items ahead of each of its words, and the q of each marked item as an
+// integer (the sum of an item's entries does not depend on their order), in units of 2^-51 times a power of two above
+// the whole list's q: that may be as large or small as the teacher's log-sum-exp makes it.
 template <int NT, int WORDS>
 struct ItemQ {
     uint32_t bits[WORDS];
     uint32_t before[WORDS];
     unsigned long long q[NCF_DISTILL_MAX_K];
     uint32_t wave[NT / 64];
+    int power;   // of that
 
     __device__ __forceinline__ uint32_t slot(int o) const {
         return before[o >> 5] + __popc(bits[o >> 5] & ((1u << (o & 31)) - 1u));
     }
-    __device__ __forceinline__ double at(int o) const { return (double)q[slot(o)] * 0x1p-51; }
+    __device__ __forceinline__ double at(int o) const { return ldexp((double)q[slot(o)], power - 51); }
+
+    // (no finite sum: c inside and outside the list are not finite either, and so is no gradient)
+    __device__ __forceinline__ static int power_of(double sum_q) {
+        return sum_q > 0.0 && sum_q < INFINITY ? ilogb(sum_q) + 1 : 0;
+    }
 
     // from the marked bits (mark_list)
-    __device__ __forceinline__ void fill(const DistArgs& a, int64_t row, int first, double ref) {
+    __device__ __forceinline__ void fill(const DistArgs& a, int64_t row, int first, double ref, double sum_q) {
         constexpr int W = (WORDS + NT - 1) / NT;
         const int lane = threadIdx.x & 63, w0 = W * (int)threadIdx.x;
         uint32_t n[W], mine = 0;
@@ -460,6 +467,7 @@ struct ItemQ {
             if (lane >= d) inc += o;
         }
         if (lane == 63) wave[threadIdx.x >> 6] = inc;
+        if (threadIdx.x == 0) power = power_of(sum_q);
         __syncthreads();
         uint32_t ahead = inc - mine, total = 0;
 #pragma unroll
@@ -477,9 +485,8 @@ struct ItemQ {
         for (int k = threadIdx.x; k < a.k; k += NT) {
             const int64_t i = list_item(a, row, k) - first;
             if (i < 0 || i >= 32 * WORDS || i + first >= a.v) continue;
-            // (no q of a log-sum-exp passes 1, up to its rounding; a NaN has made c inside and outside NaN)
-            const double e = exp((double)a.y[row * a.y_ld + k] * a.inv_t - ref);
-            atomicAdd(&q[slot((int)i)], (unsigned long long)rint(fmin(e, 2.0) * 0x1p51));
+            const double e = ldexp(exp((double)a.y[row * a.y_ld + k] * a.inv_t - ref), 51 - power_of(sum_q));
+            atomicAdd(&q[slot((int)i)], (unsigned long long)rint(fmin(e, 0x1p52)));
         }
         __syncthreads();
     }
@@ -522,11 +529,11 @@ __global__ __launch_bounds__(NT) void k_distill_grad(DistArgs a, int chunks) {
     Raw<EPT, T> raw;
     load_chunk<NT>(static_cast<const T*>(a.x) + row * a.ld + first, a.v - first, raw);
     const double* st = a.state + row * kState;
-    const float base_out = (float)st[0], base_in = (float)st[1];
+    const float base_out = __int_as_float(__double2loint(st[0])), base_in = __int_as_float(__double2hiint(st[0]));
     const double g = (double)(a.gl ? a.gl[row] : a.gl_v) * a.inv_t;
-    const float p_out = (float)(st[2] * g), p_in = (float)(st[3] * g);
+    const float p_out = (float)(st[1] * g), p_in = (float)(st[2] * g);
     mark_list<NT, WORDS>(a, row, first, l.bits);
-    l.fill(a, row, first, st[4]);
+    l.fill(a, row, first, st[4], st[3]);
     T* out = static_cast<T*>(a.grad) + row * a.grad_ld + first;
     float x[EPT];
     to_floats(raw, x);
@@ -559,7 +566,7 @@ __global__ __launch_bounds__(NT, 4) void k_distill_row(DistArgs a) {
     // reads meanwhile)
     const ListSums sums = list_sums<NT>(a, row, px, list_entry(a, row, px, threadIdx.x), red);
     if (GRAD || a.ref) mark_list<NT, WORDS>(a, row, 0, l.bits);
-    if constexpr (GRAD) l.fill(a, row, 0, sums.ref);
+    if constexpr (GRAD) l.fill(a, row, 0, sums.ref, sums.q);
     __builtin_amdgcn_sched_barrier(0);
     Raw<EPT, T> raw;
     load_chunk<NT>(px, a.v, raw);
