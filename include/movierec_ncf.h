@@ -603,7 +603,7 @@ typedef struct ncf_distill {
     const float* teacher_logits;
     int64_t k, items_ld, teacher_ld;
     const float* teacher_lse;   /* [rows] or NULL */
-    double temperature;         /* > 0 */
+    double temperature;         /* in [2^-100, 2^100] */
     const float* grad_loss;     /* [rows] or NULL: grad_loss_value */
     float grad_loss_value;
     float* loss;                /* [rows] */

@@ -1,7 +1,6 @@
 // C ABI entry points (include/movierec_ncf.h).  Host orchestration only:
 // argument validation, workspace carving and the launch sequence of each call.
 
-#include <cmath>
 #include <cstdarg>
 #include <cstdio>
 #include <cstdlib>
@@ -1592,8 +1591,8 @@ static int distill(const ncf_distill_t* d, void* ws, size_t ws_bytes, bool forwa
     if (int r = check_matrix("teacher_logits", d->teacher_logits, d->rows, d->k, d->teacher_ld)) return r;
     if (d->k > NCF_DISTILL_MAX_K)
         return fail(NCF_EINVAL, "k must be in [1, %d], got %lld", NCF_DISTILL_MAX_K, (long long)d->k);
-    if (!(d->temperature > 0.0) || std::isinf(d->temperature))
-        return fail(NCF_EINVAL, "temperature must be positive and finite, got %g", d->temperature);
+    if (!(d->temperature >= 0x1p-100 && d->temperature <= 0x1p100))   // (log2(e) / t is a factor of float32s)
+        return fail(NCF_EINVAL, "temperature must be in [2^-100, 2^100], got %g", d->temperature);
     if ((!d->state && forward != backward) || (forward && !d->loss)) return fail(NCF_EINVAL, "NULL device pointer");
     size_t need = 0;
     if (int r = ncf_distill_workspace_size(d->rows, d->v, &need)) return r;

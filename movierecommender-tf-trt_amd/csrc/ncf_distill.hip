@@ -278,10 +278,17 @@ __global__ __launch_bounds__(kDistThreads) void k_distill_sums(DistArgs a) {
     }
 }
 
-// What depends on a row's list alone: the teacher's reference, sum q, sum q log q and sum q x / t.
+// What depends on a row's list alone: the teacher's reference, sum q, sum q log q and sum q x.
 struct ListSums {
-    double ref, q, q_log_q, q_z;
+    double ref, q, q_log_q, q_x;
 };
+
+// y / t, rounded: fused into a later subtraction it would no longer equal itself (where y / t is large, a best entry's
+// q would be e to the half step that its own reference was rounded by)
+__device__ __forceinline__ double list_z(float y, double inv_t) {
+#pragma clang fp contract(off)
+    return (double)y * inv_t;
+}
 
 // A thread's first entry of the list, loaded ahead of the row.
 struct ListEntry {
@@ -296,7 +303,7 @@ __device__ __forceinline__ ListEntry list_entry(const DistArgs& a, int64_t row, 
         const int64_t i = list_item(a, row, k);
         if (i >= 0 && i < a.v) {
             e.item = i;
-            e.z = (double)a.y[row * a.y_ld + k] * a.inv_t;
+            e.z = list_z(a.y[row * a.y_ld + k], a.inv_t);
             e.x = (float)x[i];
         }
     }
@@ -333,11 +340,11 @@ __device__ __forceinline__ ListSums list_sums(const DistArgs& a, int64_t row, co
         l.q += q;
         if (q != 0.0) {
             l.q_log_q += q * lq;
-            l.q_z += q * ((double)e.x * a.inv_t);
+            l.q_x += q * (double)e.x;
         }
     });
     block_sum64(l.q, l.q_log_q, red);
-    l.q_z = block_sum64(l.q_z, red);
+    l.q_x = block_sum64(l.q_x, red);
     return l;
 }
 
@@ -386,7 +393,7 @@ __device__ __forceinline__ void write_row(const DistArgs& a, int64_t row, const 
     // sum q (log q - log p) with log p = (x - base) / t - log sum
     const bool own = a.ref && (st.way > 0.0 || m.out == 0.0);
     const double sum = (own ? m.in : m.out) * (1.0 + st.less);
-    double loss = l.q_log_q - (l.q_z - l.q * ((double)st.base_in * a.inv_t)) + l.q * log(sum);
+    double loss = l.q_log_q - (l.q_x - l.q * (double)st.base_in) * a.inv_t + l.q * log(sum);
     if (st.rest) {   // q0 (log q0 - log p0)
         const double log_p0 = own ? -(st.way + log(m.in / m.out) + log1p(st.less)) : -log1p(st.less);
         loss += (1.0 - l.q) * (log1p(-l.q) - log_p0);
@@ -485,7 +492,7 @@ struct ItemQ {
         for (int k = threadIdx.x; k < a.k; k += NT) {
             const int64_t i = list_item(a, row, k) - first;
             if (i < 0 || i >= 32 * WORDS || i + first >= a.v) continue;
-            const double e = ldexp(exp((double)a.y[row * a.y_ld + k] * a.inv_t - ref), 51 - power_of(sum_q));
+            const double e = ldexp(exp(list_z(a.y[row * a.y_ld + k], a.inv_t) - ref), 51 - power_of(sum_q));
             atomicAdd(&q[slot((int)i)], (unsigned long long)rint(fmin(e, 0x1p52)));
         }
         __syncthreads();
@@ -667,7 +674,7 @@ __global__ __launch_bounds__(NT, 4) void k_distill_row_wave(DistArgs a) {
         const double lq = entry.z - l.ref, q = in ? exp(lq) : 0.0;
         l.q = wave_sum64(q);
         l.q_log_q = wave_sum64(q != 0.0 ? q * lq : 0.0);
-        l.q_z = wave_sum64(q != 0.0 ? q * ((double)entry.x * a.inv_t) : 0.0);
+        l.q_x = wave_sum64(q != 0.0 ? q * (double)entry.x : 0.0);
         list_q[lane] = q;
         list_at[lane] = in ? (int)entry.item : -1;
         if (lane == 0) list = l;

@@ -210,8 +210,8 @@ def _distill(logits, teacher_items, teacher_logits, temperature, teacher_lse):
                          % (tuple(teacher_items.shape), teacher_logits.dtype, tuple(teacher_logits.shape)))
     if teacher_lse is not None:
         d.teacher_lse = _dense("teacher_lse", teacher_lse, (d.rows,), torch.float32, dev).data_ptr()
-    if not 0 < temperature < math.inf:
-        raise ValueError("temperature must be positive and finite, got %r" % (temperature,))
+    if not 2.0 ** -100 <= temperature <= 2.0 ** 100:
+        raise ValueError("temperature must be in [2^-100, 2^100], got %r" % (temperature,))
     d.temperature = temperature
     d.logits, d.teacher_items, d.teacher_logits = logits.data_ptr(), teacher_items.data_ptr(), teacher_logits.data_ptr()
     d.items64 = 1 if teacher_items.dtype == torch.int64 else 0
@@ -239,7 +239,7 @@ def distill_loss(logits, teacher_items, teacher_logits, temperature=1.0, teacher
     loss = sum q (log q - log p[items]).  ``teacher_lse`` (rows,) float32, the teacher's
     logsumexp(logits / temperature) over its whole catalogue, makes q the teacher's probabilities
     and adds the mass outside the list as one more class.  A row without an entry, or whose logits
-    are all -inf, has loss 0.  (Gradients by soft targets usually carry a factor temperature ** 2:
+    are all -inf, has loss 0.  ``temperature`` is in [2^-100, 2^100].  (Gradients by soft targets usually carry a factor temperature ** 2:
     pass it in ``grad_loss``.)"""
     d = _distill(logits, teacher_items, teacher_logits, temperature, teacher_lse)
     dev = logits.device
