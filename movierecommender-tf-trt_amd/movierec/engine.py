@@ -448,7 +448,7 @@ class NCFEngine(object):
         gives a row of NaN.  precision "fp16" (4-layer models of ``score_topk``'s MFMA scorer), "fp8"
         (GMF-only models: the product of their factors in 8 bits with block scales,
         ``catalogue.matmul_blocks``), "fp32" (any shape, slow); None: the first of these that the
-        shape has."""
+        shape has.  (``sample_items`` takes 8 bits only when asked to.)"""
         codes = {"fp16": N.NCF_SCORE_FP16, "fp8": N.NCF_SCORE_FP8, "fp32": N.NCF_SCORE_FP32}
         L = N.lib()
         if precision is None:
@@ -475,8 +475,13 @@ class NCFEngine(object):
         """Items drawn for ``users`` from the softmax of their logits over the catalogue, by the uniform
         numbers ``u`` (n,) or (n, draws) on the device: ``catalogue.sample_items`` on ``score_logits``,
         for as many users at a time as 1 GiB of logits holds.  Settings as there; one per user as a
-        tensor.  Returns (items int32, probabilities float32) of u's shape."""
+        tensor.  ``precision`` as there, but None takes "fp16" or else "fp32", the logits that
+        ``score_topk`` ranks by: 8 bits can name another best item, so a caller asks for them.  Returns
+        (items int32, probabilities float32) of u's shape."""
         from . import catalogue
+        if precision is None:
+            fast = N.lib().ncf_score_supported(ctypes.byref(self.shape), N.NCF_SCORE_FP16)
+            precision = "fp16" if fast else "fp32"
         ids = self._ids(users)
         n = ids.numel()
         if not torch.is_tensor(u) or u.dim() not in (1, 2) or u.shape[0] != n:

@@ -466,8 +466,10 @@ class MovierecModel(object):
         (0: all), of them the shortest leading list with ``top_p`` of the weight
         exp(logit / temperature), without items of less than ``min_p`` of the best one's weight.
         ``mask`` (n, num_items) or (num_items,): False items, such as seen ones, are never drawn.  The
-        uniform numbers come from numpy's generator with ``seed``.  Returns numpy ``(items (n, draws)
-        int32, probabilities (n, draws) float32)``; item -1 where the mask leaves nothing."""
+        uniform numbers come from numpy's generator with ``seed``.  ``precision`` None: that of the logits
+        :meth:`recommend` ranks by ("fp16" where the model has that scorer, else "fp32"); "fp8" for GMF-only
+        models: faster, on 8-bit factors.  Returns numpy ``(items (n, draws) int32, probabilities (n, draws)
+        float32)``; item -1 where the mask leaves nothing."""
         import torch
         user_ids = np.asarray(user_ids).reshape(-1)
         if user_ids.size and (user_ids.min() < 0 or user_ids.max() >= self._num_users):

@@ -1,8 +1,10 @@
 """Calls of the catalogue operators at the edge of what they take: every one is served or refused by a ValueError."""
 
+import numpy as np
 import pytest
 
 from conftest import gpu_available
+from oracle import ncf_oracle as O
 
 pytestmark = pytest.mark.gpu
 
@@ -10,6 +12,8 @@ if gpu_available():
     import torch
     from movierec import catalogue as C
     from test_catalogue_distill_gpu import both, problem
+    from test_catalogue_model_gpu import gmf_weights, model
+    from test_score_gpu import _engine
 
 
 @pytest.mark.parametrize("v", [60, 9000, 40000])
@@ -26,3 +30,18 @@ def test_distillation_at_extreme_temperatures(v):
     for t in (1e-39, 5e-324, 1e39, 1e300):
         with pytest.raises(ValueError):
             C.distill_loss(x, items, y, temperature=t)
+
+
+def test_draws_rank_by_the_logits_that_the_ranking_uses(tmp_path):
+    """Models without the MFMA scorer draw from fp32 logits unless the caller asks for fewer bits."""
+    shape = O.NCFShape(50, 2000, [], 64)
+    eng = _engine(shape, gmf_weights(shape, 5))
+    users, u = np.arange(50, dtype=np.int32), torch.zeros(50, device="cuda")
+    best = eng.score_topk(users, k=1, precision="fp32")[0].view(-1)
+    assert torch.equal(eng.sample_items(users, u, temperature=0.0)[0], best)
+    eight = eng.score_logits(users, precision="fp8").argmax(1)
+    assert not torch.equal(eight.int(), best)         # (8 bits name another for some users)
+    assert torch.equal(eng.sample_items(users, u, temperature=0.0, precision="fp8")[0], eight.int())
+    m = model(tmp_path, "g", layers=(), gmf=64, seed=4)
+    np.testing.assert_array_equal(m.recommend_sampled(np.arange(50), temperature=0.0)[0],
+                                  m.recommend(np.arange(50), k=1, precision="fp32")[0])
