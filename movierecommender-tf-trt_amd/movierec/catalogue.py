@@ -135,6 +135,26 @@ def _setting(name, value, rows, dtype, device, low, high):
     return value, None
 
 
+def check_draw(rows, n, device, temperature=1.0, top_k=0, top_p=1.0, min_p=0.0, mask=None):
+    """Checks the settings and the mask of a draw from (rows, n) logits on ``device``; returns
+    :func:`sample_items`' argument struct with them filled in."""
+    d = N.NcfDraw()
+    d.temperature, d.temperature_rows = _setting("temperature", temperature, rows, torch.float32, device, 0, math.inf)
+    d.top_k, d.top_k_rows = _setting("top_k", top_k, rows, torch.int32, device, 0, 2 ** 62)
+    d.top_p, d.top_p_rows = _setting("top_p", top_p, rows, torch.float32, device, 0, 1)
+    d.min_p, d.min_p_rows = _setting("min_p", min_p, rows, torch.float32, device, 0, 1)
+    if mask is not None:
+        if not torch.is_tensor(mask) or mask.dtype not in (torch.bool, torch.uint8):
+            raise ValueError("mask must be a bool or uint8 tensor")
+        if tuple(mask.shape) == (n,):
+            mask = mask.expand(rows, n)
+        if tuple(mask.shape) != (rows, n):
+            raise ValueError("mask must have shape (%d, %d) or (%d,), got %s" % (rows, n, n, tuple(mask.shape)))
+        d.mask_ld = _matrix("mask", mask, device)
+        d.mask = mask.data_ptr()
+    return d
+
+
 def sample_items(logits, u, temperature=1.0, top_k=0, top_p=1.0, min_p=0.0, mask=None):
     """Draws items from ``logits`` (rows, n; float32, bfloat16 or float16) by the given uniform numbers
     ``u`` (rows,) or (rows, draws), float32 or float64 in [0, 1): ``(items, probs)`` of u's shape, int32
@@ -152,8 +172,7 @@ def sample_items(logits, u, temperature=1.0, top_k=0, top_p=1.0, min_p=0.0, mask
     ld = _matrix("logits", logits)
     dev = logits.device
     rows, n = logits.shape
-    d = N.NcfDraw()
-    d.dtype = _dtype_code("logits", logits.dtype)
+    code = _dtype_code("logits", logits.dtype)
     if n < 1:
         raise ValueError("logits has no columns")
     if not torch.is_tensor(u) or u.dim() not in (1, 2) or u.shape[0] != rows:
@@ -161,19 +180,8 @@ def sample_items(logits, u, temperature=1.0, top_k=0, top_p=1.0, min_p=0.0, mask
     if u.dtype not in (torch.float32, torch.float64):
         raise ValueError("u must be float32 or float64, got %s" % u.dtype)
     _dense("u", u, u.shape, u.dtype, dev)
-    d.temperature, d.temperature_rows = _setting("temperature", temperature, rows, torch.float32, dev, 0, math.inf)
-    d.top_k, d.top_k_rows = _setting("top_k", top_k, rows, torch.int32, dev, 0, 2 ** 62)
-    d.top_p, d.top_p_rows = _setting("top_p", top_p, rows, torch.float32, dev, 0, 1)
-    d.min_p, d.min_p_rows = _setting("min_p", min_p, rows, torch.float32, dev, 0, 1)
-    if mask is not None:
-        if not torch.is_tensor(mask) or mask.dtype not in (torch.bool, torch.uint8):
-            raise ValueError("mask must be a bool or uint8 tensor")
-        if tuple(mask.shape) == (n,):
-            mask = mask.expand(rows, n)
-        if tuple(mask.shape) != (rows, n):
-            raise ValueError("mask must have shape (%d, %d) or (%d,), got %s" % (rows, n, n, tuple(mask.shape)))
-        d.mask_ld = _matrix("mask", mask, dev)
-        d.mask = mask.data_ptr()
+    d = check_draw(rows, n, dev, temperature, top_k, top_p, min_p, mask)
+    d.dtype = code
     items = torch.empty(u.shape, dtype=torch.int32, device=dev)
     probs = torch.empty(u.shape, dtype=torch.float32, device=dev)
     d.draws = 1 if u.dim() == 1 else u.shape[1]

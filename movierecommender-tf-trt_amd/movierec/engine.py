@@ -486,22 +486,18 @@ class NCFEngine(object):
         n = ids.numel()
         if not torch.is_tensor(u) or u.dim() not in (1, 2) or u.shape[0] != n:
             raise ValueError("u must have shape (%d,) or (%d, draws)" % (n, n))
-        if mask is not None and not torch.is_tensor(mask):
-            raise ValueError("mask must be a bool or uint8 tensor")
-        step = max(1, SAMPLE_LOGITS // self.num_items)
         settings = dict(temperature=temperature, top_k=top_k, top_p=top_p, min_p=min_p)
+        # the whole call's shapes, before it is cut into parts
+        catalogue.check_draw(n, self.num_items, self.device, mask=mask, **settings)
+        step = max(1, SAMPLE_LOGITS // self.num_items)
         items = torch.empty(u.shape, dtype=torch.int32, device=self.device)
         probs = torch.empty(u.shape, dtype=torch.float32, device=self.device)
-
-        def part(x, rows):
-            return x[rows] if torch.is_tensor(x) and x.shape and x.shape[0] == n else x
-
         for i in range(0, n, step):
             rows = slice(i, min(n, i + step))
             m = mask if mask is None or mask.dim() == 1 else mask[rows]
             items[rows], probs[rows] = catalogue.sample_items(
                 self.score_logits(ids[rows], precision), u[rows], mask=m,
-                **{name: part(x, rows) for name, x in settings.items()})
+                **{name: x[rows] if torch.is_tensor(x) else x for name, x in settings.items()})
         return items, probs
 
     def distill_step(self, users, items, teacher_items, teacher_logits, temperature=1.0, teacher_lse=None, k=1,

@@ -11,9 +11,10 @@ pytestmark = pytest.mark.gpu
 if gpu_available():
     import torch
     from movierec import catalogue as C
+    from movierec import engine as engine_module
     from test_catalogue_distill_gpu import both, problem
     from test_catalogue_model_gpu import gmf_weights, model
-    from test_score_gpu import _engine
+    from test_score_gpu import _engine, _weights
 
 
 @pytest.mark.parametrize("v", [60, 9000, 40000])
@@ -45,3 +46,25 @@ def test_draws_rank_by_the_logits_that_the_ranking_uses(tmp_path):
     m = model(tmp_path, "g", layers=(), gmf=64, seed=4)
     np.testing.assert_array_equal(m.recommend_sampled(np.arange(50), temperature=0.0)[0],
                                   m.recommend(np.arange(50), k=1, precision="fp32")[0])
+
+
+def test_masks_and_settings_belong_to_the_users_asked_for(monkeypatch):
+    shape = O.NCFShape(64, 700, [64, 32, 16, 8], 8)
+    eng = _engine(shape, _weights(shape, 8))
+    users, u = np.arange(20, dtype=np.int32), torch.rand(20, 4, device="cuda")
+    mask = torch.ones(64, 700, dtype=torch.bool, device="cuda")
+    t = torch.ones(64, device="cuda")
+    for part in (20, 7, 1):                           # users at a time
+        monkeypatch.setattr(engine_module, "SAMPLE_LOGITS", part * 700)
+        bad = [dict(mask=mask), dict(mask=mask[:21]), dict(mask=mask[:19]), dict(mask=mask[:1]), dict(mask=mask[:7]),
+               dict(mask=mask[:20, :699]), dict(mask=mask[0, :20]), dict(mask=mask[:20].float()),
+               dict(temperature=t), dict(temperature=t[:7]), dict(temperature=t[:6]), dict(temperature=t[:1]),
+               dict(temperature=t[0]), dict(top_k=t[:7].int()), dict(top_p=t[:21]), dict(min_p=t[:20].view(20, 1))]
+        for kw in bad:
+            with pytest.raises(ValueError):
+                eng.sample_items(users, u, **kw)
+        items, probs = eng.sample_items(users, u, mask=mask[:20], temperature=t[:20])
+        assert (items >= 0).all() and items.shape == (20, 4)
+    for kw in (dict(mask=mask[:1]), dict(temperature=t[:1]), dict(top_p=2.0)):   # (no user: still checked)
+        with pytest.raises(ValueError):
+            eng.sample_items(users[:0], u[:0], **kw)
