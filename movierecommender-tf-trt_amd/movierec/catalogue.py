@@ -16,6 +16,7 @@ The reference scores a list of items for one user and keeps the best (movierec/t
 
 import ctypes
 import math
+import numbers
 
 import torch
 
@@ -126,11 +127,18 @@ def matmul_blocks(a, a_scale, b, b_scale, bias=None, out_dtype=torch.float32):
     return y
 
 
+def _number(name, value, whole=False):
+    if type(value) is not int and (whole or type(value) is not float):
+        if not isinstance(value, numbers.Integral if whole else numbers.Real):
+            raise ValueError("%s must be %s, got %r" % (name, "an integer" if whole else "a number", value))
+    return value
+
+
 def _setting(name, value, rows, dtype, device, low, high):
     """One number for all rows, or a tensor with one per row: (number, address or None)."""
     if torch.is_tensor(value):
         return 0, _dense(name, value, (rows,), dtype, device).data_ptr()
-    if not low <= value <= high:   # (a NaN fails too)
+    if not low <= _number(name, value, dtype is torch.int32) <= high:   # (a NaN fails too)
         raise ValueError("%s must be in [%g, %g], got %r" % (name, low, high, value))
     return value, None
 
@@ -218,7 +226,7 @@ def _distill(logits, teacher_items, teacher_logits, temperature, teacher_lse):
                          % (tuple(teacher_items.shape), teacher_logits.dtype, tuple(teacher_logits.shape)))
     if teacher_lse is not None:
         d.teacher_lse = _dense("teacher_lse", teacher_lse, (d.rows,), torch.float32, dev).data_ptr()
-    if not 2.0 ** -100 <= temperature <= 2.0 ** 100:
+    if not 2.0 ** -100 <= _number("temperature", temperature) <= 2.0 ** 100:
         raise ValueError("temperature must be in [2^-100, 2^100], got %r" % (temperature,))
     d.temperature = temperature
     d.logits, d.teacher_items, d.teacher_logits = logits.data_ptr(), teacher_items.data_ptr(), teacher_logits.data_ptr()
@@ -230,7 +238,7 @@ def _distill_outputs(d, logits, grad_loss):
     if torch.is_tensor(grad_loss):
         d.grad_loss = _dense("grad_loss", grad_loss, (d.rows,), torch.float32, logits.device).data_ptr()
     else:
-        d.grad_loss_value = grad_loss
+        d.grad_loss_value = _number("grad_loss", grad_loss)
     grad = torch.empty(d.rows, d.v, dtype=logits.dtype, device=logits.device)
     d.grad, d.grad_ld = grad.data_ptr(), d.v
     return grad

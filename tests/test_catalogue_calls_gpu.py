@@ -68,3 +68,24 @@ def test_masks_and_settings_belong_to_the_users_asked_for(monkeypatch):
     for kw in (dict(mask=mask[:1]), dict(temperature=t[:1]), dict(top_p=2.0)):   # (no user: still checked)
         with pytest.raises(ValueError):
             eng.sample_items(users[:0], u[:0], **kw)
+
+
+def test_settings_that_are_no_numbers():
+    x, u = torch.zeros(3, 10, device="cuda"), torch.zeros(3, device="cuda")
+    it, y = torch.zeros(3, 1, dtype=torch.int32, device="cuda"), torch.zeros(3, 1, device="cuda")
+    bad = [lambda: C.sample_items(x, u, top_k=2.5), lambda: C.sample_items(x, u, top_k="2"),
+           lambda: C.sample_items(x, u, top_k=None), lambda: C.sample_items(x, u, temperature="1"),
+           lambda: C.sample_items(x, u, temperature=None), lambda: C.sample_items(x, u, top_p=[0.5, 0.5, 0.5]),
+           lambda: C.sample_items(x, u, min_p=1j), lambda: C.sample_items(x, u, temperature=np.ones(3)),
+           lambda: C.distill_loss(x, it, y, temperature="1"), lambda: C.distill_loss(x, it, y, temperature=None),
+           lambda: C.distill_loss(x, it, y, temperature=torch.ones(3, device="cuda")),
+           lambda: C.distill_loss_grad(x, it, y, "1"), lambda: C.distill_loss_grad(x, it, y, None),
+           lambda: C.distill_loss_grad(x, it, y, [1.0, 1.0, 1.0])]
+    for f in bad:
+        with pytest.raises(ValueError):
+            f()
+    # numbers of numpy are numbers
+    a = C.sample_items(x, u, temperature=np.float32(0.5), top_k=np.int64(3), top_p=np.float64(0.9))
+    b = C.sample_items(x, u, temperature=0.5, top_k=3, top_p=0.9)
+    assert torch.equal(a[0], b[0]) and torch.equal(a[1], b[1])
+    assert torch.equal(C.distill_loss_grad(x, it, y, np.float32(2))[1], C.distill_loss_grad(x, it, y, 2)[1])
