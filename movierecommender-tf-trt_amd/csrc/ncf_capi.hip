@@ -1516,7 +1516,8 @@ int ncf_quantize_blocks(const void* x, int32_t dtype, int64_t rows, int64_t cols
     if (int r = check_matrix("x", x, rows, cols, ld)) return r;
     if (int r = check_output("q", q, rows, cols, q_ld)) return r;
     if (!scale) return fail(NCF_EINVAL, "scale is NULL");
-    if ((rows + 127) / 128 > INT32_MAX / ((cols + 127) / 128))
+    // (a tile takes a workgroup of 256: 2^24 of them are more threads than a launch counts)
+    if ((rows + 127) / 128 > (tile ? (1 << 24) - 1 : INT32_MAX) / ((cols + 127) / 128))
         return fail(NCF_EINVAL, "%lld x %lld is too large a matrix", (long long)rows, (long long)cols);
     return hip_check(ncf::launch_quantize(x, dtype, rows, (int)cols, ld, tile != 0, static_cast<uint8_t*>(q), q_ld,
                                           scale, (hipStream_t)stream),
@@ -1562,7 +1563,7 @@ int ncf_draw_items(const ncf_draw_t* d, void* stream) {
     if (d->mask)
         if (int r = check_matrix("mask", d->mask, d->rows, d->n, d->mask_ld)) return r;
     if (!d->u || !d->items || !d->probs) return fail(NCF_EINVAL, "NULL device pointer");
-    if (ncf::draw_blocks(*d) > INT32_MAX || d->draws > INT32_MAX)
+    if (ncf::draw_count(*d) > INT32_MAX || d->draws > INT32_MAX)
         return fail(NCF_EINVAL, "%lld rows of %lld draws are too many", (long long)d->rows, (long long)d->draws);
     size_t need = 0;
     if (int r = ncf_draw_workspace_size(d->rows, d->n, &need)) return r;
@@ -1575,7 +1576,7 @@ int ncf_distill_workspace_size(int64_t rows, int64_t v, size_t* bytes) {
     if (!bytes) return fail(NCF_EINVAL, "bytes is NULL");
     if (rows < 0 || v < 1 || v > INT32_MAX - 128)
         return fail(NCF_EINVAL, "no workspace for %lld rows of %lld items", (long long)rows, (long long)v);
-    if (ncf::distill_blocks(rows, (int)v) > INT32_MAX)
+    if (ncf::distill_chunks(rows, (int)v) > INT32_MAX)
         return fail(NCF_EINVAL, "%lld rows of %lld items are too many", (long long)rows, (long long)v);
     *bytes = ncf::distill_workspace(rows, (int)v);
     return 0;

@@ -21,6 +21,7 @@
 //
 // The reference trains on labels alone (binary cross-entropy, movierec/model.py:213-214).
 
+#include <algorithm>
 #include <cmath>
 
 #include "ncf_common.h"
@@ -786,13 +787,20 @@ static DistArgs dist_args(const ncf_distill_t& c, void* ws) {
 constexpr int64_t kRowMost = 512 * 56;
 static bool by_row(int64_t v, int64_t k) { return v <= kRowMost || (v <= 2 * kRowMost && k <= kWaveList); }
 
+// Rows of one launch at most: HIP counts a launch's threads in 32 bits, and 2^21 workgroups have up to 2^31.  More
+// rows go in several launches, one behind the other, that share the workspace.
+static int64_t launch_rows(int64_t v) {
+    return std::max<int64_t>(1, ((int64_t)1 << 21) / ((v + kDistChunk - 1) / kDistChunk));
+}
+
 // for the chunks' sums and, behind them, the state where the caller takes none
 size_t distill_workspace(int64_t rows, int v) {
     if (v <= kRowMost) return 0;
+    rows = std::min(rows, launch_rows(v));
     const size_t n = (size_t)rows * ((v + kDistChunk - 1) / kDistChunk);
     return n * (sizeof(double2) + sizeof(float2)) + (size_t)rows * kState * sizeof(double);
 }
-int64_t distill_blocks(int64_t rows, int v) {
+int64_t distill_chunks(int64_t rows, int v) {
     const int64_t c = (v + kDistChunk - 1) / kDistChunk;
     return rows > INT64_MAX / c ? INT64_MAX : rows * c;
 }
@@ -836,11 +844,26 @@ static hipError_t distill_t(const DistArgs& a, bool forward, bool backward, hipS
 }
 
 hipError_t launch_distill(const ncf_distill_t& c, void* ws, bool forward, bool backward, hipStream_t st) {
-    if (c.rows <= 0) return hipSuccess;
-    const DistArgs a = dist_args(c, ws);
-    if (c.dtype == NCF_F32) return distill_t<float>(a, forward, backward, st);
-    if (c.dtype == NCF_BF16) return distill_t<__bf16>(a, forward, backward, st);
-    return distill_t<_Float16>(a, forward, backward, st);
+    const int64_t size = c.dtype == NCF_F32 ? 4 : 2, most = launch_rows(c.v);
+    for (int64_t r = 0; r < c.rows; r += most) {
+        auto from = [&](auto* p, int64_t step) { return p ? p + r * step : nullptr; };
+        ncf_distill_t part = c;
+        part.rows = std::min(c.rows - r, most);
+        part.logits = static_cast<const char*>(c.logits) + r * c.ld * size;
+        part.teacher_items = static_cast<const char*>(c.teacher_items) + r * c.items_ld * (c.items64 ? 8 : 4);
+        part.teacher_logits = c.teacher_logits + r * c.teacher_ld;
+        part.teacher_lse = from(c.teacher_lse, 1);
+        part.grad_loss = from(c.grad_loss, 1);
+        part.loss = from(c.loss, 1);
+        part.state = from(c.state, kState);
+        part.grad = from(static_cast<char*>(c.grad), c.grad_ld * size);
+        const DistArgs a = dist_args(part, ws);
+        hipError_t e = c.dtype == NCF_F32 ? distill_t<float>(a, forward, backward, st)
+                       : c.dtype == NCF_BF16 ? distill_t<__bf16>(a, forward, backward, st)
+                                             : distill_t<_Float16>(a, forward, backward, st);
+        if (e != hipSuccess) return e;
+    }
+    return hipSuccess;
 }
 
 }  // namespace ncf

@@ -20,6 +20,7 @@
 // The reference keeps the best of a list by np.argsort (movierec/trt_client.py:50-57); drawing from
 // the scores is an extension of that ranking.
 
+#include <algorithm>
 #include <cmath>
 
 #include "ncf_common.h"
@@ -1317,12 +1318,12 @@ __global__ __launch_bounds__(kLongThreads) void k_long_weigh(LongArgs l) {
     });
 }
 
-// A draw of a row: the segment in which the running sum passes the target, then the item in it.
+// A draw of a row: the segment in which the running sum passes the target, then the item in it; the draws from `first` on.
 template <typename T>
-__global__ __launch_bounds__(kLongThreads) void k_long_draw(LongArgs l) {
+__global__ __launch_bounds__(kLongThreads) void k_long_draw(LongArgs l, int64_t first) {
     __shared__ LongShared s;
     constexpr int V = Elem<T>::kVec;
-    const int64_t o = blockIdx.x, r = o / l.a.draws;
+    const int64_t o = first + blockIdx.x, r = o / l.a.draws;
     const int tid = threadIdx.x, lane = tid & 63;
     const RowSettings set = row_settings(l.a, r);
     const Bins bins = long_bins(l, r);
@@ -1442,12 +1443,15 @@ static LongLayout long_layout(int64_t rows, int64_t n, int vec) {
 
 constexpr int kRowMost = 512 * 56;   // the longest row that two workgroups a CU hold; behind it one of 1,024 does
 
+// Workgroups of one launch at most: HIP counts a launch's threads in 32 bits, and 2^21 workgroups have up to 2^31.
+// More rows (draws over long rows) go in several launches, one behind the other, that share the workspace.
+constexpr int64_t kLaunchMost = (int64_t)1 << 21;
+
 size_t draw_workspace(int64_t rows, int64_t n) {
-    return rows > 0 && n > kRowMost ? long_layout(rows, n, Elem<float>::kVec).total : 0;
+    return rows > 0 && n > kRowMost ? long_layout(std::min(rows, kLaunchMost), n, Elem<float>::kVec).total : 0;
 }
-int64_t draw_blocks(const ncf_draw_t& d) {
-    const int64_t draws = d.rows > INT64_MAX / (d.draws > 0 ? d.draws : 1) ? INT64_MAX : d.rows * d.draws;
-    return draws > d.rows ? draws : d.rows;   // (parts only where rows are few)
+int64_t draw_count(const ncf_draw_t& d) {
+    return d.rows > INT64_MAX / (d.draws > 0 ? d.draws : 1) ? INT64_MAX : d.rows * d.draws;
 }
 
 template <typename T>
@@ -1481,7 +1485,9 @@ static void draw_long(const DrawArgs& a, void* ws, bool may_k, bool may_p, hipSt
         launch(k_long_resolve<T, true>, rows, kResolveThreads, 0, st, l);
     }
     launch(k_long_weigh<T>, grid, kLongThreads, 0, st, l);
-    launch(k_long_draw<T>, dim3((unsigned)(a.rows * a.draws)), kLongThreads, 0, st, l);
+    const int64_t draws = a.rows * a.draws;
+    for (int64_t o = 0; o < draws; o += kLaunchMost)
+        launch(k_long_draw<T>, dim3((unsigned)std::min(draws - o, kLaunchMost)), kLongThreads, 0, st, l, o);
 }
 
 // The smallest workgroup that holds a row, and the next one (us for 4,096 rows, top-50, top-p 0.9): 500 items 15.2
@@ -1527,10 +1533,26 @@ hipError_t launch_draw(const ncf_draw_t& c, hipStream_t st) {
     // which cuts some row may ask for
     const bool greedy = c.temperature_rows || !(c.temperature > 0.0) || c.top_p_rows || !(c.top_p > 0.0);
     const bool may_k = c.top_k_rows || c.top_k > 0 || greedy, may_p = c.top_p_rows || c.top_p < 1.0;
-    if (c.dtype == NCF_F32) draw_t<float>(a, c.ws, may_k, may_p, st);
-    else if (c.dtype == NCF_BF16) draw_t<__bf16>(a, c.ws, may_k, may_p, st);
-    else draw_t<_Float16>(a, c.ws, may_k, may_p, st);
-    return hipGetLastError();
+    const DrawArgs all = a;
+    for (int64_t r = 0; r < all.rows; r += kLaunchMost) {
+        auto from = [&](auto* p, int64_t step) { return p ? p + r * step : nullptr; };
+        a.rows = std::min(all.rows - r, kLaunchMost);
+        a.logits = static_cast<const char*>(all.logits) + r * all.ld * (c.dtype == NCF_F32 ? 4 : 2);
+        a.mask = from(all.mask, all.mask_ld);
+        a.u = from(all.u, all.draws);
+        a.u32 = from(all.u32, all.draws);
+        a.temperature = from(all.temperature, 1);
+        a.top_k = from(all.top_k, 1);
+        a.top_p = from(all.top_p, 1);
+        a.min_p = from(all.min_p, 1);
+        a.items = all.items + r * all.draws;
+        a.probs = all.probs + r * all.draws;
+        if (c.dtype == NCF_F32) draw_t<float>(a, c.ws, may_k, may_p, st);
+        else if (c.dtype == NCF_BF16) draw_t<__bf16>(a, c.ws, may_k, may_p, st);
+        else draw_t<_Float16>(a, c.ws, may_k, may_p, st);
+        if (hipError_t e = hipGetLastError()) return e;
+    }
+    return hipSuccess;
 }
 
 }  // namespace ncf

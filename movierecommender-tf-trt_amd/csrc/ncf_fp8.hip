@@ -775,10 +775,17 @@ hipError_t launch_matmul_blocks(const uint8_t* a, int64_t lda, const float* sa, 
                                 const float* sb, int b_tile, const float* bias, int bias_step, int64_t m, int64_t n,
                                 int k, int out_dtype, void* y, int64_t ldy, hipStream_t st) {
     if (m <= 0 || n <= 0) return hipSuccess;
-    MmArgs p{a, b, sa, sb, bias, y, lda, ldb, ldy, m, n, k, (k + kScaleBlock - 1) / kScaleBlock, b_tile, bias_step, 0, 0};
-    if (out_dtype == NCF_F32) return mm_t<float>(p, st);
-    if (out_dtype == NCF_BF16) return mm_t<__bf16>(p, st);
-    return mm_t<_Float16>(p, st);
+    const int kb = (k + kScaleBlock - 1) / kScaleBlock, size = out_dtype == NCF_F32 ? 4 : 2;
+    // (HIP counts a launch's threads in 32 bits: 2^29 columns by tiles of 16 a wave are 2^31)
+    constexpr int64_t most = (int64_t)1 << 29;
+    for (int64_t c = 0; c < n; c += most) {
+        MmArgs p{a, b + c * ldb, sa, sb + (b_tile ? c / kScaleBlock : c) * kb, bias ? bias + c * bias_step : nullptr,
+                 static_cast<char*>(y) + c * size, lda, ldb, ldy, m, std::min(n - c, most), k, kb, b_tile, bias_step, 0, 0};
+        hipError_t e = out_dtype == NCF_F32 ? mm_t<float>(p, st)
+                       : out_dtype == NCF_BF16 ? mm_t<__bf16>(p, st) : mm_t<_Float16>(p, st);
+        if (e != hipSuccess) return e;
+    }
+    return hipSuccess;
 }
 
 // ----------------------------------------------------------------------------- GMF-only models

@@ -89,3 +89,61 @@ def test_settings_that_are_no_numbers():
     b = C.sample_items(x, u, temperature=0.5, top_k=3, top_p=0.9)
     assert torch.equal(a[0], b[0]) and torch.equal(a[1], b[1])
     assert torch.equal(C.distill_loss_grad(x, it, y, np.float32(2))[1], C.distill_loss_grad(x, it, y, 2)[1])
+
+
+def test_more_draws_than_workgroups_of_one_launch():
+    """5,000,000 draws of one row of 41,000 items: what a draw gives does not depend on the others."""
+    g = torch.Generator().manual_seed(1)
+    x = torch.randn(1, 41000, generator=g).cuda()
+    u = torch.rand(1, 5000000, generator=g).cuda()
+    items, probs = C.sample_items(x, u, top_k=300, top_p=0.9)
+    pick = torch.cat([torch.arange(0, 5000000, 4999), torch.arange(4999000, 5000000)]).cuda()
+    few = C.sample_items(x, u[:, pick].contiguous(), top_k=300, top_p=0.9)
+    assert torch.equal(items[:, pick], few[0]) and torch.equal(probs[:, pick], few[1])
+    assert int(items.min()) >= 0 and float(probs.min()) > 0
+
+
+def test_more_rows_than_workgroups_of_one_launch():
+    """70,000,000 rows of two items: the same as those rows by themselves, on both sides of every 2^21st."""
+    rows = 70000000
+    x = torch.randn(rows, 2, device="cuda", dtype=torch.bfloat16)
+    u = torch.rand(rows, device="cuda")
+    k = torch.randint(0, 3, (rows,), device="cuda", dtype=torch.int32)
+    at = torch.cat([torch.arange(0, rows, 2 ** 21)[:, None] + torch.arange(-3, 4), torch.arange(rows - 7, rows)[None]])
+    at = at[(at >= 0) & (at < rows)].cuda()
+    items, probs = C.sample_items(x, u, top_k=k)
+    few = C.sample_items(x[at], u[at], top_k=k[at])
+    assert torch.equal(items[at], few[0]) and torch.equal(probs[at], few[1])
+    assert int(items.min()) == 0 and int(items.max()) == 1
+    del items, probs
+    it = torch.randint(-1, 2, (rows, 1), device="cuda", dtype=torch.int32)
+    y = torch.randn(rows, 1, device="cuda")
+    lse = y.view(-1) + 0.5
+    loss, grad = C.distill_loss_grad(x, it, y, teacher_lse=lse)
+    few = C.distill_loss_grad(x[at], it[at], y[at], teacher_lse=lse[at])
+    assert torch.equal(loss[at], few[0]) and torch.equal(grad[at], few[1])
+    assert torch.isfinite(loss).all() and torch.isfinite(grad).all()
+    del loss, grad
+    loss, state = C.distill_loss(x, it, y, teacher_lse=lse)
+    few = C.distill_loss(x[at], it[at], y[at], teacher_lse=lse[at])
+    assert torch.equal(loss[at], few[0])
+    grad = C.distill_grad(x, it, y, state, teacher_lse=lse)
+    assert torch.equal(grad[at], C.distill_grad(x[at], it[at], y[at], few[1], teacher_lse=lse[at]))
+
+
+def test_product_of_more_columns_than_one_launch_takes():
+    """One row by 1,100,000,000 columns of one value: every output is its column's value, exactly."""
+    n = 1100000000
+    b = (torch.arange(n, device="cuda", dtype=torch.int32) % 127).to(torch.uint8).view(n, 1)
+    q = torch.ones(1, 1, device="cuda").to(torch.float8_e4m3fn)
+    scale = torch.ones((n + 127) // 128, 1, device="cuda")
+    scale[-1] = 2.0
+    y = C.matmul_blocks(q, torch.ones(1, 1, device="cuda"), b.view(torch.float8_e4m3fn), scale,
+                        out_dtype=torch.bfloat16).view(-1)
+    value = torch.arange(127, dtype=torch.uint8).view(torch.float8_e4m3fn).float().bfloat16().cuda()
+    for at in range(0, n, 1 << 27):
+        part = slice(at, min(n, at + (1 << 27)))
+        want = value[b.view(-1)[part].long()]
+        if part.stop == n:
+            want[-(n % 128 or 128):] *= 2
+        assert torch.equal(y[part], want), at
