@@ -574,9 +574,12 @@ typedef struct ncf_draw {
     int64_t top_k;
     int32_t* items;             /* [rows][draws] */
     float* probs;               /* [rows][draws] */
-    void* ws;                   /* ncf_draw_workspace_size bytes; may be NULL where that is 0 */
+    void* ws;                   /* ncf_draw_workspace bytes; may be NULL where that is 0 */
     size_t ws_bytes;
 } ncf_draw_t;
+/* ncf_draw_workspace: what this call needs, from its rows, n and dtype alone (rows of up to 40,960 float32 or
+ * 32,768 16-bit logits: nothing).  ncf_draw_workspace_size: enough for rows x n of any type. */
+int ncf_draw_workspace(const ncf_draw_t* draw, size_t* bytes);
 int ncf_draw_workspace_size(int64_t rows, int64_t n, size_t* bytes);
 int ncf_draw_items(const ncf_draw_t* draw, void* stream);
 
@@ -591,7 +594,7 @@ int ncf_draw_items(const ncf_draw_t* draw, void* stream);
  *   ncf_distill_loss       writes loss and state (double[rows][NCF_DISTILL_STATE])
  *   ncf_distill_grad       writes grad from the state of the same inputs (no workspace)
  *   ncf_distill_loss_grad  both (state may be NULL)
- * ws: ncf_distill_workspace_size bytes, NULL where that is 0; nothing persists in it between calls. */
+ * ws: ncf_distill_workspace bytes, NULL where that is 0; nothing persists in it between calls. */
 #define NCF_DISTILL_MAX_K 1024
 #define NCF_DISTILL_STATE 5
 typedef struct ncf_distill {
@@ -611,6 +614,9 @@ typedef struct ncf_distill {
     void* grad;                 /* [rows][v] of dtype, rows grad_ld apart; not the logits' own memory */
     int64_t grad_ld;
 } ncf_distill_t;
+/* ncf_distill_workspace: what this call needs, from its rows, v and k alone (v <= 28,672, or 57,344 with k <= 64:
+ * nothing).  ncf_distill_workspace_size: enough for rows x v and any list. */
+int ncf_distill_workspace(const ncf_distill_t* d, size_t* bytes);
 int ncf_distill_workspace_size(int64_t rows, int64_t v, size_t* bytes);
 int ncf_distill_loss(const ncf_distill_t* d, void* ws, size_t ws_bytes, void* stream);
 int ncf_distill_grad(const ncf_distill_t* d, void* stream);

@@ -1549,7 +1549,15 @@ int ncf_draw_workspace_size(int64_t rows, int64_t n, size_t* bytes) {
     if (!bytes) return fail(NCF_EINVAL, "bytes is NULL");
     if (rows < 0 || rows > INT32_MAX || n < 1 || n > INT32_MAX - 4096)   // (whole segments of items fit 32 bits)
         return fail(NCF_EINVAL, "no workspace for %lld rows of %lld items", (long long)rows, (long long)n);
-    *bytes = ncf::draw_workspace(rows, n);
+    *bytes = ncf::draw_workspace(rows, n, 2);   // (16-bit rows are long ones first)
+    return 0;
+}
+
+int ncf_draw_workspace(const ncf_draw_t* d, size_t* bytes) {
+    if (!d) return fail(NCF_EINVAL, "draw is NULL");
+    if (int r = check_dtype(d->dtype)) return r;
+    if (int r = ncf_draw_workspace_size(d->rows, d->n, bytes)) return r;
+    *bytes = ncf::draw_workspace(d->rows, d->n, d->dtype == NCF_F32 ? 4 : 2);
     return 0;
 }
 
@@ -1566,7 +1574,7 @@ int ncf_draw_items(const ncf_draw_t* d, void* stream) {
     if (ncf::draw_count(*d) > INT32_MAX || d->draws > INT32_MAX)
         return fail(NCF_EINVAL, "%lld rows of %lld draws are too many", (long long)d->rows, (long long)d->draws);
     size_t need = 0;
-    if (int r = ncf_draw_workspace_size(d->rows, d->n, &need)) return r;
+    if (int r = ncf_draw_workspace(d, &need)) return r;
     if (need && (!d->ws || d->ws_bytes < need))
         return fail(NCF_EINVAL, "workspace of %zu bytes, need %zu", d->ws ? d->ws_bytes : (size_t)0, need);
     return hip_check(ncf::launch_draw(*d, (hipStream_t)stream), "ncf_draw_items");
@@ -1578,7 +1586,14 @@ int ncf_distill_workspace_size(int64_t rows, int64_t v, size_t* bytes) {
         return fail(NCF_EINVAL, "no workspace for %lld rows of %lld items", (long long)rows, (long long)v);
     if (ncf::distill_chunks(rows, (int)v) > INT32_MAX)
         return fail(NCF_EINVAL, "%lld rows of %lld items are too many", (long long)rows, (long long)v);
-    *bytes = ncf::distill_workspace(rows, (int)v);
+    *bytes = ncf::distill_workspace(rows, (int)v, NCF_DISTILL_MAX_K);   // (long lists need it first)
+    return 0;
+}
+
+int ncf_distill_workspace(const ncf_distill_t* d, size_t* bytes) {
+    if (!d) return fail(NCF_EINVAL, "distill is NULL");
+    if (int r = ncf_distill_workspace_size(d->rows, d->v, bytes)) return r;
+    *bytes = ncf::distill_workspace(d->rows, (int)d->v, d->k);
     return 0;
 }
 
@@ -1596,7 +1611,7 @@ static int distill(const ncf_distill_t* d, void* ws, size_t ws_bytes, bool forwa
         return fail(NCF_EINVAL, "temperature must be in [2^-100, 2^100], got %g", d->temperature);
     if ((!d->state && forward != backward) || (forward && !d->loss)) return fail(NCF_EINVAL, "NULL device pointer");
     size_t need = 0;
-    if (int r = ncf_distill_workspace_size(d->rows, d->v, &need)) return r;
+    if (int r = ncf_distill_workspace(d, &need)) return r;
     if (forward && need && (!ws || ws_bytes < need))
         return fail(NCF_EINVAL, "workspace of %zu bytes, need %zu", ws ? ws_bytes : (size_t)0, need);
     if (backward)

@@ -794,8 +794,8 @@ static int64_t launch_rows(int64_t v) {
 }
 
 // for the chunks' sums and, behind them, the state where the caller takes none
-size_t distill_workspace(int64_t rows, int v) {
-    if (v <= kRowMost) return 0;
+size_t distill_workspace(int64_t rows, int v, int64_t k) {
+    if (by_row(v, k)) return 0;
     rows = std::min(rows, launch_rows(v));
     const size_t n = (size_t)rows * ((v + kDistChunk - 1) / kDistChunk);
     return n * (sizeof(double2) + sizeof(float2)) + (size_t)rows * kState * sizeof(double);

@@ -1441,14 +1441,16 @@ static LongLayout long_layout(int64_t rows, int64_t n, int vec) {
     return l;
 }
 
-constexpr int kRowMost = 512 * 56;   // the longest row that two workgroups a CU hold; behind it one of 1,024 does
+constexpr int kRowMost = 512 * 56;   // the longest row that two workgroups a CU hold; behind it one of 1,024 does,
+// up to so many logits a thread (nothing spilled)
+constexpr int items_most(size_t size) { return size == 4 ? 40 : 32; }
 
 // Workgroups of one launch at most: HIP counts a launch's threads in 32 bits, and 2^21 workgroups have up to 2^31.
 // More rows (draws over long rows) go in several launches, one behind the other, that share the workspace.
 constexpr int64_t kLaunchMost = (int64_t)1 << 21;
 
-size_t draw_workspace(int64_t rows, int64_t n) {
-    return rows > 0 && n > kRowMost ? long_layout(std::min(rows, kLaunchMost), n, Elem<float>::kVec).total : 0;
+size_t draw_workspace(int64_t rows, int64_t n, size_t size) {
+    return rows > 0 && n > 1024 * items_most(size) ? long_layout(std::min(rows, kLaunchMost), n, Elem<float>::kVec).total : 0;
 }
 int64_t draw_count(const ncf_draw_t& d) {
     return d.rows > INT64_MAX / (d.draws > 0 ? d.draws : 1) ? INT64_MAX : d.rows * d.draws;
@@ -1495,7 +1497,7 @@ static void draw_long(const DrawArgs& a, void* ws, bool may_k, bool may_p, hipSt
 // of 27,278 17.3 and 59.5, 2,048 88 and 408; one of 40,000 18.9 and 57.5, 1,024 84 and 269 (fp32).
 template <typename T>
 static void draw_t(const DrawArgs& a, void* ws, bool may_k, bool may_p, hipStream_t st) {
-    constexpr int kMost = sizeof(T) == 4 ? 40 : 32;   // (nothing spilled)
+    constexpr int kMost = items_most(sizeof(T));
     const dim3 grid((unsigned)a.rows);
     if (a.n <= 64 * 8) launch(k_draw_row<T, 64, 8>, grid, 64, 0, st, a);
     else if (a.n <= 64 * 32) launch(k_draw_row<T, 64, 32>, grid, 64, 0, st, a);

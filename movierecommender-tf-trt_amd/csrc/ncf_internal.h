@@ -1013,9 +1013,9 @@ hipError_t launch_gmf_logits(const ncf_shape_t& s, void* ws, const float* emb, c
 
 // drawing items (ncf_draw.hip), distillation (ncf_distill.hip)
 hipError_t launch_draw(const ncf_draw_t& d, hipStream_t st);
-size_t draw_workspace(int64_t rows, int64_t n);
+size_t draw_workspace(int64_t rows, int64_t n, size_t size);  // logits of `size` bytes
 int64_t draw_count(const ncf_draw_t& d);  // rows * draws, held at INT64_MAX
-size_t distill_workspace(int64_t rows, int v);
+size_t distill_workspace(int64_t rows, int v, int64_t k);
 int64_t distill_chunks(int64_t rows, int v);  // of all rows, held at INT64_MAX
 hipError_t launch_distill(const ncf_distill_t& d, void* ws, bool forward, bool backward, hipStream_t st);
 

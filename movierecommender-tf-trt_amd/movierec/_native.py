@@ -159,8 +159,10 @@ _SIGNATURES = {
     "ncf_quantize_blocks": (ctypes.c_int, [_vp, _i32, _i64, _i64, _i64, _i32, _vp, _i64, _vp, _vp]),
     "ncf_matmul_blocks": (ctypes.c_int, [_vp, _i64, _vp, _vp, _i64, _vp, _i32, _vp, _i64, _i64, _i64, _i32, _vp,
                                          _i64, _vp]),
+    "ncf_draw_workspace": (ctypes.c_int, [_P(NcfDraw), _P(ctypes.c_size_t)]),
     "ncf_draw_workspace_size": (ctypes.c_int, [_i64, _i64, _P(ctypes.c_size_t)]),
     "ncf_draw_items": (ctypes.c_int, [_P(NcfDraw), _vp]),
+    "ncf_distill_workspace": (ctypes.c_int, [_P(NcfDistill), _P(ctypes.c_size_t)]),
     "ncf_distill_workspace_size": (ctypes.c_int, [_i64, _i64, _P(ctypes.c_size_t)]),
     "ncf_distill_loss": (ctypes.c_int, [_P(NcfDistill), _vp, ctypes.c_size_t, _vp]),
     "ncf_distill_grad": (ctypes.c_int, [_P(NcfDistill), _vp]),

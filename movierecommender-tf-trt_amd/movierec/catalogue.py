@@ -73,10 +73,10 @@ def _call(fn, device, *args):
             N.check(fn(*args, N.stream_handle(idx)))
 
 
-def _workspace(size_fn, rows, cols, device):
-    """Scratch for a call over rows x cols (None where it needs none)."""
+def _workspace(size_fn, d, device):
+    """Scratch for the call that struct ``d`` describes (None where it needs none)."""
     nbytes = ctypes.c_size_t()
-    N.check(size_fn(rows, cols, ctypes.byref(nbytes)))
+    N.check(size_fn(ctypes.byref(d), ctypes.byref(nbytes)))
     return torch.empty(nbytes.value, dtype=torch.uint8, device=device) if nbytes.value else None
 
 
@@ -197,7 +197,7 @@ def sample_items(logits, u, temperature=1.0, top_k=0, top_p=1.0, min_p=0.0, mask
         d.logits, d.rows, d.n, d.ld = logits.data_ptr(), rows, n, ld
         d.u, d.u64 = u.data_ptr(), 1 if u.dtype == torch.float64 else 0
         d.items, d.probs = items.data_ptr(), probs.data_ptr()
-        ws = _workspace(N.lib().ncf_draw_workspace_size, rows, n, dev)
+        ws = _workspace(N.lib().ncf_draw_workspace, d, dev)
         if ws is not None:
             d.ws, d.ws_bytes = ws.data_ptr(), ws.numel()
         _call(N.lib().ncf_draw_items, dev, ctypes.byref(d))
@@ -261,7 +261,7 @@ def distill_loss(logits, teacher_items, teacher_logits, temperature=1.0, teacher
     dev = logits.device
     loss = torch.empty(d.rows, dtype=torch.float32, device=dev)
     state = torch.empty(d.rows, N.NCF_DISTILL_STATE, dtype=torch.float64, device=dev)
-    ws = _workspace(N.lib().ncf_distill_workspace_size, d.rows, d.v, dev)
+    ws = _workspace(N.lib().ncf_distill_workspace, d, dev)
     d.loss, d.state = loss.data_ptr(), state.data_ptr()
     if d.rows:
         _call(N.lib().ncf_distill_loss, dev, ctypes.byref(d), N.ptr(ws), ws.numel() if ws is not None else 0)
@@ -287,7 +287,7 @@ def distill_loss_grad(logits, teacher_items, teacher_logits, grad_loss=1.0, temp
     dev = logits.device
     loss = torch.empty(d.rows, dtype=torch.float32, device=dev)
     grad = _distill_outputs(d, logits, grad_loss)
-    ws = _workspace(N.lib().ncf_distill_workspace_size, d.rows, d.v, dev)
+    ws = _workspace(N.lib().ncf_distill_workspace, d, dev)
     d.loss = loss.data_ptr()
     if d.rows:
         _call(N.lib().ncf_distill_loss_grad, dev, ctypes.byref(d), N.ptr(ws), ws.numel() if ws is not None else 0)

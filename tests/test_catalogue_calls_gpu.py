@@ -147,3 +147,23 @@ def test_product_of_more_columns_than_one_launch_takes():
         if part.stop == n:
             want[-(n % 128 or 128):] *= 2
         assert torch.equal(y[part], want), at
+
+
+def test_scratch_is_what_the_rows_need():
+    """Rows that a workgroup holds ask for no scratch: beside its outputs a call allocates next to nothing."""
+    def grown(call):
+        torch.cuda.synchronize()
+        torch.cuda.empty_cache()
+        before = torch.cuda.memory_allocated()
+        torch.cuda.reset_peak_memory_stats()
+        out = call()
+        torch.cuda.synchronize()
+        return torch.cuda.max_memory_allocated() - before - sum(o.numel() * o.element_size() for o in out)
+
+    u = torch.rand(500, device="cuda")
+    for n, dtype in ((32768, torch.bfloat16), (40960, torch.float32)):
+        x = torch.randn(500, n, device="cuda").to(dtype)
+        assert grown(lambda: C.sample_items(x, u, top_k=50)) < 1 << 16
+    x = torch.randn(500, 50000, device="cuda")
+    it, y = torch.zeros(500, 64, dtype=torch.int32, device="cuda"), torch.zeros(500, 64, device="cuda")
+    assert grown(lambda: C.distill_loss(x, it, y)) < 1 << 12      # (outputs are rounded up to 512 bytes)
