@@ -554,8 +554,8 @@ int ncf_matmul_blocks(const void* a, int64_t a_ld, const float* a_scale, const v
  *   5. draw d: the first item, in the order of the ids, at which the running sum of the weights passes
  *      u[row][d] times their total (u outside [0, 1): the nearest end)
  * items[row][d] = that item, probs[row][d] = its share of the total; -1 and 0 where no item is allowed.
- * Weights are summed as integers in units of 2^-min(51, 62 - ceil(log2 n)): a result does not depend
- * on the launch.  temperature / top_k / top_p / min_p: one value, or, where the pointer is not NULL,
+ * Weights are summed as integers in units of 2^-min(51, 62 - ceil(log2 n)), an item of less than half a unit
+ * not at all: a result does not depend on the launch.  temperature / top_k / top_p / min_p: one value, or, where the pointer is not NULL,
  * one per row (float32, top_k int32).  u is float32 (u64 == 0) or float64. */
 typedef struct ncf_draw {
     const void* logits;
