@@ -35,6 +35,4 @@ __device__ __forceinline__ vu32x4 load16(const void* p) {
     return *reinterpret_cast<const u*>(p);
 }
 
-inline bool dtype_ok(int d) { return d == NCF_F32 || d == NCF_BF16 || d == NCF_F16; }
-
 }  // namespace ncf
