@@ -1693,6 +1693,8 @@ int ncf_score_logits(const ncf_shape_t* s, const ncf_model_t* model, const int32
         if (e != hipSuccess) return hip_check(e, "score preparation");
         return hip_check(ncf::launch_score_logits(*s, L, ws, n, logits, st), "score logits");
     }
+    if (s->num_layers == 0)
+        return hip_check(ncf::launch_gmf_logits_fp32(*s, model->emb, model->mlp, users, n, logits, st), "GMF logits");
     const int64_t I = s->num_items;
     if (I > ncf::kMaxBatch)
         return fail(NCF_EINVAL, "the fp32 scorer handles catalogues of up to %lld items", (long long)ncf::kMaxBatch);

@@ -1011,6 +1011,10 @@ GmfLayout gmf_layout(const ncf_shape_t& s, int64_t n);
 hipError_t launch_gmf_logits(const ncf_shape_t& s, void* ws, const float* emb, const float* mlp, const int32_t* users,
                              int64_t n, float* logits, hipStream_t st);
 
+// the same in fp32 (ncf_generic.hip), the bits of the fp32 forward
+hipError_t launch_gmf_logits_fp32(const ncf_shape_t& s, const float* emb, const float* mlp, const int32_t* users,
+                                  int64_t n, float* logits, hipStream_t st);
+
 // drawing items (ncf_draw.hip), distillation (ncf_distill.hip)
 hipError_t launch_draw(const ncf_draw_t& d, hipStream_t st);
 size_t draw_workspace(int64_t rows, int64_t n, size_t size);  // logits of `size` bytes

@@ -447,7 +447,7 @@ class NCFEngine(object):
         """The logits of ``users`` for every item, float32 (n, num_items); a user outside the table
         gives a row of NaN.  precision "fp16" (4-layer models of ``score_topk``'s MFMA scorer), "fp8"
         (GMF-only models: the product of their factors in 8 bits with block scales,
-        ``catalogue.matmul_blocks``), "fp32" (any shape, slow); None: the first of these that the
+        ``catalogue.matmul_blocks``), "fp32" (any shape; slow for models with layers); None: the first of these that the
         shape has.  (``sample_items`` takes 8 bits only when asked to.)"""
         codes = {"fp16": N.NCF_SCORE_FP16, "fp8": N.NCF_SCORE_FP8, "fp32": N.NCF_SCORE_FP32}
         L = N.lib()

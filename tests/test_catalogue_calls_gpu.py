@@ -167,3 +167,17 @@ def test_scratch_is_what_the_rows_need():
     x = torch.randn(500, 50000, device="cuda")
     it, y = torch.zeros(500, 64, dtype=torch.int32, device="cuda"), torch.zeros(500, 64, device="cuda")
     assert grown(lambda: C.distill_loss(x, it, y)) < 1 << 12      # (outputs are rounded up to 512 bytes)
+
+
+@pytest.mark.parametrize("dims", [(70, 130, [], 12), (200, 1, [], 64), (3, 2111, [], 130), (129, 64, [], 16),
+                                  (65, 65, [], 1)], ids=str)
+def test_fp32_logits_of_gmf_models_are_the_forwards(dims):
+    """Every item's logit in fp32 has the bits of the pair's own forward (the same roundings in the same order)."""
+    shape = O.NCFShape(*dims)
+    eng = _engine(shape, gmf_weights(shape, 9))
+    users = torch.from_numpy(np.random.RandomState(3).permutation(dims[0] + 2).astype(np.int32) - 1).cuda()
+    z = eng.score_logits(users, precision="fp32")
+    pairs = eng.predict_logits(users.view(-1, 1).expand(-1, dims[1]), torch.arange(dims[1]).repeat(users.numel()))
+    assert torch.equal(torch.nan_to_num(z.view(-1), nan=77.0), torch.nan_to_num(pairs, nan=77.0))
+    known = (users >= 0) & (users < dims[0])
+    assert torch.equal(torch.isnan(z).all(1), ~known) and torch.equal(torch.isnan(z).any(1), ~known)
