@@ -746,7 +746,9 @@ static hipError_t mm_tile(MmArgs p, hipStream_t st) {
     return hipGetLastError();
 }
 
-// Which kernel, and both sides of each choice (us):
+// Which kernel, and both sides of each choice (us); k_mm_tile also needs rows that start at multiples of 16 bytes (as
+// quantize_blocks lays them out; 4,096 x 4,096 x 1,000 fp32 61, at 1,000 bytes a row 132 by k_mm_direct, 8,192 x 4,096 x
+// 4,095 309 and 2,065):
 //   more than 64 tiles of 256 x 256, k > 128: k_mm_tile (2,304 x 2,304 x 1,024, 81 tiles: fp32 45, so 58 by k_mm_direct;
 //     2,048 x 2,048, 64 tiles: 44, so 29; 4,096 x 4,096 x 144: 22, so 24)
 //   k <= 128 and 1,024 waves of 64 x 64: k_mm_short (4,096 x 4,096 x 64 fp32 15, so 36; 2,048 x 1,682: both 10.5)
