@@ -499,6 +499,8 @@ class MovierecModel(object):
             raise ValueError("x must be [users (b,), items (b, c)], found {} and {}".format(users.shape, items.shape))
         if not 0 < temperature < math.inf:
             raise ValueError("temperature must be positive and finite, found {}".format(temperature))
+        if int(top) < 1:
+            raise ValueError("top must be >= 1, found {}".format(top))
         b, c = items.shape
         for m in (self, teacher):
             m.model.engine.check_ids(users, items)

@@ -181,3 +181,12 @@ def test_fp32_logits_of_gmf_models_are_the_forwards(dims):
     assert torch.equal(torch.nan_to_num(z.view(-1), nan=77.0), torch.nan_to_num(pairs, nan=77.0))
     known = (users >= 0) & (users < dims[0])
     assert torch.equal(torch.isnan(z).all(1), ~known) and torch.equal(torch.isnan(z).any(1), ~known)
+
+
+def test_teacher_lists_of_no_length_are_refused(tmp_path):
+    m = model(tmp_path, "t")
+    x = [np.arange(3), np.arange(12).reshape(3, 4)]
+    for top in (0, -1):
+        with pytest.raises(ValueError):
+            m.distill_on_batch(x, m, top=top)
+    assert np.isfinite(m.distill_on_batch(x, m, top=9))      # (more than there are candidates: all)
