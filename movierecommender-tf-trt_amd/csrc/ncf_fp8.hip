@@ -304,8 +304,9 @@ __global__ __launch_bounds__(kBlock) void k_mm_direct(MmArgs p) {
 // operands' steps go straight from memory to LDS (16 bytes a lane), the next while this one is multiplied.
 // In LDS the 16-byte pieces of a row are permuted by the row (piece c at c ^ (row / 2 % 8)), so the 16
 // lanes that read a fragment touch all 64 banks; a lane's fragment is pieces g and g + 4 of its row, in
-// both operands alike.  8,192 x 4,096 x 4,096 with a scale per tile: bf16 out 236 us, 1.16 PFLOP/s, fp32 out 244;
-// bound by the fp16 matrix instructions (a library product of 8,192^3 in bf16 reaches 1.25).
+// both operands alike.  8,192 x 4,096 x 4,096 with a scale per tile: bf16 out 238 us, 1.15 PFLOP/s, fp32 out 244
+// (a library product of 8,192^3 in bf16 reaches 1.25); matrix instructions are busy 44 % of the time, widening and
+// scaled additions beside them.
 
 constexpr int kTile = 256, kTileThreads = 512, kTileWaves = kTileThreads / 64;
 constexpr int kTileMI = 4, kTileNI = 8;   // 16-row, 16-column tiles of a wave
@@ -459,10 +460,9 @@ __global__ __launch_bounds__(kTileThreads, 2) void k_mm_tile(MmArgs p) {
 // registers and goes along the columns, 128 bytes of each row of y at a time, the next columns' operand
 // loaded meanwhile; the workgroup's four waves go along the same columns.  Products pass through a ring of
 // two such pieces in LDS, placed by their address in y, so that every store writes whole, aligned lines of
-// 128 bytes whatever the distance of the rows (8,192 x 27,278 fp32, rows 8 bytes off: 16-byte stores at
-// their own addresses took 100 us of 303).
-// Measured, 8,192 x 27,278 x 64: fp32 175 us (5.1 TB/s written; these stores alone, without a product, take
-// 162), bf16 95-102; rows on their lines (27,264) 167 and 90.
+// 128 bytes whatever the distance of the rows (8,192 x 27,278 fp32, rows 8 bytes off: 308 us with 16-byte stores
+// at their own addresses, 215 so).
+// Measured, 8,192 x 27,278 x 64: fp32 173 us (5.2 TB/s written), bf16 95-102; rows on their lines (27,264) 167 and 90.
 
 constexpr int kShortRows = 32;
 constexpr int kShortWaves = kBlock / 64;
