@@ -1011,7 +1011,7 @@ GmfLayout gmf_layout(const ncf_shape_t& s, int64_t n);
 hipError_t launch_gmf_logits(const ncf_shape_t& s, void* ws, const float* emb, const float* mlp, const int32_t* users,
                              int64_t n, float* logits, hipStream_t st);
 
-// the same in fp32 (ncf_generic.hip), the bits of the fp32 forward
+// the same in fp32, the bits of the fp32 forward
 hipError_t launch_gmf_logits_fp32(const ncf_shape_t& s, const float* emb, const float* mlp, const int32_t* users,
                                   int64_t n, float* logits, hipStream_t st);
 
